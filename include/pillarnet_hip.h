@@ -475,6 +475,72 @@ int pn_points_to_voxel(const float* points, long long n, int feats, const float*
                        int reverse_index, int max_points, int max_voxels, int32_t* grid_map, float* voxels,
                        int32_t* coors, int32_t* num_points);
 
+/* ------------------------------------------------------------------------
+ * The feed-forward block of the RoI heads (det3d/models/roi_heads/roi_ffn_head.py:34-39,101-102, the FC stacks with
+ * Dropout of roi_head_template.py:23-39, the mixers of mlp_layers.py:24-117).  Element types: PN_DTYPE_F32 / BF16;
+ * sums, statistics and accumulators are fp32.  Rows are [rows, cols] with unit column stride; where a row stride (in
+ * elements) is taken it is >= cols, outputs without one are dense.  Empty inputs (0 rows) launch nothing.
+ * ------------------------------------------------------------------------ */
+#define PN_ACT_NONE 0
+#define PN_ACT_RELU 1
+#define PN_ACT_GELU 2  /* x * Phi(x), the erf form */
+
+/* Activation + dropout: y = keep ? act(x) * 65536 / (65536 - threshold) : 0.  An element is kept when its 16 bits of the
+ * counter-based generator reach `threshold` (= round(p * 65536), 0: keep all, 65536: drop all); the generator (Philox4x32-10)
+ * is keyed by rng = {seed, offset} (two uint64 in device memory, read when the kernel runs), `call` (< 65536: the dropout's
+ * number within a pass) and the element's index row * cols + col, so no mask is stored and strides do not matter.
+ * Backward: dx = keep ? g * scale * act'(x) : 0 with the same rng contents; `saved` is x for PN_ACT_GELU, y for PN_ACT_RELU,
+ * NULL for PN_ACT_NONE.  Dropped elements are exactly zero, whatever x or g hold there. */
+int pn_act_dropout_forward(int dtype, const void* x, long long rows, long long cols, long long ldx, int act,
+                           unsigned threshold, const void* rng, unsigned call, void* y, pnStream stream);
+int pn_act_dropout_backward(int dtype, const void* g, const void* saved, long long rows, long long cols, long long ldg,
+                            long long lds, int act, unsigned threshold, const void* rng, unsigned call, void* dx,
+                            pnStream stream);
+/* used = state; state.offset += 1 (both {seed, offset}): one draw per pass, also when the pass is a replayed graph. */
+int pn_dropout_draw(void* state, void* used, pnStream stream);
+
+/* Residual join with the norms around it:
+ *   u = post(branch)   v = dropout(u)   h = round(x + scale * gate * v)   y = act(norm(h))
+ * post: none / layer / rms; norm: none / layer / rms / affine (weight and bias only); a NULL weight is 1, a NULL bias 0.
+ * gate: NULL or [rows / rows_per_gate, cols] (rows_per_gate == rows: one vector for all rows; 1: a gate for each row).
+ * branch == NULL: h is x and is not written.  Weights, biases and gate have type param_dtype. */
+#define PN_NORM_NONE 0
+#define PN_NORM_LAYER 1
+#define PN_NORM_RMS 2
+#define PN_NORM_AFFINE 3
+#define PN_NORM_MAX_COLS 16384
+typedef struct {
+  int32_t dtype, param_dtype, post_kind, norm_kind, act, cols;
+  int64_t rows, rows_per_gate, ldx, ldb;   /* ldb: row stride of the branch */
+  float scale, post_eps, norm_eps;
+  uint32_t threshold, call;                /* dropout of the branch, as pn_act_dropout_forward */
+  const void *rng, *x, *branch, *gate, *post_weight, *post_bias, *norm_weight, *norm_bias;
+} pnResidualNorm;
+/* h [rows, cols] (branch given), y [rows, cols] (norm given), stats [rows][4] fp32 (what the backward pass needs; NULL
+ * while serving). */
+int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* y, float* stats, pnStream stream);
+/* gh, gy: gradients of h and y (either may be NULL).  dx [rows, cols]; dbranch [rows, cols], NULL where the branch enters
+ * as it is (no gate, post norm, dropout, scale 1: its gradient is dx); the parameters' gradients have type param_dtype and
+ * gate's shape for dgate; any may be NULL.  Deterministic: column sums go through chunk sums in the workspace. */
+size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p);
+int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const float* stats, const void* gh, const void* gy,
+                              void* dx, void* dbranch, void* dweight, void* dbias, void* dpost_weight, void* dpost_bias,
+                              void* dgate, void* workspace, size_t workspace_bytes, pnStream stream);
+
+/* Products in 8-bit floating point (e4m3) with a power-of-two scale for each block of 128 along the contraction.
+ * Quantise: block scale 2^e, e the smallest exponent >= -126 with (largest finite magnitude) <= 448 * 2^e; bytes are
+ * x / 2^e rounded to nearest even; infinities and NaN become NaN.
+ *   q  [rows][kp] bytes (kp = cols rounded up to 128, zero padded), q_scale: 32-bit words [ceil(kp / 512)][rows], byte
+ *      b & 3 of word (b >> 2, row) = e + 127 of block b;  qt / qt_scale: the same of the transpose ([cols][mp]).
+ *   block_rows 1: blocks of 1 x 128 (q) and 128 x 1 (qt); 128: one scale for each 128 x 128 tile, in both.
+ *   colsum [ceil(rows / 128)][cols] fp32 or NULL: column sums of the input for pn_fp8_colsum.  q or qt may be NULL. */
+int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q, void* q_scale,
+                    void* qt, void* qt_scale, float* colsum, pnStream stream);
+int pn_fp8_colsum(const float* partial, long long rows, int cols, int out_dtype, void* out, pnStream stream);
+/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) on operands that pn_fp8_quantize laid out (k: the unpadded contraction). */
+int pn_fp8_gemm(const void* x, const void* x_scale, long long m, const void* w, const void* w_scale, int n, int k,
+                const void* bias, int bias_dtype, int act, int out_dtype, void* out, long long ldo, pnStream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,5 +11,5 @@ from .builder import (build_backbone, build_detector, build_head, build_neck,  #
 from .checkpoint import (load_checkpoint, load_state_dict, resume, save_checkpoint,  # noqa: F401
                          save_epoch_checkpoint)
 from .wire import collate_kitti  # noqa: F401
-from . import solver, wire  # noqa: F401
+from . import ffn_ops, solver, wire  # noqa: F401
 from .frame_graph import FrameGraphs  # noqa: F401

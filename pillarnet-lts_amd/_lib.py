@@ -5,7 +5,7 @@ operator in this package goes through `lib()`.
 """
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_longlong, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpillarnet_hip.so")
@@ -13,6 +13,9 @@ LIB_PATH = os.environ.get("PN_LIB_PATH", LIB_PATH)   # tuning: A/B two builds in
 
 PN_MAX_BATCH = 32
 PN_DTYPE_F32, PN_DTYPE_BF16 = 0, 1
+PN_ACT = {"none": 0, "relu": 1, "gelu": 2}
+PN_NORM = {"none": 0, "layer": 1, "rms": 2, "affine": 3}
+PN_NORM_MAX_COLS = 16384
 
 
 class PillarnetHipError(RuntimeError):
@@ -43,6 +46,16 @@ class pnDecodeCommon(ctypes.Structure):
     _fields_ = [
         ("batch", c_int32), ("pillar_size", c_float), ("x_min", c_float), ("y_min", c_float),
         ("has_range", c_int32), ("range", c_float * 6),
+    ]
+
+
+class pnResidualNorm(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("param_dtype", c_int32), ("post_kind", c_int32), ("norm_kind", c_int32), ("act", c_int32),
+        ("cols", c_int32), ("rows", c_int64), ("rows_per_gate", c_int64), ("ldx", c_int64), ("ldb", c_int64),
+        ("scale", c_float), ("post_eps", c_float), ("norm_eps", c_float), ("threshold", c_uint32), ("call", c_uint32),
+        ("rng", c_void_p), ("x", c_void_p), ("branch", c_void_p), ("gate", c_void_p), ("post_weight", c_void_p),
+        ("post_bias", c_void_p), ("norm_weight", c_void_p), ("norm_bias", c_void_p),
     ]
 
 
@@ -127,6 +140,19 @@ SIGNATURES = {
     "pn_merge_sweeps_workspace_bytes": (c_size_t, [c_int]),
     "pn_merge_sweeps": (c_int, [c_void_p, c_int, c_int, POINTER(c_int32), c_int, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "pn_act_dropout_forward": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_longlong, c_int, c_uint32, c_void_p,
+                                       c_uint32, c_void_p, c_void_p]),
+    "pn_act_dropout_backward": (c_int, [c_int, c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong, c_int,
+                                        c_uint32, c_void_p, c_uint32, c_void_p, c_void_p]),
+    "pn_dropout_draw": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "pn_residual_norm_forward": (c_int, [POINTER(pnResidualNorm), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pn_residual_norm_workspace_bytes": (c_size_t, [POINTER(pnResidualNorm)]),
+    "pn_residual_norm_backward": (c_int, [POINTER(pnResidualNorm)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
+    "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p]),
+    "pn_fp8_colsum": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p]),
+    "pn_fp8_gemm": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
+                            c_void_p, c_longlong, c_void_p]),
 }
 
 _lib = None

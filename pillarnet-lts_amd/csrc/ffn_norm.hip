@@ -1,0 +1,525 @@
+// Residual join with the norms on its two sides, gate, scale and dropout:
+//   u = post(f)   v = dropout(u)   h = round(x + scale * gate * v)   y = act(norm(h))
+// post / norm: layer (mean and variance over the row), rms, affine (weight and bias only), none.  One launch per direction
+// instead of up to a dozen; every row is read once and kept in registers between its two norms.
+//
+// Statistics are two-pass (mean, then the mean of squared distances) in fp32 over the registers.  The norm reads h as it is
+// stored, so the backward pass, which reads the stored h again, differentiates exactly what was computed.
+#include "ffn_common.h"
+
+struct NormArgs {
+  pnResidualNorm p;
+  const void *gh, *gy;
+  void *h, *y, *dx, *df;
+  void* dgate_rows;        // backward with a gate for each row: its gradient needs no sum over rows
+  float* stats;            // [rows][4]: mean and factor of the norm, mean and factor of the post norm
+  float* partial;          // backward: [chunks][sums][cols]
+  int chunk_rows;          // rows of one chunk (a multiple of the workgroup's row slots), chunks never span two gates
+  int chunks_per_group;
+  long long group_rows;
+  float keep_scale;
+};
+
+// sums over the L threads that share a row (L <= 64: shuffles; more: one LDS exchange, two buffers so that one barrier is
+// enough).  The order of the additions depends on L alone.
+template <int L, int NT> struct RowSum {
+  float2* lds;             // [2][NT / 64]
+  int turn = 0;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    constexpr int W = L < 64 ? L : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+      a += __shfl_xor(a, o);
+      b += __shfl_xor(b, o);
+    }
+    if (L > 64) {
+      float2* buf = lds + turn * (NT / 64);
+      turn ^= 1;
+      const int wave = threadIdx.x >> 6, first = wave & ~(L / 64 - 1);
+      if ((threadIdx.x & 63) == 0) buf[wave] = make_float2(a, b);
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int i = 0; i < (L >= 64 ? L / 64 : 1); ++i) {
+        const float2 v = buf[first + i];
+        a += v.x;
+        b += v.y;
+      }
+    }
+    return make_float2(a, b);
+  }
+};
+
+__device__ __forceinline__ void load_param(const void* p, int dtype, int col, int n, float (&o)[8], float fill) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = fill;
+  } else if (dtype == PN_DTYPE_F32) {
+    load8(reinterpret_cast<const float*>(p) + col, n, o);
+  } else {
+    load8(reinterpret_cast<const __bf16*>(p) + col, n, o);
+  }
+}
+
+// mean and 1 / sqrt(var + eps) of the row held as v[K][8] (elements from `cols` on are not part of it)
+template <int K, typename Sum>
+__device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, float eps, int cols, int c0, int cstep, Sum& sum) {
+  if (kind != PN_NORM_LAYER && kind != PN_NORM_RMS) return make_float2(0.f, 1.f);
+  float mean = 0.f, s = 0.f;
+  if (kind == PN_NORM_LAYER) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[k][i];
+    mean = sum(s, 0.f).x / (float)cols;
+  }
+  s = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = v[k][i] - mean;
+      if (c0 + k * cstep + i < cols) s = fmaf(d, d, s);
+    }
+  const float var = sum(s, 0.f).x / (float)cols;
+  return make_float2(mean, 1.f / sqrtf(var + eps));
+}
+
+template <typename T, int L, int K, int NT>
+__global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
+  constexpr int SLOTS = NT / L;
+  __shared__ float2 lds[2 * (NT / 64)];
+  RowSum<L, NT> sum{lds};
+  const pnResidualNorm& p = a.p;
+  const int slot = threadIdx.x / L, t = threadIdx.x % L, C = p.cols;
+  const T* X = reinterpret_cast<const T*>(p.x);
+  const T* F = reinterpret_cast<const T*>(p.branch);
+  T* H = reinterpret_cast<T*>(a.h);
+  T* Y = reinterpret_cast<T*>(a.y);
+  PhiloxKey key{};
+  if (p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
+  for (long long base = (long long)blockIdx.x * SLOTS; base < p.rows; base += (long long)gridDim.x * SLOTS) {
+    const bool live = base + slot < p.rows;
+    const long long row = live ? base + slot : p.rows - 1;
+    float h[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * L + t) * 8;
+      load8(X + row * p.ldx + c, C - c, h[k]);
+    }
+    float2 fs = make_float2(0.f, 1.f);
+    if (F) {
+      float f[K][8];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        load8(F + row * p.ldb + c, C - c, f[k]);
+      }
+      fs = row_stats<K>(f, p.post_kind, p.post_eps, C, t * 8, L * 8, sum);
+      const char* gate = reinterpret_cast<const char*>(p.gate);
+      if (gate) gate += row / p.rows_per_gate * C * (p.param_dtype == PN_DTYPE_F32 ? 4 : 2);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        float w[8], b[8], g[8];
+        load_param(p.post_weight, p.param_dtype, c, C - c, w, 1.f);
+        load_param(p.post_bias, p.param_dtype, c, C - c, b, 0.f);
+        load_param(gate, p.param_dtype, c, C - c, g, 1.f);
+        uint32_t keep = 0xffu;
+        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + c, p.threshold);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float u = f[k][i];
+          if (p.post_kind != PN_NORM_NONE) u = fmaf((u - fs.x) * fs.y, w[i], b[i]);
+          u = (keep >> i & 1) ? u * a.keep_scale : 0.f;
+          h[k][i] = (float)(T)fmaf(p.scale * g[i], u, h[k][i]);
+        }
+        if (live) store8(H + row * C + c, C - c, h[k]);
+        // what lies behind the row's end must not enter the norm's sums
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i >= C) h[k][i] = 0.f;
+      }
+    }
+    float2 hs = make_float2(0.f, 1.f);
+    if (Y) {
+      hs = row_stats<K>(h, p.norm_kind, p.norm_eps, C, t * 8, L * 8, sum);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        float w[8], b[8];
+        load_param(p.norm_weight, p.param_dtype, c, C - c, w, 1.f);
+        load_param(p.norm_bias, p.param_dtype, c, C - c, b, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = act_f(fmaf((h[k][i] - hs.x) * hs.y, w[i], b[i]), p.act);
+        if (live) store8(Y + row * C + c, C - c, w);
+      }
+    }
+    if (a.stats && live && t == 0)
+      *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(hs.x, hs.y, fs.x, fs.y);
+  }
+}
+
+// Backward.  A workgroup owns a chunk of consecutive rows and keeps the column sums (gradients of weights, biases and gate)
+// in registers over the whole chunk; its partial sums go to memory once, and residual_norm_sum_kernel adds the chunks in
+// order: no atomics, the same bits on every run.
+static constexpr int NSUM_NORM = 2, NSUM_ALL = 5;      // weight, bias | post weight, post bias, gate
+
+template <typename T, int L, int K, int NT, bool BRANCH>
+__global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
+  constexpr int SLOTS = NT / L, NS = BRANCH ? NSUM_ALL : NSUM_NORM;
+  __shared__ float2 lds[2 * (NT / 64)];
+  __shared__ float cols_lds[SLOTS > 1 ? NT * 8 : 1];
+  RowSum<L, NT> sum{lds};
+  const pnResidualNorm& p = a.p;
+  const int slot = threadIdx.x / L, t = threadIdx.x % L, C = p.cols;
+  const int group = blockIdx.x / a.chunks_per_group, chunk = blockIdx.x % a.chunks_per_group;
+  const long long g_begin = (long long)group * a.group_rows, g_end = min(g_begin + a.group_rows, (long long)p.rows);
+  const long long r_begin = g_begin + (long long)chunk * a.chunk_rows, r_end = min(r_begin + a.chunk_rows, g_end);
+  const T* H = reinterpret_cast<const T*>(p.branch ? a.h : p.x);
+  const long long ldh = p.branch ? C : p.ldx;
+  const T* F = reinterpret_cast<const T*>(p.branch);
+  const T* GH = reinterpret_cast<const T*>(a.gh);
+  const T* GY = reinterpret_cast<const T*>(a.gy);
+  PhiloxKey key{};
+  if (BRANCH && p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
+  const char* gate_row = reinterpret_cast<const char*>(p.gate);
+  const float inv_c = 1.f / (float)C;
+  float acc[NS][K][8];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[s][k][i] = 0.f;
+
+  for (long long base = r_begin; base < r_end; base += SLOTS) {
+    const bool live = base + slot < r_end;
+    const long long row = live ? base + slot : r_end - 1;
+    const float4 st = a.stats ? *reinterpret_cast<const float4*>(a.stats + row * 4) : make_float4(0.f, 1.f, 0.f, 1.f);
+    float dh[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * L + t) * 8;
+      if (GH) {
+        load8(GH + row * C + c, C - c, dh[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dh[k][i] = 0.f;
+      }
+    }
+    if (GY) {
+      float tw[K][8], hh[K][8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        float w[8], b[8];
+        load8(GY + row * C + c, C - c, tw[k]);
+        load8(H + row * ldh + c, C - c, hh[k]);
+        load_param(p.norm_weight, p.param_dtype, c, C - c, w, 1.f);
+        if (p.act == PN_ACT_RELU) load_param(p.norm_bias, p.param_dtype, c, C - c, b, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hh[k][i] = (hh[k][i] - st.x) * st.y;
+          if (c + i >= C) hh[k][i] = 0.f;
+          float g = tw[k][i];
+          if (p.act == PN_ACT_RELU && fmaf(hh[k][i], w[i], b[i]) <= 0.f) g = 0.f;
+          if (live) {
+            acc[0][k][i] = fmaf(g, hh[k][i], acc[0][k][i]);
+            acc[1][k][i] += g;
+          }
+          tw[k][i] = g * w[i];
+          s1 += tw[k][i];
+          s2 = fmaf(tw[k][i], hh[k][i], s2);
+        }
+      }
+      if (p.norm_kind == PN_NORM_LAYER || p.norm_kind == PN_NORM_RMS) {
+        const float2 m = sum(s1, s2);
+        const float m1 = p.norm_kind == PN_NORM_LAYER ? m.x * inv_c : 0.f, m2 = m.y * inv_c;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dh[k][i] = fmaf(st.y, (tw[k][i] - m1) - hh[k][i] * m2, dh[k][i]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dh[k][i] += tw[k][i];
+      }
+    }
+    if (a.dx) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        if (live) store8(reinterpret_cast<T*>(a.dx) + row * C + c, C - c, dh[k]);
+      }
+    }
+    if constexpr (BRANCH) {
+      const char* gate = gate_row ? gate_row + row / p.rows_per_gate * C * (p.param_dtype == PN_DTYPE_F32 ? 4 : 2) : nullptr;
+      float fh[K][8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        float w[8], b[8], g[8], dg[8];
+        load8(F + row * p.ldb + c, C - c, fh[k]);
+        load_param(p.post_weight, p.param_dtype, c, C - c, w, 1.f);
+        load_param(p.post_bias, p.param_dtype, c, C - c, b, 0.f);
+        load_param(gate, p.param_dtype, c, C - c, g, 1.f);
+        uint32_t keep = 0xffu;
+        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + c, p.threshold);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          fh[k][i] = (fh[k][i] - st.z) * st.w;
+          if (c + i >= C) fh[k][i] = 0.f;
+          const float u = p.post_kind != PN_NORM_NONE ? fmaf(fh[k][i], w[i], b[i]) : fh[k][i];
+          const bool kept = keep >> i & 1;
+          const float sd = p.scale * dh[k][i];
+          const float du = kept ? g[i] * sd * a.keep_scale : 0.f;
+          const float v = kept ? u * a.keep_scale : 0.f;
+          dg[i] = sd * v;
+          if (live && c + i < C) {
+            acc[NS - 1][k][i] += dg[i];
+            acc[NS - 3][k][i] = fmaf(du, fh[k][i], acc[NS - 3][k][i]);
+            acc[NS - 2][k][i] += du;
+          }
+          dh[k][i] = p.post_kind != PN_NORM_NONE ? du * w[i] : du;
+          s1 += dh[k][i];
+          s2 = fmaf(dh[k][i], fh[k][i], s2);
+        }
+        if (a.dgate_rows && live) {
+          if (p.param_dtype == PN_DTYPE_F32) store8(reinterpret_cast<float*>(a.dgate_rows) + row * C + c, C - c, dg);
+          else store8(reinterpret_cast<__bf16*>(a.dgate_rows) + row * C + c, C - c, dg);
+        }
+      }
+      if (p.post_kind == PN_NORM_LAYER || p.post_kind == PN_NORM_RMS) {
+        const float2 m = sum(s1, s2);
+        const float m1 = p.post_kind == PN_NORM_LAYER ? m.x * inv_c : 0.f, m2 = m.y * inv_c;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dh[k][i] = st.w * ((dh[k][i] - m1) - fh[k][i] * m2);
+      }
+      if (a.df) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int c = (k * L + t) * 8;
+          if (live) store8(reinterpret_cast<T*>(a.df) + row * C + c, C - c, dh[k]);
+        }
+      }
+    }
+  }
+
+  float* out = a.partial + (size_t)blockIdx.x * NS * C;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    if (SLOTS == 1) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + t) * 8;
+        store8(out + s * C + c, C - c, acc[s][k]);
+      }
+    } else {                                     // add the workgroup's row slots, in order
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cols_lds[slot * L * 8 + t * 8 + i] = acc[s][k][i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < L * 8; c += NT) {
+          float v = 0.f;
+          for (int q = 0; q < SLOTS; ++q) v += cols_lds[q * L * 8 + c];
+          if (k * L * 8 + c < C) out[s * C + k * L * 8 + c] = v;
+        }
+      }
+    }
+  }
+}
+
+// out[v][c] = sum over the chunks of vector v: blockIdx.x picks the vector (weight, bias, post weight, post bias, then
+// one gate row each), blockIdx.y its 64 columns; 16 chunk lanes.
+struct SumArgs {
+  const float* partial;
+  void* out[NSUM_ALL];
+  int cols, sums, chunks, chunks_per_group, out_bf16;
+};
+__global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
+  __shared__ float lds[16][64];
+  const int v = blockIdx.x, s = v < NSUM_ALL - 1 ? v : NSUM_ALL - 1, group = v - s;
+  void* out = a.out[s];
+  if (!out) return;                                                        // the same for the whole workgroup
+  const bool per_group = s == NSUM_ALL - 1;
+  const int first = per_group ? group * a.chunks_per_group : 0, count = per_group ? a.chunks_per_group : a.chunks;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 64 + lane;
+  float acc = 0.f;
+  if (c < a.cols) {
+    const float* p = a.partial + ((size_t)first * a.sums + s) * a.cols + c;
+    for (int i = w; i < count; i += 16) acc += p[(size_t)i * a.sums * a.cols];
+  }
+  lds[w][lane] = acc;
+  __syncthreads();
+  if (w == 0 && c < a.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += lds[i][lane];
+    const size_t at = (size_t)group * a.cols + c;
+    if (a.out_bf16) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
+    else reinterpret_cast<float*>(out)[at] = t;
+  }
+}
+
+static int norm_check(const pnResidualNorm* p) {
+  PN_CHECK_ARG(p, "residual_norm: null pointer");
+  PN_CHECK_ARG(p->dtype == PN_DTYPE_F32 || p->dtype == PN_DTYPE_BF16, "residual_norm: element type %d (fp32 or bf16)", p->dtype);
+  PN_CHECK_ARG(p->param_dtype == PN_DTYPE_F32 || p->param_dtype == PN_DTYPE_BF16, "residual_norm: parameter type %d (fp32 or bf16)",
+               p->param_dtype);
+  PN_CHECK_ARG(p->cols >= 1 && p->cols <= PN_NORM_MAX_COLS, "residual_norm: %d columns (1..%d)", p->cols, PN_NORM_MAX_COLS);
+  PN_CHECK_ARG(p->rows >= 0 && p->rows < (1ll << 40) / p->cols, "residual_norm: %lld rows", (long long)p->rows);
+  PN_CHECK_ARG(p->post_kind >= PN_NORM_NONE && p->post_kind <= PN_NORM_RMS, "residual_norm: post norm %d (none, layer, rms)",
+               p->post_kind);
+  PN_CHECK_ARG(p->norm_kind >= PN_NORM_NONE && p->norm_kind <= PN_NORM_AFFINE, "residual_norm: norm %d", p->norm_kind);
+  PN_CHECK_ARG(p->act == PN_ACT_NONE || p->act == PN_ACT_RELU, "residual_norm: activation %d (none or relu)", p->act);
+  PN_CHECK_ARG(p->branch || (!p->gate && p->post_kind == PN_NORM_NONE && !p->threshold),
+               "residual_norm: gate, post norm and dropout act on a branch");
+  PN_CHECK_ARG(p->branch || p->norm_kind != PN_NORM_NONE, "residual_norm: neither a branch nor a norm");
+  PN_CHECK_ARG(p->threshold <= 65536u && p->call < 65536u && (p->rng || !p->threshold), "residual_norm: dropout threshold %u, call %u",
+               p->threshold, p->call);
+  PN_CHECK_ARG(p->rows == 0 || (p->x && (p->rows == 1 || (p->ldx >= p->cols && (!p->branch || p->ldb >= p->cols)))),
+               "residual_norm: x missing or a row stride below the row length");
+  PN_CHECK_ARG(!p->gate || (p->rows_per_gate >= 1 && p->rows % p->rows_per_gate == 0),
+               "residual_norm: %lld rows do not divide into gates of %lld rows", (long long)p->rows, (long long)p->rows_per_gate);
+  return PN_OK;
+}
+
+static NormArgs norm_args(const pnResidualNorm* p) {
+  NormArgs a = {};
+  a.p = *p;
+  a.keep_scale = !p->threshold ? 1.f : p->threshold < 65536u ? 65536.f / (65536.f - (float)p->threshold) : 0.f;
+  if (!p->gate) a.p.rows_per_gate = p->rows > 0 ? p->rows : 1;
+  return a;
+}
+
+// Threads per row: the fewest that hold the row at eight elements each, so that a narrow row does not idle a wave.
+#define NORM_BY_COLS(C, GO)                                                      \
+  (C) <= 64 ? GO(8, 1, 256) : (C) <= 128 ? GO(16, 1, 256) : (C) <= 256 ? GO(32, 1, 256) : (C) <= 512 ? GO(64, 1, 256) \
+  : (C) <= 1024 ? GO(128, 1, 256) : (C) <= 2048 ? GO(256, 1, 256) : (C) <= 4096 ? GO(512, 1, 512)              \
+  : (C) <= 8192 ? GO(1024, 1, 1024) : GO(1024, 2, 1024)
+
+template <typename T, int L, int K, int NT> static int norm_fwd(const NormArgs& a, hipStream_t s) {
+  const long long need = (a.p.rows + NT / L - 1) / (NT / L);
+  const unsigned grid = (unsigned)(need < (1 << 30) ? need : (1 << 30));
+  hipLaunchKernelGGL((residual_norm_fwd_kernel<T, L, K, NT>), dim3(grid), dim3(NT), 0, s, a);
+  PN_CHECK_LAUNCH("residual_norm_fwd_kernel");
+  return PN_OK;
+}
+
+extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* y, float* stats, void* stream) {
+  const int rc = norm_check(p);
+  if (rc != PN_OK) return rc;
+  if (p->rows == 0) return PN_OK;
+  PN_CHECK_ARG(((uintptr_t)stats & 15) == 0, "residual_norm: the statistics must be 16-byte aligned");
+  PN_CHECK_ARG((h || !p->branch) && (y || p->norm_kind == PN_NORM_NONE), "residual_norm: output missing");
+  NormArgs a = norm_args(p);
+  a.h = h;
+  a.y = p->norm_kind == PN_NORM_NONE ? nullptr : y;
+  a.stats = stats;
+  hipStream_t s = (hipStream_t)stream;
+#define GO_F32(L, K, NT) norm_fwd<float, L, K, NT>(a, s)
+#define GO_BF16(L, K, NT) norm_fwd<__bf16, L, K, NT>(a, s)
+  if (p->dtype == PN_DTYPE_F32) return NORM_BY_COLS(p->cols, GO_F32);
+  return NORM_BY_COLS(p->cols, GO_BF16);
+#undef GO_F32
+#undef GO_BF16
+}
+
+// Chunks of the backward pass: about NORM_WGS workgroups in all, whole passes over the row slots, none across two gates.
+static constexpr int NORM_WGS = 1024;
+struct NormChunks { long long groups, group_rows; int per_group, rows, sums; };
+static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
+  NormChunks c;
+  c.groups = p->gate && p->rows_per_gate > 1 ? p->rows / p->rows_per_gate : 1;
+  if (c.groups < 1) c.groups = 1;
+  c.group_rows = c.groups > 1 ? p->rows_per_gate : p->rows;
+#define SLOTS_OF(L, K, NT) (NT / L)
+  const int slots = NORM_BY_COLS(p->cols, SLOTS_OF);
+#undef SLOTS_OF
+  const long long passes = (c.group_rows + slots - 1) / slots;
+  long long want = (NORM_WGS + c.groups - 1) / c.groups;
+  if (want > passes) want = passes;
+  if (want < 1) want = 1;
+  const long long per = (passes + want - 1) / want;
+  c.rows = (int)(per * slots);
+  c.per_group = (int)((passes + per - 1) / per);
+  c.sums = branch ? NSUM_ALL : NSUM_NORM;
+  return c;
+}
+static bool norm_reads_branch(const pnResidualNorm* p) { return p->branch && (p->gate || p->post_kind != PN_NORM_NONE || p->threshold || p->scale != 1.f); }
+
+extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
+  if (norm_check(p) != PN_OK) return 0;
+  const NormChunks c = norm_chunks(p, norm_reads_branch(p));
+  return (size_t)c.groups * c.per_group * c.sums * p->cols * sizeof(float);
+}
+
+template <typename T, int L, int K, int NT> static int norm_bwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
+  if (branch) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, L, K, NT, true>), dim3(grid), dim3(NT), 0, s, a);
+  else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, L, K, NT, false>), dim3(grid), dim3(NT), 0, s, a);
+  PN_CHECK_LAUNCH("residual_norm_bwd_kernel");
+  return PN_OK;
+}
+
+extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const float* stats, const void* gh,
+                                         const void* gy, void* dx, void* dbranch, void* dweight, void* dbias,
+                                         void* dpost_weight, void* dpost_bias, void* dgate, void* ws, size_t ws_bytes,
+                                         void* stream) {
+  const int rc = norm_check(p);
+  if (rc != PN_OK) return rc;
+  const bool branch = norm_reads_branch(p);
+  PN_CHECK_ARG(gh || gy, "residual_norm: no gradient given");
+  PN_CHECK_ARG(!gy || p->norm_kind != PN_NORM_NONE, "residual_norm: gradient of an output that there is not");
+  PN_CHECK_ARG(p->rows == 0 || !gy || h || !p->branch, "residual_norm: the stored rows are needed");
+  PN_CHECK_ARG(p->rows == 0 || stats || (p->norm_kind != PN_NORM_LAYER && p->norm_kind != PN_NORM_RMS && p->post_kind == PN_NORM_NONE),
+               "residual_norm: the stored statistics are needed");
+  PN_CHECK_ARG(((uintptr_t)stats & 15) == 0, "residual_norm: the statistics must be 16-byte aligned");
+  PN_CHECK_ARG(branch || !dbranch, "residual_norm: the branch's gradient is dx itself");
+  PN_CHECK_ARG(!dgate || p->gate, "residual_norm: gradient of a gate that there is not");
+  const NormChunks c = norm_chunks(p, branch);
+  PN_CHECK_ARG(c.groups * c.per_group < (1ll << 31), "residual_norm: too many gates");
+  hipStream_t s = (hipStream_t)stream;
+  const long long chunks = p->rows ? c.groups * c.per_group : 0;
+  if (chunks) {
+    if (ws_bytes < (size_t)chunks * c.sums * p->cols * sizeof(float) || !ws) {
+      pn_set_error("residual_norm: workspace of %zu bytes is too small", ws_bytes);
+      return PN_ENOSPC;
+    }
+    NormArgs a = norm_args(p);
+    a.h = const_cast<void*>(h);
+    a.stats = const_cast<float*>(stats);
+    a.gh = gh;
+    a.gy = gy;
+    a.dx = dx;
+    a.df = dbranch;
+    if (p->gate && p->rows_per_gate == 1 && p->rows > 1) {
+      a.dgate_rows = dgate;
+      dgate = nullptr;
+    }
+    a.partial = (float*)ws;
+    a.chunk_rows = c.rows;
+    a.chunks_per_group = c.per_group;
+    a.group_rows = c.group_rows;
+#define GO_F32(L, K, NT) norm_bwd<float, L, K, NT>(a, branch, (unsigned)chunks, s)
+#define GO_BF16(L, K, NT) norm_bwd<__bf16, L, K, NT>(a, branch, (unsigned)chunks, s)
+    const int r = p->dtype == PN_DTYPE_F32 ? (NORM_BY_COLS(p->cols, GO_F32)) : (NORM_BY_COLS(p->cols, GO_BF16));
+#undef GO_F32
+#undef GO_BF16
+    if (r != PN_OK) return r;
+  }
+  if (dweight || dbias || dpost_weight || dpost_bias || dgate) {
+    const long long vecs = dgate ? NSUM_ALL - 1 + c.groups : (dpost_weight || dpost_bias) ? NSUM_ALL - 1 : NSUM_NORM;
+    if (!p->rows) dgate = nullptr;                 // no rows, no gates
+    SumArgs q = {(const float*)ws, {dweight, dbias, dpost_weight, dpost_bias, dgate}, p->cols, c.sums, (int)chunks,
+                 chunks ? c.per_group : 0, p->param_dtype == PN_DTYPE_BF16};
+    hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((unsigned)vecs, (p->cols + 63) / 64), dim3(1024), 0, s, q);
+    PN_CHECK_LAUNCH("residual_norm_sum_kernel");
+  }
+  return PN_OK;
+}

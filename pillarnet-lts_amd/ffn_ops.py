@@ -1,0 +1,454 @@
+"""Operators of the RoI heads' feed-forward blocks (det3d/models/roi_heads/roi_ffn_head.py:34-39,101-102, the FC stacks
+with Dropout of roi_head_template.py:23-39, the mixers of mlp_layers.py:24-117) on hand-written kernels:
+
+  act_dropout       activation + dropout; the mask is drawn again in the backward pass and never stored
+  residual_norm     residual + scale * gate * dropout(post_norm(branch)), then the next block's norm
+  fp8_linear        product in 8-bit floating point (e4m3) with a power-of-two scale for each block of 128
+  fp8_linear_train  the same while training, with both gradients in fp8
+
+All take fp32 or bf16 tensors on the GPU, run on the current stream of the tensors' device, allocate through torch's
+caching allocator only and wait for nothing, so they can be captured into a HIP graph.  A graph that holds a backward pass
+is captured while no eager autograd graph over the same leaves is alive (torch's own rule for captured backward passes)."""
+from collections import namedtuple
+from ctypes import byref
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import PillarnetHipError
+
+_DTYPES = {torch.float32: _lib.PN_DTYPE_F32, torch.bfloat16: _lib.PN_DTYPE_BF16}
+
+
+def _require(cond, message):
+    if not cond:
+        raise PillarnetHipError(message)
+
+
+def _check(what, *tensors):
+    """GPU tensors of one device, fp32 or bf16."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device.type != "cuda":
+            raise PillarnetHipError(f"{what}: tensors must live on the GPU (no CPU fallback)")
+        if t.device != dev:
+            raise PillarnetHipError(f"{what}: tensors on {dev} and {t.device}")
+        if t.dtype not in _DTYPES:
+            raise PillarnetHipError(f"{what}: {t.dtype} (fp32 or bf16)")
+
+
+def _call(name, device, *args):
+    """One C entry on `device`'s current stream, with `device` current during the launch."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(x):
+    """x as [rows, cols] with unit column stride and a row stride >= cols; a copy only where no view has them."""
+    C = x.shape[-1]
+    if x.is_contiguous():
+        return x.view(-1, C) if C else x.reshape(0, 0)
+    try:
+        v = x.view(-1, C)
+        if v.stride(1) == 1 and (v.shape[0] <= 1 or v.stride(0) >= C):
+            return v
+    except RuntimeError:
+        pass
+    return x.contiguous().view(-1, C)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---- activation + dropout ----------------------------------------------------------------------------------------------
+def dropout_threshold(p):
+    """The 16-bit threshold of a drop probability: p is taken to the nearest 1 / 65536, at least one step for p > 0 and
+    at most 65535 for p < 1; the kept elements are scaled by 65536 / (65536 - threshold), so the mean is kept exactly."""
+    _require(0.0 <= p <= 1.0, f"dropout probability {p} (0 to 1)")
+    if p == 0.0 or p == 1.0:
+        return int(p) * 65536
+    return min(65535, max(1, round(p * 65536)))
+
+
+class DropoutState:
+    """(seed, offset) of the generator in device memory.  `draw()` hands out the pair a pass uses -- an int64 tensor [2]
+    that its forward and backward share -- and moves the offset on, on the device: a captured and replayed graph draws new
+    masks on every replay."""
+
+    def __init__(self, seed, device="cuda"):
+        seed = int(seed) & (1 << 64) - 1
+        self.state = torch.tensor([seed - (1 << 64) if seed >> 63 else seed, 0], dtype=torch.int64, device=device)
+        _require(self.state.device.type == "cuda", "DropoutState: the state must live on the GPU (no CPU fallback)")
+
+    def draw(self):
+        used = torch.empty_like(self.state)
+        _call("pn_dropout_draw", self.state.device, self.state.data_ptr(), used.data_ptr())
+        return used
+
+
+def _check_rng(what, rng, device, call):
+    _require(isinstance(rng, torch.Tensor) and rng.dtype == torch.int64 and rng.shape == (2,) and rng.is_contiguous() and
+             rng.device == device, f"{what}: the generator's state is an int64 tensor [2] (seed, offset) on the inputs' device")
+    _require(0 <= call < 65536, f"{what}: call {call} (0 to 65535)")
+
+
+def _act_dropout_forward(x, threshold, rng, call, act):
+    v = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), v.shape[0], v.shape[1], v.stride(0), act, threshold,
+          _ptr(rng), call, y.data_ptr())
+    return y
+
+
+class _ActDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, threshold, rng, call, act):
+        y = _act_dropout_forward(x, threshold, rng, call, act)
+        ctx.save_for_backward(rng, x if act == _lib.PN_ACT["gelu"] else y if act == _lib.PN_ACT["relu"] else None)
+        ctx.args = (threshold, call, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        rng, saved = ctx.saved_tensors
+        threshold, call, act = ctx.args
+        gv = _rows(g)
+        sv = None if saved is None else _rows(saved)
+        dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), gv.shape[0], gv.shape[1],
+              gv.stride(0), 0 if sv is None else sv.stride(0), act, threshold, _ptr(rng), call, dx.data_ptr())
+        return dx, None, None, None, None
+
+
+def act_dropout(x, p, rng=None, call=0, act="none"):
+    """dropout(act(x), p) with act "none" | "relu" | "gelu" (erf form), differentiable in x.
+
+    rng: int64 [2] (seed, offset) on x's device, what `DropoutState.draw()` returns; it is read when the kernels run, the
+    backward pass included, so its contents stay until then.  call (< 65536) tells the dropouts of one pass apart.  p = 0
+    needs no rng, p = 1 gives zeros.  The mask depends on (seed, offset, call, element index) only, not on strides."""
+    _check("act_dropout", x)
+    _require(act in _lib.PN_ACT, f"act_dropout: activation {act!r}")
+    _require(x.dim() >= 1, "act_dropout: a tensor of at least one dimension")
+    threshold = dropout_threshold(p)
+    if threshold:
+        _check_rng("act_dropout", rng, x.device, call)
+    else:
+        if act == "none":
+            return x
+        rng, call = None, 0
+    if _wants_grad(x):
+        return _ActDropout.apply(x, threshold, rng, call, _lib.PN_ACT[act])
+    return _act_dropout_forward(x.detach(), threshold, rng, call, _lib.PN_ACT[act])
+
+
+# ---- residual join and norms -------------------------------------------------------------------------------------------
+class Norm(namedtuple("Norm", "kind weight bias eps")):
+    """kind "layer" | "rms" | "affine" (weight and bias only); weight / bias [C] or None (1 / 0)."""
+
+    def __new__(cls, kind, weight=None, bias=None, eps=1e-5):
+        _require(kind in ("layer", "rms", "affine"), f"Norm: kind {kind!r}")
+        return super().__new__(cls, kind, weight, bias, float(eps))
+
+    @classmethod
+    def of(cls, module):
+        """of an nn.LayerNorm / nn.RMSNorm over the last dimension."""
+        kind = {torch.nn.LayerNorm: "layer", torch.nn.RMSNorm: "rms"}.get(type(module))
+        _require(kind is not None and len(module.normalized_shape) == 1, f"Norm.of: {module}")
+        eps = module.eps if module.eps is not None else torch.finfo(torch.float32).eps
+        return cls(kind, module.weight, getattr(module, "bias", None), eps)
+
+
+_JoinCfg = namedtuple("_JoinCfg", "post norm post_eps norm_eps scale threshold call act rows_per_gate")
+
+
+def _join_struct(cfg, x, f, gate, pw, pb, w, b, rng):
+    """(struct, row views that must outlive the launch)."""
+    xv, fv = _rows(x), None if f is None else _rows(f)
+    params = [t for t in (gate, pw, pb, w, b) if t is not None]
+    s = _lib.pnResidualNorm(
+        _DTYPES[x.dtype], _DTYPES[params[0].dtype] if params else _lib.PN_DTYPE_F32, cfg.post, cfg.norm, cfg.act, x.shape[-1],
+        xv.shape[0], cfg.rows_per_gate, xv.stride(0), 0 if fv is None else fv.stride(0), cfg.scale, cfg.post_eps, cfg.norm_eps,
+        cfg.threshold, cfg.call, _ptr(rng), xv.data_ptr(), _ptr(fv), _ptr(gate), _ptr(pw), _ptr(pb), _ptr(w), _ptr(b))
+    return s, (xv, fv)
+
+
+def _join_forward(cfg, x, f, gate, pw, pb, w, b, rng, want_stats):
+    s, keep = _join_struct(cfg, x, f, gate, pw, pb, w, b, rng)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if cfg.norm else None
+    stats = torch.empty((s.rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
+    if s.rows:                          # (an empty tensor has no address to tell the branch by)
+        _call("pn_residual_norm_forward", x.device, byref(s), _ptr(h), _ptr(y), _ptr(stats))
+    return h, y, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, rng, x, f, gate, pw, pb, w, b):
+        h, y, stats = _join_forward(cfg, x, f, gate, pw, pb, w, b, rng, True)
+        reads_f = f is not None and (gate is not None or cfg.post or cfg.threshold or cfg.scale != 1.0)
+        ctx.cfg, ctx.has_branch, ctx.reads_f = cfg, f is not None, reads_f
+        # the norm's backward reads the rows it normalised; x itself is needed only where it is those rows
+        ctx.save_for_backward(rng, h if f is not None else x, f if reads_f else None, gate, pw, pb, w, b, stats)
+        ctx.set_materialize_grads(False)
+        return (h, y) if f is not None and cfg.norm else h if f is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        cfg = ctx.cfg
+        rng, h, f, gate, pw, pb, w, b, stats = ctx.saved_tensors
+        if ctx.has_branch:
+            gh, gy = grads if cfg.norm else (grads[0], None)
+        else:
+            gh, gy = None, grads[0]
+        if gh is None and gy is None:
+            return (None,) * 9
+        dev, shape, dt = h.device, h.shape, h.dtype
+        need = ctx.needs_input_grad[2:]
+        # without reads_f the struct still needs a branch pointer to say that h is a stored tensor: h stands in, unread
+        s, keep = _join_struct(cfg, h, (f if ctx.reads_f else h) if ctx.has_branch else None, gate, pw, pb, w, b, rng)
+        gh = None if gh is None else gh.contiguous()
+        gy = None if gy is None else gy.contiguous()
+        dx = torch.empty(shape, dtype=dt, device=dev) if need[0] or (need[1] and not ctx.reads_f) else None
+        df = torch.empty(shape, dtype=dt, device=dev) if need[1] and ctx.reads_f else None
+        sums = [torch.empty_like(t, memory_format=torch.contiguous_format) if n and t is not None else None
+                for t, n in zip((w, b, pw, pb, gate), (need[5], need[6], need[3], need[4], need[2]))]
+        if s.rows == 0:
+            for t in sums:
+                if t is not None:
+                    t.zero_()
+        else:
+            size = _lib.lib().pn_residual_norm_workspace_bytes(byref(s))
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            _call("pn_residual_norm_backward", dev, byref(s), _ptr(h), _ptr(stats), _ptr(gh), _ptr(gy), _ptr(dx), _ptr(df),
+                  *[_ptr(t) for t in sums], ws.data_ptr(), size)
+        dw, db, dpw, dpb, dgate = sums
+        if ctx.has_branch and not ctx.reads_f:
+            df = dx if need[1] else None
+        return None, None, dx if need[0] else None, df, dgate, dpw, dpb, dw, db
+
+
+def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=None, dropout=None, act="none"):
+    """h = x + scale * gate * dropout(post_norm(branch)), rounded to x's type; y = act(norm(h)).
+
+    x, branch: [..., C], one type (C up to 16384).  gate: None, [C] (layer scale), x's shape, or one row for each leading
+    sample -- [B, C] or [B, 1, C] with x [B, ..., C].  post_norm: Norm "layer" / "rms" or None; norm: any Norm or None;
+    dropout: (p, rng, call) as act_dropout or None; act ("none" | "relu") on y.  Differentiable in x, branch, gate and the norms'
+    weights and biases.  Returns (h, y) with branch and norm, h without a norm, y without a branch (h is then x itself).
+
+    The norm reads h as stored, so y is the norm of the returned h; its gradient is that of what was computed."""
+    what = "residual_norm"
+    _check(what, *[t for t in (x, branch, gate) if t is not None])
+    _require(x.dim() >= 1 and 1 <= x.shape[-1] <= _lib.PN_NORM_MAX_COLS, f"{what}: rows of 1 to {_lib.PN_NORM_MAX_COLS} elements")
+    C = x.shape[-1]
+    _require(branch is not None or norm is not None, f"{what}: neither a branch nor a norm")
+    _require(branch is not None or (gate is None and post_norm is None and dropout is None and scale == 1.0),
+             f"{what}: gate, scale, post norm and dropout act on a branch")
+    _require(branch is None or (branch.shape == x.shape and branch.dtype == x.dtype),
+             f"{what}: the branch has another shape or type than x")
+    _require(act in ("none", "relu") and (act == "none" or norm is not None), f"{what}: activation {act!r}")
+    _require(post_norm is None or post_norm.kind != "affine", f"{what}: the post norm is layer or rms")
+    pw, pb = (post_norm.weight, post_norm.bias) if post_norm is not None else (None, None)
+    w, b = (norm.weight, norm.bias) if norm is not None else (None, None)
+    for t in (pw, pb, w, b):
+        if t is not None:
+            _check(what, x, t)
+            _require(t.shape == (C,), f"{what}: weights and biases have shape [{C}]")
+    R = x.numel() // C
+    rows_per_gate = max(R, 1)
+    if gate is not None:
+        if gate.shape == (C,):
+            pass
+        elif gate.shape == x.shape:
+            rows_per_gate = 1
+        else:
+            _require(x.dim() >= 2 and gate.shape[0] == x.shape[0] and gate.shape[-1] == C and gate.numel() == x.shape[0] * C,
+                     f"{what}: a gate of shape {tuple(gate.shape)} for {tuple(x.shape)}")
+            rows_per_gate = max(R // max(x.shape[0], 1), 1)
+    threshold, rng, call = 0, None, 0
+    if dropout is not None:
+        p, rng, call = dropout
+        threshold = dropout_threshold(p)
+        if threshold:
+            _check_rng(what, rng, x.device, call)
+        else:
+            rng, call = None, 0
+    params = [gate, pw, pb, w, b]
+    kinds = {t.dtype for t in params if t is not None}
+    if len(kinds) > 1:                  # the kernels read parameters of one type
+        params = [None if t is None else t.float() for t in params]
+    gate, pw, pb, w, b = [None if t is None else t.contiguous() for t in params]
+    cfg = _JoinCfg(_lib.PN_NORM[post_norm.kind] if post_norm is not None else 0, _lib.PN_NORM[norm.kind] if norm is not None else 0,
+                   post_norm.eps if post_norm is not None else 0.0, norm.eps if norm is not None else 0.0, float(scale), threshold, call,
+                   _lib.PN_ACT[act], rows_per_gate)
+    if _wants_grad(x, branch, gate, pw, pb, w, b):
+        return _ResidualNorm.apply(cfg, rng, x, branch, gate, pw, pb, w, b)
+    h, y, _ = _join_forward(cfg, x, branch, gate, pw, pb, w, b, rng, False)
+    return (h, y) if h is not None and y is not None else h if y is None else y
+
+
+# ---- products in fp8 ---------------------------------------------------------------------------------------------------
+class Fp8Rows:
+    """[rows, cols] in e4m3 with block scales, as pn_fp8_quantize lays them out: q uint8 [rows, kp], scale uint8
+    [ceil(kp / 512), rows, 4]."""
+    __slots__ = ("q", "scale", "rows", "cols")
+
+    def __init__(self, rows, cols, device):
+        kp = -(-cols // 128) * 128
+        self.rows, self.cols = rows, cols
+        self.q = torch.empty((rows, kp), dtype=torch.uint8, device=device)
+        self.scale = torch.empty((-(-kp // 512), rows, 4), dtype=torch.uint8, device=device)
+
+    def values(self):
+        """What the bytes stand for, fp32 [rows, cols] (for tests and inspection)."""
+        kp = self.q.shape[1]
+        e = self.scale.permute(1, 0, 2).reshape(self.rows, -1)[:, : kp // 128].to(torch.int32)
+        s = (e << 23).view(torch.float32).repeat_interleave(128, 1)
+        return (self.q.view(torch.float8_e4m3fn).float() * s)[:, : self.cols]
+
+
+def fp8_quantize(x, block_rows=1, rows=True, transposed=False, colsum=False):
+    """x [..., C] -> (Fp8Rows of x or None, Fp8Rows of its transpose or None, column-sum partials or None), in one pass.
+    block_rows 1: a scale for each 128 elements along the contraction (the row, or the column for the transpose);
+    128: one for each 128 x 128 tile (weights)."""
+    _check("fp8_quantize", x)
+    _require(x.dim() >= 1 and x.shape[-1] >= 1, "fp8_quantize: empty rows")
+    _require(block_rows in (1, 128), f"fp8_quantize: blocks of {block_rows} rows (1 or 128)")
+    _require(rows or transposed, "fp8_quantize: nothing asked for")
+    v = _rows(x.detach())
+    M, C = v.shape
+    q = Fp8Rows(M, C, x.device) if rows else None
+    qt = Fp8Rows(C, M, x.device) if transposed else None
+    cs = torch.empty((-(-M // 128), C), dtype=torch.float32, device=x.device) if colsum else None
+    _call("pn_fp8_quantize", x.device, _DTYPES[x.dtype], v.data_ptr(), M, C, v.stride(0), block_rows, _ptr(q and q.q),
+          _ptr(q and q.scale), _ptr(qt and qt.q), _ptr(qt and qt.scale), _ptr(cs))
+    return q, qt, cs
+
+
+def fp8_matmul(x, w, bias=None, act="none", out_dtype=torch.bfloat16):
+    """x, w: Fp8Rows with the same contraction -> act(x @ w.T + bias) [x.rows, w.rows]."""
+    _require(x.cols == w.cols, f"fp8_matmul: contractions of {x.cols} and {w.cols}")
+    _require(out_dtype in _DTYPES and act in _lib.PN_ACT, f"fp8_matmul: output {out_dtype}, activation {act!r}")
+    _require(x.q.device == w.q.device, f"fp8_matmul: operands on {x.q.device} and {w.q.device}")
+    if bias is not None:
+        _check("fp8_matmul", bias)
+        _require(bias.shape == (w.rows,) and bias.device == x.q.device, f"fp8_matmul: the bias has shape [{w.rows}]")
+        bias = bias.contiguous()
+    out = torch.empty((x.rows, w.rows), dtype=out_dtype, device=x.q.device)
+    _call("pn_fp8_gemm", out.device, x.q.data_ptr(), x.scale.data_ptr(), x.rows, w.q.data_ptr(), w.scale.data_ptr(), w.rows,
+          x.cols, _ptr(bias), _DTYPES[bias.dtype] if bias is not None else 0, _lib.PN_ACT[act], _DTYPES[out_dtype], out.data_ptr(),
+          w.rows)
+    return out
+
+
+class Fp8Weight:
+    """A layer's weight [N, K] laid out once for fp8_linear: e4m3 bytes, one scale for each 128 x 128 tile."""
+
+    def __init__(self, weight, bias=None):
+        _check("Fp8Weight", weight)
+        _require(weight.dim() == 2 and weight.shape[0] >= 1, "Fp8Weight: a weight [out_features, in_features]")
+        self.data = fp8_quantize(weight.detach(), 128)[0]
+        self._set_bias(bias)
+
+    def _set_bias(self, bias):
+        self.out_features, self.in_features = self.data.rows, self.data.cols
+        if bias is not None:
+            _check("Fp8Weight", bias)
+            _require(bias.shape == (self.out_features,) and bias.device == self.data.q.device,
+                     f"Fp8Weight: the bias has shape [{self.out_features}]")
+            bias = bias.detach().contiguous()
+        self.bias = bias
+
+    @classmethod
+    def from_blocks(cls, values, exponents, bias=None):
+        """values: float8_e4m3fn [N, K]; exponents: integers [ceil(N / 128), ceil(K / 128)], the weight of tile (i, j) being
+        values * 2^exponents[i, j] (-126 to 127)."""
+        _require(values.device.type == "cuda" and exponents.device == values.device,
+                 "Fp8Weight: tensors must live on the GPU (no CPU fallback)")
+        _require(values.dtype == torch.float8_e4m3fn and values.dim() == 2 and min(values.shape) >= 1,
+                 "Fp8Weight: values are float8_e4m3fn [out_features, in_features]")
+        N, K = values.shape
+        nb, kb = -(-N // 128), -(-K // 128)
+        _require(exponents.shape == (nb, kb) and not exponents.is_floating_point(), f"Fp8Weight: exponents are integers [{nb}, {kb}]")
+        self = cls.__new__(cls)
+        d = self.data = Fp8Rows(N, K, values.device)
+        d.q.zero_()[:, :K] = values.view(torch.uint8)
+        bytes_ = torch.nn.functional.pad((exponents + 127).clamp(1, 254).to(torch.uint8), (0, d.scale.shape[0] * 4 - kb))
+        d.scale.copy_(bytes_.repeat_interleave(128, 0)[:N].view(N, -1, 4).permute(1, 0, 2))
+        self._set_bias(bias)
+        return self
+
+
+def fp8_linear(x, weight, act="none", out_dtype=None):
+    """act(x @ W.T + bias) [..., N] for x [..., K] and an Fp8Weight: x is laid out in blocks of 1 x 128 on the way.
+    out_dtype: fp32 or bf16 (default: x's).  Forward only; fp8_linear_train is the form with gradients."""
+    _check("fp8_linear", x)
+    _require(isinstance(weight, Fp8Weight), "fp8_linear: the weight is an Fp8Weight")
+    _require(x.shape[-1] == weight.in_features, f"fp8_linear: rows of {x.shape[-1]} for a weight of {weight.in_features}")
+    _require(x.device == weight.data.q.device, f"fp8_linear: x on {x.device}, the weight on {weight.data.q.device}")
+    _require(not _wants_grad(x), "fp8_linear: forward only (fp8_linear_train has gradients)")
+    q = fp8_quantize(x)[0]
+    out = fp8_matmul(q, weight.data, weight.bias, act, x.dtype if out_dtype is None else out_dtype)
+    return out.view(*x.shape[:-1], weight.out_features)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        xq, xt, _ = fp8_quantize(x, 1, True, need_w)
+        wq, wt, _ = fp8_quantize(weight, 128, True, need_x)
+        y = fp8_matmul(xq, wq, bias, "none", x.dtype).view(*x.shape[:-1], weight.shape[0])
+        ctx.x_t, ctx.w_t = xt, wt              # one byte an element; x and the weight themselves are not kept
+        ctx.meta = (x.shape, weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        shape, w_dtype, b_dtype = ctx.meta
+        dx = dw = db = None
+        gv = _rows(g)
+        M, N = gv.shape
+        if need_x or need_w:
+            gq, gt, cs = fp8_quantize(gv, 1, need_x, need_w, need_b)
+        elif need_b:
+            cs = fp8_quantize(gv, 1, True, False, True)[2]
+        if need_x:
+            dx = fp8_matmul(gq, ctx.w_t, None, "none", g.dtype).view(shape)
+        if need_w:
+            if M == 0:
+                dw = torch.zeros((N, shape[-1]), dtype=w_dtype, device=g.device)
+            else:
+                dw = fp8_matmul(gt, ctx.x_t, None, "none", w_dtype)
+        if need_b:
+            db = torch.empty(N, dtype=b_dtype, device=g.device)
+            _call("pn_fp8_colsum", g.device, cs.data_ptr(), M, N, _DTYPES[b_dtype], db.data_ptr())
+        return dx, dw, db
+
+
+def fp8_linear_train(x, weight, bias=None):
+    """x @ weight.T + bias for x [..., K], weight [N, K] (fp32 or bf16 master weight), with every product in fp8:
+      y = Q(x) Qw(weight)^T + bias,  dx = Q(g) Qw(weight),  dweight = Q(g^T) Q(x^T)^T,  dbias = column sums of g (fp32 sums of g
+    itself), where Q rounds in blocks of 1 x 128 along the product's contraction and Qw in 128 x 128 tiles; the rounding's own
+    derivative is taken as one.  dweight and dbias come in the parameters' types."""
+    _check("fp8_linear_train", *[t for t in (x, weight, bias) if t is not None])
+    _require(x.dim() >= 1 and weight.dim() == 2 and min(weight.shape) >= 1 and x.shape[-1] == weight.shape[1],
+             f"fp8_linear_train: x {tuple(x.shape)} for a weight {tuple(weight.shape)}")
+    _require(bias is None or bias.shape == (weight.shape[0],), f"fp8_linear_train: the bias has shape [{weight.shape[0]}]")
+    return _Fp8Linear.apply(x, weight, bias)

@@ -1,0 +1,126 @@
+"""Feed-forward operators without a GPU: the generator's published test vectors, the oracle's rounding against torch's own
+e4m3 conversion, and what the entry points refuse (Python and C ABI)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import ffn_oracle as fo
+from pillarnet_lts_amd import _lib, ffn_ops
+from pillarnet_lts_amd._lib import PillarnetHipError
+
+
+@pytest.mark.parametrize("counter,key,want", [
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))])
+def test_generator_matches_its_published_vectors(counter, key, want):
+    got = fo.philox4x32([np.array([c], dtype=np.uint64) for c in counter], key)
+    assert tuple(int(v[0]) for v in got) == want
+
+
+def test_oracle_rounding_equals_the_types_own():
+    x = np.concatenate([np.linspace(-460, 460, 40001), 2.0 ** np.arange(-14, 9), -(2.0 ** np.arange(-14, 9)) * 1.0625])
+    x = x.astype(np.float32)
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).double().numpy()
+    inside = np.abs(x) <= 448
+    np.testing.assert_array_equal(fo.round_e4m3(x)[inside], want[inside])
+    assert np.isnan(fo.round_e4m3(np.array([np.inf, -np.inf, np.nan, 1e4]))).all()
+
+
+def test_block_exponent_is_the_smallest_that_holds_the_block():
+    v = np.array([[448.0], [448.5], [447.0], [1.75], [1.7500001], [0.0], [2.0 ** -140], [3e38]]).astype(np.float32)
+    e = fo.block_exponents(v.astype(np.float64), 1)[:, 0]
+    assert list(e[:3]) == [0, 1, 0] and list(e[3:5]) == [-8, -7] and list(e[5:7]) == [-126, -126]
+    assert (np.abs(v[:, 0]) <= 448 * np.exp2(e.astype(np.float64))).all()
+
+
+def test_threshold_keeps_its_range():
+    t = ffn_ops.dropout_threshold
+    assert (t(0.0), t(1.0), t(0.5), t(1e-9), t(1 - 1e-9)) == (0, 65536, 32768, 1, 65535)
+    for p in (0.0, 1e-9, 0.1, 0.3, 0.5, 1 - 1e-9, 1.0):
+        assert t(p) == fo.threshold(p)
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(PillarnetHipError):
+            t(p)
+
+
+def test_host_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.zeros(8)
+    for call in (lambda: ffn_ops.act_dropout(x, 0.5, torch.zeros(2, dtype=torch.int64)),
+                 lambda: ffn_ops.residual_norm(x, x, norm=ffn_ops.Norm("layer", w, w)),
+                 lambda: ffn_ops.fp8_quantize(x), lambda: ffn_ops.Fp8Weight(x),
+                 lambda: ffn_ops.Fp8Weight.from_blocks(x.to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.int32)),
+                 lambda: ffn_ops.fp8_linear_train(x, x), lambda: ffn_ops.DropoutState(1, "cpu")):
+        with pytest.raises(PillarnetHipError, match="GPU"):
+            call()
+    with pytest.raises(PillarnetHipError):
+        ffn_ops.Norm("group", w, w)
+
+
+def _join(**kw):
+    d = dict(dtype=0, param_dtype=0, post_kind=0, norm_kind=1, act=0, cols=8, rows=4, rows_per_gate=4, ldx=8, ldb=8, scale=1.0,
+             post_eps=1e-5, norm_eps=1e-5, threshold=0, call=0, x=16, branch=16)
+    d.update(kw)
+    return _lib.pnResidualNorm(**d)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=2), dict(param_dtype=7), dict(cols=0), dict(cols=16385), dict(rows=-1), dict(post_kind=3), dict(norm_kind=4),
+    dict(act=2), dict(branch=None, gate=16), dict(branch=None, post_kind=1), dict(branch=None, threshold=5, rng=16),
+    dict(branch=None, norm_kind=0), dict(threshold=65537, rng=16), dict(threshold=1), dict(call=65536), dict(x=None),
+    dict(ldx=7), dict(ldb=7), dict(gate=16, rows_per_gate=3), dict(gate=16, rows_per_gate=0)])
+def test_residual_norm_arguments_are_checked_before_the_gpu(bad):
+    L = _lib.lib()
+    s = _join(**bad)
+    assert L.pn_residual_norm_forward(ctypes.byref(s), 16, 16, None, None) == -1 and L.pn_last_error()
+    assert L.pn_residual_norm_backward(ctypes.byref(s), 16, 16, 16, 16, 16, None, None, None, None, None, None, 16, 1 << 20, None) == -1
+    assert L.pn_residual_norm_workspace_bytes(ctypes.byref(s)) == 0
+
+
+def test_residual_norm_outputs_and_workspace_are_checked():
+    L = _lib.lib()
+    s = _join()
+    p = ctypes.byref(s)
+    assert L.pn_residual_norm_forward(None, 16, 16, None, None) == -1
+    assert L.pn_residual_norm_forward(p, None, 16, None, None) == -1 and L.pn_residual_norm_forward(p, 16, None, None, None) == -1
+    assert L.pn_residual_norm_forward(p, 16, 16, 20, None) == -1                       # statistics off their alignment
+    back = lambda h=16, st=16, gh=16, gy=16, df=None, dg=None, ws=16, n=1 << 20, q=p: L.pn_residual_norm_backward(
+        q, h, st, gh, gy, 16, df, None, None, None, None, dg, ws, n, None)
+    assert back(gh=None, gy=None) == -1 and back(h=None) == -1 and back(st=None) == -1
+    assert back(df=16) == -1                                                            # the branch's gradient is dx here
+    assert back(dg=16) == -1
+    assert back(n=8) == -2 and b"workspace" in L.pn_last_error() and back(ws=None) == -2
+    assert L.pn_residual_norm_workspace_bytes(p) >= 2 * 8 * 4
+    none = _join(rows=0)
+    assert L.pn_residual_norm_forward(ctypes.byref(none), None, None, None, None) == 0  # nothing to do, nothing launched
+
+
+def test_dropout_and_fp8_arguments_are_checked_before_the_gpu():
+    L = _lib.lib()
+    fwd = lambda dt=0, x=16, r=2, c=8, ld=8, act=0, t=5, rng=16, call=0, y=16: L.pn_act_dropout_forward(
+        dt, x, r, c, ld, act, t, rng, call, y, None)
+    for bad in (dict(dt=3), dict(x=None), dict(r=-1), dict(ld=7), dict(act=3), dict(t=65537), dict(rng=None), dict(call=65536),
+                dict(y=None), dict(r=1 << 40, c=1 << 10)):
+        assert fwd(**bad) == -1 and L.pn_last_error()
+    assert fwd(r=0, x=None, y=None) == 0
+    assert L.pn_act_dropout_backward(0, 16, None, 2, 8, 8, 8, 2, 5, 16, 0, 16, None) == -1      # gelu needs x
+    assert L.pn_act_dropout_backward(0, None, 16, 2, 8, 8, 8, 1, 5, 16, 0, 16, None) == -1
+    assert L.pn_dropout_draw(None, 16, None) == -1
+    q = lambda dt=0, x=16, r=4, c=8, ld=8, b=1, q=16, s=16, qt=None, st=None: L.pn_fp8_quantize(dt, x, r, c, ld, b, q, s, qt, st, None, None)
+    for bad in (dict(dt=2), dict(x=None), dict(r=-1), dict(c=0), dict(ld=7), dict(b=64), dict(q=None), dict(s=None), dict(qt=16),
+                dict(q=24)):
+        assert q(**bad) == -1
+    assert q(r=0) == 0
+    g = lambda x=16, m=4, w=16, n=8, k=8, act=0, od=0, out=16, ldo=8: L.pn_fp8_gemm(x, 16, m, w, 16, n, k, None, 0, act, od, out, ldo, None)
+    for bad in (dict(x=None), dict(m=-1), dict(w=None), dict(n=0), dict(k=0), dict(act=3), dict(od=2), dict(out=None), dict(ldo=7),
+                dict(x=24)):
+        assert g(**bad) == -1
+    assert g(m=0) == 0
+    assert L.pn_fp8_colsum(None, 4, 8, 0, 16, None) == -1 and L.pn_fp8_colsum(16, 4, 8, 5, 16, None) == -1
+
+
+def test_struct_layout_matches_header():
+    assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers

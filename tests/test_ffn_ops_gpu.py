@@ -1,0 +1,628 @@
+"""Feed-forward operators on the GPU against oracle/ffn_oracle.py (64 bits).
+
+Tolerances are counted in half steps of the types, u = eps / 2 relative to the value a rounding acts on:
+  dropout      two fp32 roundings (scale, product) and the output's; GELU adds an absolute error of |x| * 4u (erff within
+               2 ulp = 4u of a value below 1, its argument's two roundings times max |t erf'(t)| = 0.49, the sum's rounding,
+               all halved by the factor 0.5: 3.5u).
+  norms        a sum over a row takes at most 8 K serial, 6 shuffle and 16 cross-wave additions (K <= 2): 38 roundings, and as
+               many for the second statistic, so every normalised value is within 96u of r * (|t| + mean |t|) + |n|; the
+               gradients add two more such sums.
+  column sums  R rows (and chunks) are added in fp32: (R + 64)u of the sum of magnitudes, plus what the summands are off.
+  fp8          bytes and scales are exact.  Products: whole numbers below 2^24 are exact; an fp32 result may be off by one step
+               for each of K additions, 2K u of the sum of magnitudes.  A bf16 result comes from the fp8 matrix instruction, which
+               drops from each product what lies 2^-16 below the largest of its eight (measured with single pairs of products):
+               up to 7 * 2^-16 of that largest product more, so 7 * 2^-16 of the sum of magnitudes."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import ffn_oracle as fo
+from pillarnet_lts_amd import ffn_ops
+from pillarnet_lts_amd._lib import PillarnetHipError
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+
+
+def d(t):
+    return t.detach().double().cpu().numpy()
+
+
+def within(got, want, tol, what=""):
+    got = d(got)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(got - want) / np.maximum(tol, 1e-300)):.3g} x tolerance"
+
+
+def rng_of(seed, offset, cuda):
+    return torch.tensor([seed, offset], dtype=torch.int64, device=cuda)
+
+
+# ---- activation + dropout ----------------------------------------------------------------------------------------------
+@BOTH
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("shape", [(1,), (1, 1), (3, 7), (5, 8), (2, 3, 64), (129, 257), (1000, 33)])
+@pytest.mark.parametrize("p", [0.0, 0.3, 1.0])
+def test_act_dropout(cuda, dtype, act, shape, p):
+    rs = np.random.RandomState(len(shape) * 7 + shape[0])
+    seed, off, call = 0x1234567890ABCDEF, (5 << 32) + 77, 11
+    x = torch.from_numpy(rs.randn(*shape).astype(np.float32) * 2).to(dtype).to(cuda).requires_grad_()
+    g = torch.from_numpy(rs.randn(*shape).astype(np.float32)).to(dtype).to(cuda)
+    y = ffn_ops.act_dropout(x, p, rng_of(seed, off, cuda) if p else None, call, act)
+    xd, gd = d(x), d(g)
+    k = fo.drop_scale(p, seed, off, call, shape)
+    want = fo.act(xd, act) * k
+    extra = 4 * U32 * np.abs(xd) * k if act == "gelu" else 0.0
+    within(y, want, (U[dtype] + 3 * U32) * np.abs(want) + extra, "y")
+    if y is x:
+        assert act == "none" and p == 0
+        return
+    dx, = torch.autograd.grad(y, x, g)
+    want = gd * k * fo.act_grad(xd, act)
+    # gelu': Phi within 4u, x phi(x) <= 0.25 within 8u (exp 2 ulp = 4u, its argument's rounding times |x^2 / 2| phi: 1u, products)
+    extra = 8 * U32 * np.abs(gd) * k * (1 + np.abs(xd)) if act == "gelu" else 0.0
+    within(dx, want, (U[dtype] + 4 * U32) * np.abs(want) + extra, "dx")
+    assert (d(dx)[k == 0] == 0).all() and (d(y)[k == 0] == 0).all()
+
+
+@BOTH
+def test_act_dropout_strides_and_masked_places(cuda, dtype):
+    """the mask goes by the element's index, whatever the strides; nothing behind a dropped element gets out."""
+    rs = np.random.RandomState(3)
+    wide = torch.from_numpy(rs.randn(37, 90).astype(np.float32)).to(dtype).to(cuda)
+    rng = rng_of(99, 1, cuda)
+    base = ffn_ops.act_dropout(wide[:, 3:72].contiguous(), 0.4, rng)
+    assert torch.equal(ffn_ops.act_dropout(wide[:, 3:72], 0.4, rng), base)                       # odd offset, odd stride
+    assert torch.equal(ffn_ops.act_dropout(wide[:, 3:72].t().contiguous().t(), 0.4, rng), base)  # column-major
+    even = wide[:, 8:72]
+    assert torch.equal(ffn_ops.act_dropout(even, 0.4, rng), ffn_ops.act_dropout(even.contiguous(), 0.4, rng))
+    x = wide[:, 3:72].clone()
+    kept = torch.from_numpy(fo.drop_scale(0.4, 99, 1, 0, (37, 69)) > 0).to(cuda)
+    x[~kept] = torch.tensor([math.nan, math.inf, -math.inf], device=cuda, dtype=dtype).repeat((~kept).sum() // 3 + 1)[: (~kept).sum()]
+    for act in ("none", "relu", "gelu"):
+        xl = x.clone().requires_grad_()
+        y = ffn_ops.act_dropout(xl, 0.4, rng, 0, act)
+        assert torch.isfinite(y).all() and (y[~kept] == 0).all()
+        gr = torch.where(kept, 1.0, math.nan).to(dtype)
+        dx, = torch.autograd.grad(y, xl, gr)
+        assert (dx[~kept] == 0).all() if act != "relu" else not torch.isnan(dx[~kept]).any()
+        assert torch.isfinite(dx).all()
+        e, = torch.autograd.grad(ffn_ops.act_dropout(xl, 0.4, rng, 0, act).sum(), xl)            # expanded gradient
+        f, = torch.autograd.grad(ffn_ops.act_dropout(xl, 0.4, rng, 0, act), xl, torch.ones_like(xl))
+        assert torch.equal(e, f)
+
+
+def test_act_dropout_gradient_against_differences(cuda):
+    x = torch.randn(64, 40, generator=torch.Generator().manual_seed(0)).to(cuda)
+    rng, g = rng_of(5, 6, cuda), torch.randn(64, 40, generator=torch.Generator().manual_seed(1)).to(cuda)
+    for act in ("none", "relu", "gelu"):
+        xl = x.clone().requires_grad_()
+        dx, = torch.autograd.grad(ffn_ops.act_dropout(xl, 0.25, rng, 2, act), xl, g)
+        h = 2.0 ** -7                  # truncation h^2/6 max |gelu'''| (< 1.3) * scale 4/3 * |g|; rounding u |y| / h; a ReLU's kink within h
+        step = (ffn_ops.act_dropout(x + h, 0.25, rng, 2, act) - ffn_ops.act_dropout(x - h, 0.25, rng, 2, act)) / (2 * h) * g
+        ok = x.abs() > 2 * h if act == "relu" else torch.ones_like(x, dtype=torch.bool)
+        tol = g.abs() * (h * h / 6 * 1.3 * 4 / 3 + 16 * U32 * (x.abs() + 1) * 4 / 3 / h) + 1e-7
+        assert ((step - dx).abs() <= tol)[ok].all(), act
+
+
+def test_dropout_state_moves_on_and_replays(cuda):
+    st = ffn_ops.DropoutState((1 << 64) - 3, cuda)
+    a, b = st.draw(), st.draw()
+    assert a.tolist() == [-3, 0] and b.tolist() == [-3, 1] and st.state.tolist() == [-3, 2]
+    x = torch.randn(70, 130, device=cuda, dtype=torch.bfloat16)
+    k = fo.drop_scale(0.5, (1 << 64) - 3, 1, 0, (70, 130)) > 0
+    assert np.array_equal(d(ffn_ops.act_dropout(x, 0.5, b)) != 0, k & (d(x) != 0))
+    out = torch.empty_like(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ffn_ops.act_dropout(x, 0.5, st.draw())
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out.copy_(ffn_ops.act_dropout(x, 0.5, st.draw()))
+    for i in range(3, 6):
+        graph.replay()
+        want = ffn_ops.act_dropout(x, 0.5, rng_of(-3, i, cuda))
+        assert torch.equal(out, want), i
+
+
+def test_act_dropout_beyond_32_bit_offsets(cuda):
+    """4.3e9 elements: the last groups have element indices past 2^32."""
+    cols, rows = 1 << 20, 4099
+    x = torch.ones((rows, cols), dtype=torch.bfloat16, device=cuda)
+    y = ffn_ops.act_dropout(x, 0.5, rng_of(7, 8, cuda), 3)
+    for row in (0, 4095, 4096, 4098):
+        k = fo.drop_scale(0.5, 7, 8, 3, (64,), start=row * cols + cols - 64)
+        assert np.array_equal(d(y[row, -64:]), k)
+
+
+def test_act_dropout_refusals(cuda):
+    x, rng = torch.zeros(4, 8, device=cuda), rng_of(1, 2, cuda)
+    for call in (lambda: ffn_ops.act_dropout(x.half(), 0.5, rng), lambda: ffn_ops.act_dropout(x, 0.5), lambda: ffn_ops.act_dropout(x, 1.5, rng),
+                 lambda: ffn_ops.act_dropout(x, 0.5, rng.int()), lambda: ffn_ops.act_dropout(x, 0.5, rng.cpu()),
+                 lambda: ffn_ops.act_dropout(x, 0.5, rng, 65536), lambda: ffn_ops.act_dropout(x, 0.5, rng, act="silu"),
+                 lambda: ffn_ops.act_dropout(torch.zeros((), device=cuda), 0.5, rng)):
+        with pytest.raises(PillarnetHipError):
+            call()
+    for shape in ((0, 8), (4, 0), (0,)):
+        e = torch.zeros(shape, device=cuda, requires_grad=True)
+        y = ffn_ops.act_dropout(e, 0.5, rng, act="gelu")
+        assert y.shape == shape and torch.autograd.grad(y.sum(), e)[0].shape == shape
+
+
+# ---- residual join and norms -------------------------------------------------------------------------------------------
+def _join_case(cuda, dtype, pdtype, B, T, C, post, norm, gate, p, branch, act, scale, seed=0, strided=False):
+    rs = np.random.RandomState(seed + B * 31 + T * 7 + C)
+    n = lambda *s, m=0.0, sd=1.0: torch.from_numpy((rs.randn(*s) * sd + m).astype(np.float32))
+
+    def data(*s, **kw):
+        t = n(*s, **kw).to(dtype).to(cuda)
+        if strided:                             # the same values at an odd offset inside wider rows
+            w = torch.zeros(*s[:-1], s[-1] + 5, dtype=dtype, device=cuda)
+            w[..., 3:3 + s[-1]] = t
+            t = w[..., 3:3 + s[-1]]
+        return t
+
+    par = lambda *s, **kw: n(*s, **kw).to(pdtype).to(cuda).requires_grad_()
+    t = dict(x=data(B, T, C, sd=2.0, m=0.3).requires_grad_())
+    if branch:
+        t["f"] = data(B, T, C, m=0.2).requires_grad_()
+        if gate:
+            t["gate"] = par(*{"channel": (C,), "sample": (B, C), "row": (B, T, C)}[gate], m=0.5)
+        if post:
+            t["pw"], t["pb"] = par(C, m=1.0, sd=0.2), par(C, sd=0.2)
+    if norm:
+        t["w"], t["b"] = par(C, m=1.0, sd=0.2), par(C, sd=0.2)
+    args = dict(scale=scale if branch else 1.0, gate=t.get("gate"), act=act,
+                post_norm=ffn_ops.Norm(post, t["pw"], t["pb"], 1e-5) if post and branch else None,
+                norm=ffn_ops.Norm(norm, t["w"], t["b"], 1e-3) if norm else None,
+                dropout=(p, rng_of(21, 4, cuda), 9) if branch and p else None)
+    return t, args, (lambda: ffn_ops.residual_norm(t["x"], t.get("f"), **args))
+
+
+def _join_check(t, args, out, grads, gh, gy, dtype, pdtype, p, post, norm, gate, act):
+    """h, y and every gradient against the formulas, each from the values the kernels stored."""
+    v = {k: d(q) for k, q in t.items()}
+    shape = v["x"].shape
+    R = shape[0] * shape[1]
+    u = U[dtype]
+    branch = "f" in t
+    y = h = None
+    if branch and norm:
+        h, y = out
+    elif branch:
+        h = out
+    else:
+        y = out
+    s = args["scale"]
+    k = fo.drop_scale(p if branch else 0, 21, 4, 9, shape)
+    if branch:
+        fn, fm, fr = fo.normalise(v["f"], post, 1e-5)
+        fu = fn * v["pw"] + v["pb"] if post else fn
+        ga = v["gate"] if gate else np.ones(1)
+        ga = ga[:, None, :] if gate == "sample" else ga
+        fe = 96 * U32 * (fr * (np.abs(v["f"]) + np.abs(v["f"]).mean(-1, keepdims=True)) + np.abs(fn)) if post else 0 * fn   # of fn
+        ue = fe * np.abs(v.get("pw", 1.0)) + 2 * U32 * np.abs(fu)
+        want = v["x"] + s * ga * fu * k
+        within(h, want, u * np.abs(want) + 4 * U32 * (np.abs(v["x"]) + np.abs(s * ga * fu * k)) + np.abs(s * ga * k) * ue, "h")
+        hv = d(h)
+    else:
+        hv = v["x"]
+    if norm:
+        hn, hm, hr = fo.normalise(hv, norm, 1e-3)
+        stat = norm != "affine"
+        he = 96 * U32 * (hr * (np.abs(hv) + np.abs(hv).mean(-1, keepdims=True)) + np.abs(hn)) if stat else 0 * hn
+        pre = hn * v["w"] + v["b"]
+        want = fo.act(pre, act)
+        pe = he * np.abs(v["w"]) + 3 * U32 * (np.abs(hn * v["w"]) + np.abs(v["b"]))
+        within(y, want, u * np.abs(want) + pe, "y")
+    if grads is None:
+        return
+    zero = np.zeros(shape)
+    dh, de = (d(gh).copy() if gh is not None else zero.copy()), zero.copy()
+    if norm and gy is not None:
+        live = (pre > 0) if act == "relu" else np.ones(shape, bool)
+        sure = (np.abs(pre) > pe) if act == "relu" else np.ones(shape, bool)
+        assert sure.mean() > 0.99
+        live = np.where(sure, live, d(y) > 0)        # within rounding of the kink either side is right: take the kernel's
+        gp = d(gy) * live
+        tw = gp * v["w"]
+        n_ = fo.normalise_grad(tw, hn, hr, norm)
+        A = np.abs(tw) + np.abs(tw).mean(-1, keepdims=True) + np.abs(hn) * np.abs(tw * hn).mean(-1, keepdims=True)
+        if stat:
+            de += hr * (160 * U32 * A + np.abs(tw * he).mean(-1, keepdims=True) * np.abs(hn) + he * np.abs((tw * hn).mean(-1, keepdims=True)))
+        else:
+            de += 3 * U32 * np.abs(tw)
+        dh = dh + n_
+        de += 2 * U32 * (np.abs(dh) + np.abs(n_))
+        for name, q, qe in (("w", gp * hn, np.abs(gp) * he), ("b", gp, zero)):
+            want = q.sum((0, 1))
+            within(grads[name], want, U[pdtype] * np.abs(want) + (R + 64) * U32 * np.abs(q).sum((0, 1)) + qe.sum((0, 1)), "d" + name)
+    within(grads["x"], dh, u * np.abs(dh) + de, "dx")
+    if not branch:
+        return
+    du = s * ga * dh * k
+    due = np.abs(s * ga * k) * (de + 4 * U32 * np.abs(dh))
+    if gate:
+        q, qe = s * dh * fu * k, np.abs(s * k) * (de * np.abs(fu) + np.abs(dh) * ue) + 4 * U32 * np.abs(s * dh * fu * k)
+        ax = {"channel": (0, 1), "sample": 1, "row": ()}[gate]
+        want = q.sum(ax)
+        within(grads["gate"], want, U[pdtype] * np.abs(want) + (R + 64) * U32 * np.abs(q).sum(ax) + qe.sum(ax), "dgate")
+    if post:
+        for name, q, qe in (("pw", du * fn, due * np.abs(fn) + np.abs(du) * fe), ("pb", du, due)):
+            want = q.sum((0, 1))
+            within(grads[name], want, U[pdtype] * np.abs(want) + (R + 64) * U32 * np.abs(q).sum((0, 1)) + qe.sum((0, 1)), "d" + name)
+        tp = du * v["pw"]
+        want = fo.normalise_grad(tp, fn, fr, post)
+        tpe = due * np.abs(v["pw"])
+        A = np.abs(tp) + np.abs(tp).mean(-1, keepdims=True) + np.abs(fn) * np.abs(tp * fn).mean(-1, keepdims=True)
+        e = fr * (160 * U32 * A + tpe + tpe.mean(-1, keepdims=True) + np.abs(fn) * (tpe * np.abs(fn)).mean(-1, keepdims=True)
+                  + np.abs(tp * fe).mean(-1, keepdims=True) * np.abs(fn) + fe * np.abs((tp * fn).mean(-1, keepdims=True)))
+        within(grads["f"], want, u * np.abs(want) + e, "df")
+    else:
+        within(grads["f"], du, u * np.abs(du) + due, "df")
+
+
+def _join_run(cuda, dtype, pdtype, B, T, C, post, norm, gate, p, branch, act="none", scale=0.5, use=("h", "y"), strided=False):
+    t, args, call = _join_case(cuda, dtype, pdtype, B, T, C, post, norm, gate, p, branch, act, scale, strided=strided)
+    out = call()
+    outs = list(out) if isinstance(out, tuple) else [out]
+    names = [n for n, on in (("h", branch), ("y", norm)) if on]
+    gen = torch.Generator().manual_seed(1)
+    g = {n: torch.randn(B, T, C, generator=gen).to(dtype).to(cuda) for n in names}
+    used = [n for n in names if n in use]
+    grads = torch.autograd.grad([o for o, n in zip(outs, names) if n in used], list(t.values()), [g[n] for n in used], allow_unused=True)
+    grads = dict(zip(t, grads))
+    _join_check(t, args, out, grads, g.get("h") if "h" in used else None, g.get("y") if "y" in used else None, dtype, pdtype, p, post,
+                norm, gate, act)
+    with torch.no_grad():
+        again = call()
+    for a, b in zip(outs, again if isinstance(again, tuple) else [again]):
+        assert torch.equal(a, b)                 # serving gives the training pass's bits
+
+
+@BOTH
+@pytest.mark.parametrize("C", [1, 7, 8, 33, 64, 65, 128, 200, 256, 500, 512, 1000, 1024, 2048, 2050, 4096, 5001, 8192, 16384])
+def test_residual_norm_widths(cuda, dtype, C):
+    _join_run(cuda, dtype, dtype, 2, 37, C, "rms", "layer", "channel", 0.1, True)
+
+
+@BOTH
+@pytest.mark.parametrize("post", [None, "layer", "rms"])
+@pytest.mark.parametrize("norm", [None, "layer", "rms", "affine"])
+@pytest.mark.parametrize("gate", [None, "channel", "sample", "row"])
+def test_residual_norm_kinds(cuda, dtype, post, norm, gate):
+    _join_run(cuda, dtype, torch.float32, 3, 41, 72, post, norm, gate, 0.3 if gate != "row" else 0.0, True,
+              act="relu" if norm == "layer" else "none")
+
+
+@BOTH
+@pytest.mark.parametrize("norm", ["layer", "rms", "affine"])
+@pytest.mark.parametrize("B,T", [(1, 1), (1, 2), (5, 1), (4, 700)])
+def test_residual_norm_without_a_branch(cuda, dtype, norm, B, T):
+    _join_run(cuda, dtype, dtype, B, T, 48, None, norm, None, 0.0, False, act="relu")
+
+
+@BOTH
+@pytest.mark.parametrize("use", [("h",), ("y",)])
+def test_residual_norm_with_one_output_used(cuda, dtype, use):
+    _join_run(cuda, dtype, dtype, 2, 19, 96, "rms", "layer", "sample", 0.2, True, use=use)
+    _join_run(cuda, dtype, dtype, 2, 19, 96, None, "layer", None, 0.0, True, scale=1.0, use=use)     # the branch's gradient is dx
+
+
+@BOTH
+@pytest.mark.parametrize("B,T,C", [(1, 1, 256), (300, 1, 64), (7, 1, 5001), (1, 5000, 40), (64, 3, 520)])
+def test_residual_norm_row_counts(cuda, dtype, B, T, C):
+    _join_run(cuda, dtype, dtype, B, T, C, "layer", "rms", "sample", 0.5, True)
+
+
+@BOTH
+def test_residual_norm_strided_rows(cuda, dtype):
+    _join_run(cuda, dtype, dtype, 2, 21, 67, "rms", "layer", "channel", 0.2, True, strided=True)
+    _join_run(cuda, dtype, dtype, 2, 21, 64, None, "layer", None, 0.0, False, strided=True)
+
+
+def test_residual_norm_mixed_parameter_types_and_missing_weights(cuda):
+    x, f = torch.randn(2, 30, 64, device=cuda).bfloat16(), torch.randn(2, 30, 64, device=cuda).bfloat16()
+    w16, g32 = torch.randn(64, device=cuda).bfloat16().requires_grad_(), torch.randn(64, device=cuda, requires_grad=True)
+    h, y = ffn_ops.residual_norm(x, f, gate=g32, norm=ffn_ops.Norm("rms", w16))
+    h2, y2 = ffn_ops.residual_norm(x, f, gate=g32, norm=ffn_ops.Norm("rms", w16.detach().float(), torch.zeros(64, device=cuda)))
+    assert torch.equal(h, h2) and torch.equal(y, y2)
+    dw, dg = torch.autograd.grad(y.float().sum(), (w16, g32))
+    assert dw.dtype == torch.bfloat16 and dg.dtype == torch.float32 and dw.abs().sum() > 0
+    plain = ffn_ops.residual_norm(x, norm=ffn_ops.Norm("layer"))
+    n = fo.normalise(d(x), "layer", 1e-5)[0]
+    within(plain, n, U[torch.bfloat16] * np.abs(n) + 1e-5, "y")
+
+
+def test_residual_norm_masked_branch_and_equal_rows(cuda):
+    """infinities behind dropped elements do not reach h or the gradients; a constant row has variance zero."""
+    x = torch.randn(8, 64, device=cuda, requires_grad=True)
+    f = torch.randn(8, 64, device=cuda)
+    kept = torch.from_numpy(fo.drop_scale(0.5, 21, 4, 9, (8, 64)) > 0).to(cuda)
+    f = torch.where(kept, f, math.inf).requires_grad_()
+    gate = torch.randn(64, device=cuda, requires_grad=True)
+    h, y = ffn_ops.residual_norm(x, f, gate=gate, norm=ffn_ops.Norm("layer"), dropout=(0.5, rng_of(21, 4, cuda), 9))
+    grads = torch.autograd.grad((h, y), (x, f, gate), (torch.randn_like(h), torch.randn_like(y)))
+    assert all(torch.isfinite(q).all() for q in (h, y, *grads)) and (grads[1][~kept] == 0).all()
+    c = torch.full((5, 100), 3.25, device=cuda)
+    assert (ffn_ops.residual_norm(c, norm=ffn_ops.Norm("layer")) == 0).all()
+
+
+def test_residual_norm_gradient_against_differences(cuda):
+    t, args, call = _join_case(cuda, torch.float32, torch.float32, 2, 6, 24, "rms", "layer", "sample", 0.25, True, "none", 0.5)
+    gen = torch.Generator().manual_seed(2)
+    gh, gy = torch.randn(2, 6, 24, generator=gen).to(cuda), torch.randn(2, 6, 24, generator=gen).to(cuda)
+    grads = dict(zip(t, torch.autograd.grad(call(), list(t.values()), (gh, gy))))
+    loss = lambda: sum((o.double() * g.double()).sum().item() for o, g in zip(call(), (gh, gy)))
+    gen = torch.Generator().manual_seed(3)
+    for name, leaf in t.items():
+        v = torch.randn(leaf.shape, generator=gen).to(cuda)
+        slope = (grads[name].double() * v.double()).sum().item()
+        keep, step = leaf.detach().clone(), 2.0 ** -7
+        with torch.no_grad():
+            leaf.copy_(keep + step * v); up = loss()
+            leaf.copy_(keep - step * v); down = loss()
+            leaf.copy_(keep)
+        got = (up - down) / (2 * step)
+        # rounding: 576 outputs of size <= 8 with gradients of size 1, each within 8u, added at random: 24 * 64 * u / step; truncation:
+        # step^2 / 6 times a third derivative along v, which is below the slope's own scale times 100 for rows of 24
+        scale_ = grads[name].double().norm().item() * v.double().norm().item()
+        assert abs(got - slope) <= 24 * 64 * U32 / step + step * step / 6 * 100 * scale_, (name, got, slope)
+
+
+def test_residual_norm_repeats_its_bits(cuda):
+    t, args, call = _join_case(cuda, torch.bfloat16, torch.float32, 4, 900, 256, "rms", "layer", "sample", 0.1, True, "none", 0.5)
+    g = [torch.randn(4, 900, 256, device=cuda).bfloat16() for _ in range(2)]
+    first = torch.autograd.grad(call(), list(t.values()), g)
+    for _ in range(3):
+        for a, b in zip(first, torch.autograd.grad(call(), list(t.values()), g)):
+            assert torch.equal(a, b)
+
+
+def test_residual_norm_refusals(cuda):
+    x = torch.zeros(4, 6, 8, device=cuda)
+    w, N = torch.zeros(8, device=cuda), ffn_ops.Norm
+    for call in (lambda: ffn_ops.residual_norm(x), lambda: ffn_ops.residual_norm(x, x.bfloat16(), norm=N("layer")),
+                 lambda: ffn_ops.residual_norm(x, x[:2]), lambda: ffn_ops.residual_norm(x, gate=w, norm=N("rms")),
+                 lambda: ffn_ops.residual_norm(x, x, gate=torch.zeros(3, 8, device=cuda)), lambda: ffn_ops.residual_norm(x, x, act="relu"),
+                 lambda: ffn_ops.residual_norm(x, x, gate=w[:7]), lambda: ffn_ops.residual_norm(x, x, post_norm=N("affine", w)),
+                 lambda: ffn_ops.residual_norm(x, norm=N("layer", w[:4])), lambda: ffn_ops.residual_norm(x, norm=N("layer", w.double())),
+                 lambda: ffn_ops.residual_norm(x, norm=N("layer", w.cpu())), lambda: ffn_ops.residual_norm(x, x, dropout=(0.5, None, 0)),
+                 lambda: ffn_ops.residual_norm(x, x, norm=N("rms"), act="gelu"), lambda: ffn_ops.residual_norm(x.half(), norm=N("rms")),
+                 lambda: ffn_ops.residual_norm(torch.zeros(2, 16385, device=cuda), norm=N("rms"))):
+        with pytest.raises(PillarnetHipError):
+            call()
+    e, g = torch.zeros(0, 6, 8, device=cuda, requires_grad=True), torch.ones(8, device=cuda, requires_grad=True)
+    h, y = ffn_ops.residual_norm(e, e * 2, gate=g, norm=N("layer", g))
+    de, dg = torch.autograd.grad(y.sum() + h.sum(), (e, g))
+    assert h.shape == y.shape == de.shape == (0, 6, 8) and (dg == 0).all()
+
+
+# ---- fp8 ---------------------------------------------------------------------------------------------------------------
+def _values(rs, R, C, dtype):
+    x = rs.randn(R, C) * np.exp(rs.randn(R, 1) * 3) * np.exp(rs.randn(1, C))
+    x[rs.rand(R, C) < 0.05] = 0
+    return torch.from_numpy(x.astype(np.float32)).to(dtype)
+
+
+@BOTH
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("R,C", [(1, 1), (1, 128), (3, 129), (127, 64), (128, 128), (129, 300), (700, 515), (260, 1024)])
+def test_fp8_quantize_is_exact(cuda, dtype, block_rows, R, C):
+    x = _values(np.random.RandomState(R + C), R, C, dtype)
+    q, qt, cs = ffn_ops.fp8_quantize(x.to(cuda), block_rows, True, True, True)
+    want = fo.quantise(d(x), block_rows)
+    wt = fo.quantise(d(x).T, 1) if block_rows == 1 else want.T
+    np.testing.assert_array_equal(d(q.values()), want)
+    np.testing.assert_array_equal(d(qt.values()), wt)
+    assert (q.q[:, C:] == 0).all() and (qt.q[:, R:] == 0).all()               # padding that products run over
+    e = fo.block_exponents(d(x), block_rows).repeat(block_rows, 0)[:R] + 127
+    got = q.scale.permute(1, 0, 2).reshape(R, -1)[:, : e.shape[1]].cpu().numpy()
+    np.testing.assert_array_equal(got, e)
+    blocks = np.add.reduceat(np.abs(d(x)), np.arange(0, R, 128), 0)
+    within(cs, np.add.reduceat(d(x), np.arange(0, R, 128), 0), 128 * U32 * blocks, "column sums")
+    q2 = ffn_ops.fp8_quantize(x.to(cuda), block_rows)[0]
+    assert torch.equal(q2.q, q.q)
+    wide = torch.zeros(R, C + 7, dtype=dtype, device=cuda)
+    wide[:, 3:3 + C] = x.to(cuda)
+    q3 = ffn_ops.fp8_quantize(wide[:, 3:3 + C], block_rows, True, True)
+    assert torch.equal(q3[0].q, q.q) and torch.equal(q3[1].q, qt.q)
+
+
+@BOTH
+def test_fp8_quantize_extremes(cuda, dtype):
+    x = torch.zeros(6, 256)
+    x[0, 5], x[1, 7], x[2, 9] = math.inf, -math.inf, math.nan
+    x[0, :4], x[2, 128:] = 100.0, 3.0
+    x[3, 0], x[3, 1] = 2.0 ** -130, 3e38                                       # fp32 subnormal next to the largest values
+    x[4, :2] = torch.tensor([2.0 ** -133, 2.0 ** -149])
+    x = x.to(dtype)
+    got = d(ffn_ops.fp8_quantize(x.to(cuda))[0].values())
+    want = fo.quantise(d(x))
+    np.testing.assert_array_equal(got, want)
+    # 100 = 400 / 4 in its block; 400 lies halfway between 384 and 416, and 384 (mantissa 100) is the even one: 96
+    assert np.isnan(got[0, 5]) and np.isnan(got[1, 7]) and np.isnan(got[2, 9]) and got[0, 0] == 96 and got[2, 200] == 3
+
+
+SHAPES = [(1, 1, 1), (1, 128, 16), (1, 515, 33), (2, 1000, 129), (7, 256, 7), (16, 384, 256), (17, 130, 64), (33, 640, 100), (64, 512, 200),
+          (65, 127, 257), (128, 128, 128), (129, 1152, 130), (300, 257, 1), (500, 3136, 256), (513, 300, 515), (1030, 96, 1025)]
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+@BOTH
+def test_fp8_matmul_exact_on_whole_numbers(cuda, dtype, M, K, N):
+    """whole numbers times block scales: every partial sum is a whole number below 2^24 times one power of two, so the result has
+    to be exact, whatever the order of the sums."""
+    rs = np.random.RandomState(M + K + N)
+    x, w = rs.randint(-8, 9, (M, K)).astype(np.float64), rs.randint(-8, 9, (N, K)).astype(np.float64)
+    sx, sw = 2.0 ** rs.randint(-2, 3, (M, 1)), 2.0 ** rs.randint(-2, 3, (1, 1))
+    kb = np.arange(K) // 128                                                    # blocks differ in scale; products stay whole / 256
+    x, w = x * 2.0 ** (kb % 3) * sx, w * 2.0 ** -(kb % 3) * sw
+    b = rs.randint(-4, 5, N).astype(np.float32)
+    xt, wt = torch.from_numpy(x).float().to(dtype).to(cuda), torch.from_numpy(w).float().to(cuda)
+    assert np.array_equal(d(xt), x)
+    want = x @ w.T + b
+    y = ffn_ops.fp8_linear(xt, ffn_ops.Fp8Weight(wt, torch.from_numpy(b).to(cuda)), out_dtype=torch.float32)
+    np.testing.assert_array_equal(d(y), want)
+    r = ffn_ops.fp8_linear(xt.view(1, M, K), ffn_ops.Fp8Weight(wt), act="relu", out_dtype=torch.bfloat16)
+    want = torch.from_numpy(np.maximum(x @ w.T, 0)).to(torch.bfloat16).double().numpy()[None]
+    np.testing.assert_array_equal(d(r), want)
+
+
+def _product_tol(a, b, dtype, out):
+    return (2 * a.shape[1] * U32 + (7 * 2.0 ** -16 if dtype == torch.bfloat16 else 0)) * (np.abs(a) @ np.abs(b).T) + U[dtype] * np.abs(out) + 4 * U32 * np.abs(out)
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+@BOTH
+def test_fp8_linear_against_64_bits(cuda, dtype, M, K, N):
+    rs = np.random.RandomState(M * 3 + K + N)
+    x, w = _values(rs, M, K, dtype), torch.from_numpy((rs.randn(N, K) / K ** 0.5).astype(np.float32))
+    b = torch.from_numpy(rs.randn(N).astype(np.float32))
+    xq, wq = fo.quantise(d(x)), fo.quantise(d(w), 128)
+    plan = ffn_ops.Fp8Weight(w.to(cuda), b.to(cuda))
+    pre = xq @ wq.T + d(b)
+    for act in ("none", "relu", "gelu"):
+        want = fo.act(pre, act)
+        tol = 1.13 * (_product_tol(xq, wq, dtype, 0 * pre) + 8 * U32 * np.abs(pre) + U32 * np.abs(d(b))) + 4 * U32 * np.abs(pre) + U[dtype] * np.abs(want)   # |gelu'| <= 1.13
+        got = ffn_ops.fp8_linear(x.to(cuda), plan, act)
+        assert got.dtype == dtype
+        within(got, want, tol, act)
+    if K * N >= 4096 and M >= 16:               # at random, K roundings of 2u add up to about 2u sqrt(K) of the result
+        got = d(ffn_ops.fp8_linear(x.to(cuda), plan, out_dtype=torch.float32))
+        assert np.linalg.norm(got - pre) <= 4 * U32 * math.sqrt(K) * np.linalg.norm(pre)
+
+
+def test_fp8_weight_from_blocks_and_infinities(cuda):
+    rs = np.random.RandomState(0)
+    w = torch.from_numpy(rs.randn(200, 300).astype(np.float32)).to(cuda)
+    a = ffn_ops.Fp8Weight(w)
+    e = torch.from_numpy(fo.block_exponents(d(w), 128)).to(cuda)
+    v = (w * torch.exp2(-e.float()).repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)[:, :300]).to(torch.float8_e4m3fn)
+    b = ffn_ops.Fp8Weight.from_blocks(v, e)
+    assert torch.equal(a.data.q, b.data.q) and torch.equal(a.data.values(), b.data.values())
+    x = torch.randn(5, 300, device=cuda)
+    x[2, 17] = math.inf
+    y = ffn_ops.fp8_linear(x, b)
+    assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3, 4]]).all()     # an infinity marks its own row only
+    z = ffn_ops.fp8_linear(torch.zeros(3, 300, device=cuda), b)
+    assert (z == 0).all()
+
+
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16], ids=["w32", "w16"])
+@BOTH
+@pytest.mark.parametrize("M,K,N,bias", [(1, 8, 8, True), (5, 130, 260, False), (130, 257, 96, True), (512, 640, 256, True), (700, 129, 515, False)])
+def test_fp8_linear_train(cuda, dtype, wdtype, M, K, N, bias):
+    rs = np.random.RandomState(M + K)
+    x = _values(rs, M, K, dtype).to(cuda).requires_grad_()
+    w = torch.from_numpy((rs.randn(N, K) / K ** 0.5).astype(np.float32)).to(wdtype).to(cuda).requires_grad_()
+    b = torch.from_numpy(rs.randn(N).astype(np.float32)).to(cuda).requires_grad_() if bias else None
+    g = _values(rs, M, N, dtype).to(cuda)
+    y = ffn_ops.fp8_linear_train(x.view(1, M, K), w, b)[0]
+    leaves = [x, w] + ([b] if bias else [])
+    dx, dw, *db = torch.autograd.grad(y, leaves, g)
+    xq, wq = fo.quantise(d(x)), fo.quantise(d(w), 128)
+    want = xq @ wq.T + (d(b) if bias else 0)
+    within(y, want, _product_tol(xq, wq, dtype, want) + (U32 * np.abs(d(b)) if bias else 0), "y")
+    gq, gt, xt = fo.quantise(d(g)), fo.quantise(d(g).T), fo.quantise(d(x).T)
+    want = gq @ wq
+    within(dx, want, _product_tol(gq, wq.T, dtype, want), "dx")
+    want = gt @ xt.T
+    assert dw.dtype == wdtype
+    within(dw, want, _product_tol(gt, xt, wdtype, want), "dw")
+    if bias:
+        want = d(g).sum(0)
+        within(db[0], want, U32 * np.abs(want) + (M + 8) * U32 * np.abs(d(g)).sum(0), "db")
+
+
+def test_fp8_linear_train_gradient_against_differences(cuda):
+    """where the rounding is exact (small whole numbers) the product is linear, and differences are exact."""
+    rs = np.random.RandomState(4)
+    x = torch.from_numpy(rs.randint(-7, 8, (6, 140)).astype(np.float32)).to(cuda).requires_grad_()
+    w = torch.from_numpy(rs.randint(-7, 8, (10, 140)).astype(np.float32)).to(cuda).requires_grad_()
+    b = torch.from_numpy(rs.randint(-7, 8, 10).astype(np.float32)).to(cuda).requires_grad_()
+    g = torch.from_numpy(rs.randint(-3, 4, (6, 10)).astype(np.float32)).to(cuda)
+    grads = torch.autograd.grad(ffn_ops.fp8_linear_train(x, w, b), (x, w, b), g)
+    for leaf, gr in zip((x, w, b), grads):
+        for at in [(0,) * leaf.dim(), tuple(s - 1 for s in leaf.shape)]:
+            keep = leaf.detach()[at].item()
+            vals = []
+            for s in (1.0, -1.0):
+                with torch.no_grad():
+                    leaf[at] = keep + s
+                    vals.append((ffn_ops.fp8_linear_train(x, w, b) * g).double().sum().item())
+                    leaf[at] = keep
+            assert (vals[0] - vals[1]) / 2 == gr[at].item()
+
+
+def test_fp8_partial_gradients_and_refusals(cuda):
+    x, w = torch.randn(20, 64, device=cuda), torch.randn(32, 64, device=cuda)
+    b = torch.randn(32, device=cuda, requires_grad=True)
+    full = [t.clone().requires_grad_() for t in (x, w)]
+    ref = torch.autograd.grad(ffn_ops.fp8_linear_train(*full, b).sum(), full + [b])
+    for i in range(2):
+        leaves = [t.clone().requires_grad_(k == i) for k, t in enumerate((x, w))]
+        assert torch.equal(torch.autograd.grad(ffn_ops.fp8_linear_train(*leaves, b.detach()).sum(), leaves[i])[0], ref[i])
+    assert torch.equal(torch.autograd.grad(ffn_ops.fp8_linear_train(x, w, b).sum(), b)[0], ref[2])
+    e = torch.zeros(0, 64, device=cuda, requires_grad=True)
+    wl = w.clone().requires_grad_()
+    de, dw, db = torch.autograd.grad(ffn_ops.fp8_linear_train(e, wl, b).sum(), (e, wl, b))
+    assert de.shape == (0, 64) and (dw == 0).all() and (db == 0).all()
+    plan = ffn_ops.Fp8Weight(w)
+    assert ffn_ops.fp8_linear(e.detach(), plan).shape == (0, 32)
+    for call in (lambda: ffn_ops.fp8_linear(x[:, :60], plan), lambda: ffn_ops.fp8_linear(x, w), lambda: ffn_ops.fp8_linear(x.half(), plan),
+                 lambda: ffn_ops.fp8_linear(x.clone().requires_grad_(), plan), lambda: ffn_ops.fp8_linear(x, plan, act="silu"),
+                 lambda: ffn_ops.fp8_linear(x, plan, out_dtype=torch.float16), lambda: ffn_ops.Fp8Weight(w, b[:5]),
+                 lambda: ffn_ops.fp8_linear_train(x, w.t()), lambda: ffn_ops.fp8_linear_train(x, w, b[:3]),
+                 lambda: ffn_ops.fp8_quantize(x, 64), lambda: ffn_ops.fp8_quantize(x, rows=False),
+                 lambda: ffn_ops.Fp8Weight.from_blocks(w.to(torch.float8_e4m3fn), torch.zeros(2, 1, device=cuda, dtype=torch.int32)),
+                 lambda: ffn_ops.Fp8Weight.from_blocks(w, torch.zeros(1, 1, device=cuda, dtype=torch.int32))):
+        with pytest.raises(PillarnetHipError):
+            call()
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------
+def test_feed_forward_block_captured_and_on_another_stream(cuda):
+    """one block as the heads use it -- norm, fp8 product, activation + dropout, fp8 product, residual join -- forward and backward,
+    eagerly, on a side stream, and captured with a draw inside: every replay gives the eager pass's bits for its draw."""
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen).to(cuda)
+    x0, g = r(3, 50, 96), r(3, 50, 96)
+    P = dict(w1=r(192, 96) / 10, b1=r(192), w2=r(96, 192) / 14, b2=r(96), nw=r(96), nb=r(96), gate=r(3, 96), pw=r(96), pb=r(96))
+    st = ffn_ops.DropoutState(42, cuda)
+
+    def step(rng):
+        x, p = x0.clone().requires_grad_(), {k: v.clone().requires_grad_() for k, v in P.items()}
+        n = ffn_ops.residual_norm(x, norm=ffn_ops.Norm("layer", p["nw"], p["nb"]))
+        a = ffn_ops.act_dropout(ffn_ops.fp8_linear_train(n, p["w1"], p["b1"]), 0.2, rng, 0, "gelu")
+        f = ffn_ops.fp8_linear_train(a, p["w2"], p["b2"])
+        h, y = ffn_ops.residual_norm(x, f, gate=p["gate"], scale=0.7, post_norm=ffn_ops.Norm("rms", p["pw"], p["pb"]),
+                                     norm=ffn_ops.Norm("layer", p["nw"], p["nb"]), dropout=(0.1, rng, 1))
+        return [h, y, *torch.autograd.grad((h, y), [x, *p.values()], (g, g))]
+
+    want = [[t.detach().clone() for t in step(rng_of(42, i, cuda))] for i in range(4)]
+    assert any(not torch.equal(a, b) for a, b in zip(want[0], want[1]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(st.draw())
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want[0]):
+        assert torch.equal(a, b)
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [t.detach() for t in step(st.draw())]
+    for i in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (a, b) in enumerate(zip(out, want[i])):
+            assert torch.equal(a, b), (i, k)
+        (x0 @ P["w1"].t()).relu().sum().item()                                   # eager work between replays
