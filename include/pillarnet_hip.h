@@ -528,18 +528,42 @@ int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const floa
                               void* dgate, void* workspace, size_t workspace_bytes, pnStream stream);
 
 /* Products in 8-bit floating point (e4m3) with a power-of-two scale for each block of 128 along the contraction.
- * Quantise: block scale 2^e, e the smallest exponent >= -126 with (largest finite magnitude) <= 448 * 2^e; bytes are
- * x / 2^e rounded to nearest even; infinities and NaN become NaN.
- *   q  [rows][kp] bytes (kp = cols rounded up to 128, zero padded), q_scale: 32-bit words [ceil(kp / 512)][rows], byte
- *      b & 3 of word (b >> 2, row) = e + 127 of block b;  qt / qt_scale: the same of the transpose ([cols][mp]).
- *   block_rows 1: blocks of 1 x 128 (q) and 128 x 1 (qt); 128: one scale for each 128 x 128 tile, in both.
- *   colsum [ceil(rows / 128)][cols] fp32 or NULL: column sums of the input for pn_fp8_colsum.  q or qt may be NULL. */
-int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q, void* q_scale,
-                    void* qt, void* qt_scale, float* colsum, pnStream stream);
-int pn_fp8_colsum(const float* partial, long long rows, int cols, int out_dtype, void* out, pnStream stream);
-/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) on operands that pn_fp8_quantize laid out (k: the unpadded contraction). */
-int pn_fp8_gemm(const void* x, const void* x_scale, long long m, const void* w, const void* w_scale, int n, int k,
-                const void* bias, int bias_dtype, int act, int out_dtype, void* out, long long ldo, pnStream stream);
+ * Block scale 2^e, e the smallest exponent >= -126 with (largest finite magnitude) <= 448 * 2^e; bytes are x / 2^e rounded to
+ * nearest even; infinities and NaN become NaN and mark the results they enter.
+ *
+ * An operand [rows, cols] (the contraction along cols) is one allocation of pn_fp8_operand_bytes(rows, cols) bytes, 256-byte
+ * aligned:
+ *   bytes   [ceil(rows / 16)][ceil(cols / 128)] tiles of 2 KB = two planes h of 64 entries l of 16 bytes; entry l of plane h:
+ *           row l % 16 of the tile, k = l / 16 * 32 + h * 16 .. + 15 of the block; what lies past rows or cols is zero;
+ *   scales  behind them, words [ceil(blocks / 4)][rows]: byte b % 4 of word (b / 4, row) = e + 127 of block b of the row.
+ * pn_fp8_quantize writes q, the operand of x, and / or qt, that of its transpose.  block_rows 1: blocks of 1 x 128 along either
+ * operand's contraction (activations, gradients); 128: one scale for each 128 x 128 tile, the same in both (weights).
+ * colsum: NULL or [ceil(rows / 128)][cols] fp32, column sums of x over each 128 rows. */
+size_t pn_fp8_operand_bytes(long long rows, long long cols);
+int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q, void* qt,
+                    float* colsum, pnStream stream);
+/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) on operands x [m, k], w [n, k].  out: fp32 or bf16, row stride ldo; sums are
+ * fp32 (a bf16 result comes from the fp8 matrix instruction, which rounds the products of eight neighbouring k to 16 bits below
+ * the largest of them before it adds; an fp32 result from the same bytes widened to bf16, exactly). */
+int pn_fp8_gemm(const void* x, long long m, const void* w, int n, int k, const void* bias, int bias_dtype, int act, int out_dtype,
+                void* out, long long ldo, pnStream stream);
+/* The same for x as it is (fp32 / bf16 rows): its layout is part of the call.  Few rows need no workspace (the size is 0). */
+size_t pn_fp8_linear_workspace_bytes(long long m, int n, int k);
+int pn_fp8_linear(int dtype, const void* x, long long m, long long ldx, const void* w, int n, int k, const void* bias, int bias_dtype,
+                  int act, int out_dtype, void* out, long long ldo, void* workspace, size_t workspace_bytes, pnStream stream);
+/* Training, y [m, n] = x w^T + bias with x [m, k] and the weight [n, k] as they are; all sizes 1 .. 2^22:
+ *   forward   y (x's type, dense); keeps the transposed operands of x (save_x) and of the weight (save_w) in `saved`
+ *             (pn_fp8_train_saved_bytes, for the backward pass); workspace: pn_fp8_train_workspace_bytes(.., 0).
+ *   backward  dx = Q(g) Qw(w) [m, k] (g's type), dw = Q(g^T) Q(x^T)^T [n, k] (w_dtype), db = column sums of g [n] (db_dtype); any
+ *             may be NULL (save_w is needed for dx, save_x for dw); workspace: pn_fp8_train_workspace_bytes(.., 1).
+ * Both workspaces are the caller's and only used within the call's launches. */
+size_t pn_fp8_train_saved_bytes(long long m, int n, int k);
+size_t pn_fp8_train_workspace_bytes(long long m, int n, int k, int backward);
+int pn_fp8_train_forward(int dtype, const void* x, long long m, long long ldx, int w_dtype, const void* w, int n, int k, long long ldw,
+                         const void* bias, int bias_dtype, void* y, int save_x, int save_w, void* saved, void* workspace,
+                         pnStream stream);
+int pn_fp8_train_backward(int dtype, const void* g, long long m, long long ldg, int w_dtype, int n, int k, const void* saved, void* dx,
+                          void* dw, void* db, int db_dtype, void* workspace, pnStream stream);
 
 #ifdef __cplusplus
 }

@@ -148,11 +148,19 @@ SIGNATURES = {
     "pn_residual_norm_forward": (c_int, [POINTER(pnResidualNorm), c_void_p, c_void_p, c_void_p, c_void_p]),
     "pn_residual_norm_workspace_bytes": (c_size_t, [POINTER(pnResidualNorm)]),
     "pn_residual_norm_backward": (c_int, [POINTER(pnResidualNorm)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
-    "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                c_void_p, c_void_p]),
-    "pn_fp8_colsum": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p]),
-    "pn_fp8_gemm": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
-                            c_void_p, c_longlong, c_void_p]),
+    "pn_fp8_operand_bytes": (c_size_t, [c_longlong, c_longlong]),
+    "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pn_fp8_gemm": (c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong,
+                            c_void_p]),
+    "pn_fp8_linear_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
+    "pn_fp8_linear": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
+                              c_void_p, c_longlong, c_void_p, c_size_t, c_void_p]),
+    "pn_fp8_train_saved_bytes": (c_size_t, [c_longlong, c_int, c_int]),
+    "pn_fp8_train_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int, c_int]),
+    "pn_fp8_train_forward": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_int, c_int, c_longlong, c_void_p,
+                                     c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "pn_fp8_train_backward": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_int, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -13,123 +13,135 @@
 struct QuantArgs {
   const void* x;
   long long rows, ldx;
-  int cols;
-  unsigned char* q;          // [rows][kp], kp = cols rounded up to 128
-  unsigned char* q_scale;    // dwords [ceil(kp / 512)][rows], byte (k block & 3)
-  unsigned char* qt;         // [cols][mp], mp = rows rounded up to 128
-  unsigned char* qt_scale;   // dwords [ceil(mp / 512)][cols]
+  int cols, col_blocks;
+  unsigned char *q, *q_scale, *qt, *qt_scale;
   float* colsum;             // [ceil(rows / 128)][cols]
 };
 
-// e + 127 of a block with largest finite magnitude `bits` (as an integer: magnitudes order like their bit patterns)
-__device__ __forceinline__ int block_scale(uint32_t bits) {
-  const int b = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return b < 1 ? 1 : b;
+// The tile's 128 x 128 bytes, rows of PITCH in LDS, to eight tiles of an operand: whole 2 KB runs.
+template <int PITCH>
+__device__ __forceinline__ void write_tiles(const unsigned char* lds, unsigned char* q, long long group0, int groups, long long blocks, long long block) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int u = (int)threadIdx.x + i * 256, g = u >> 7, h = (u >> 6) & 1, l = u & 63;
+    const unsigned char* src = lds + (g * 16 + (l & 15)) * PITCH + (l >> 4) * 32 + h * 16;
+    const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 8);
+    if (g < groups) *reinterpret_cast<uint4*>(q + ((group0 + g) * blocks + block) * 2048 + (u & 127) * 16) = make_uint4(a.x, a.y, b.x, b.y);
+  }
 }
-__device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }   // 2^(127 - byte)
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
-}
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
 template <typename T, bool BLOCK>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
-  constexpr int PITCH = 136;                          // LDS row of a column's 128 bytes, 8-byte aligned
+  typedef Raw8<T> R;
+  constexpr int PITCH = 136, MAGS = R::MAGS;          // LDS row of a column's 128 bytes, 8-byte aligned
   __shared__ __attribute__((aligned(16))) unsigned char tile[128 * PITCH];
-  __shared__ uint32_t wave_max[4][128];
+  __shared__ uint32_t wave_max[4][16 * MAGS];
   __shared__ float wave_sum[4][128];
   const int tid = threadIdx.x, wave = tid >> 6, c8 = tid & 15, r8 = tid >> 4;
-  const int kb = blockIdx.x, col0 = kb * 128 + c8 * 8;
-  const long long mb = blockIdx.y, row0 = mb * 128 + r8 * 8;
+  const int kb = (int)(blockIdx.x % (unsigned)a.col_blocks), col0 = kb * 128 + c8 * 8;
+  const long long mb = blockIdx.x / (unsigned)a.col_blocks, row0 = mb * 128 + r8 * 8;
   const T* X = reinterpret_cast<const T*>(a.x);
-  float v[8][8];
+  // All eight loads before anything that waits for one: no branch between them but the tile's own (a load behind a branch of
+  // its own waits for the one before: eight trips to memory instead of one).
+  R v[8];
+  if (kb * 128 + 128 <= a.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8(X + (row0 + i) * a.ldx + col0, row0 + i < a.rows ? a.cols - col0 : 0, v[i]);
+    for (int i = 0; i < 8; ++i) v[i].load(X + (row0 + i < a.rows ? row0 + i : a.rows - 1) * a.ldx + col0);
+  } else {
+    const int n = a.cols - col0, first = n > 0 ? col0 : a.cols - 1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i].load_part(X + (row0 + i < a.rows ? row0 + i : a.rows - 1) * a.ldx + first, n > 0 ? (n < 8 ? n : 8) : 1);
+    if (n <= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i].clear();
+    }
+  }
+  if (mb * 128 + 128 > a.rows) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (row0 + i >= a.rows) v[i].clear();
+  }
 
-  uint32_t rmax[8], cmax[8];
+  uint32_t rmax[8], cmax[MAGS], any = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cmax[j] = 0;
+  for (int j = 0; j < MAGS; ++j) cmax[j] = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    rmax[i] = 0;
+    rmax[i] = v[i].template row_mag<false>();
+    any = R::mag_max(any, rmax[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t m = finite_bits(v[i][j]);
-      rmax[i] = umax(rmax[i], m);
-      cmax[j] = umax(cmax[j], m);
+    for (int j = 0; j < MAGS; ++j) cmax[j] = R::mag_max(cmax[j], v[i].template mag<false>(j));
+  }
+  if (R::mag_inf(any)) {                              // rare: leave out what is not finite
+#pragma unroll
+    for (int j = 0; j < MAGS; ++j) cmax[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      rmax[i] = v[i].template row_mag<true>();
+#pragma unroll
+      for (int j = 0; j < MAGS; ++j) cmax[j] = R::mag_max(cmax[j], v[i].template mag<true>(j));
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) rmax[i] = umax(rmax[i], (uint32_t)__shfl_xor((int)rmax[i], o));
   }
   if (BLOCK) {                                        // one scale for the tile
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = umax(m, rmax[i]);
+    for (int i = 0; i < 8; ++i) m = R::mag_max(m, rmax[i]);
+    m = R::mag_bits(mag_max16<R>(m));
     m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
     m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
     if ((tid & 63) == 0) wave_max[wave][0] = m;
     __syncthreads();
     m = umax(umax(wave_max[0][0], wave_max[1][0]), umax(wave_max[2][0], wave_max[3][0]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = m;
-  } else if (a.qt) {
+    for (int i = 0; i < 8; ++i) rmax[i] = m;
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      cmax[j] = umax(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 16));
-      cmax[j] = umax(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 32));
-      if ((tid & 48) == 0) wave_max[wave][c8 * 8 + j] = cmax[j];
-    }
-    __syncthreads();
+    for (int i = 0; i < 8; ++i) rmax[i] = R::mag_bits(mag_max16<R>(rmax[i]));
+    if (a.qt) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = c8 * 8 + j;
-      cmax[j] = umax(umax(wave_max[0][c], wave_max[1][c]), umax(wave_max[2][c], wave_max[3][c]));
+      for (int j = 0; j < MAGS; ++j) {
+        cmax[j] = R::mag_max(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 16));
+        cmax[j] = R::mag_max(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 32));
+        if ((tid & 48) == 0) wave_max[wave][c8 * MAGS + j] = cmax[j];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < MAGS; ++j) {
+        const int c = c8 * MAGS + j;
+        cmax[j] = R::mag_max(R::mag_max(wave_max[0][c], wave_max[1][c]), R::mag_max(wave_max[2][c], wave_max[3][c]));
+      }
     }
   }
+  const long long row_blocks = (a.rows + 127) / 128;
   if (a.q) {
-    const long long kp = (long long)gridDim.x * 128;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (row0 + i >= a.rows) continue;
       const int sc = block_scale(rmax[i]);
-      const float f = inv_scale(sc);
-      const uint2 o = make_uint2(pack4(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f),
-                                 pack4(v[i][4] * f, v[i][5] * f, v[i][6] * f, v[i][7] * f));
-      *reinterpret_cast<uint2*>(a.q + (row0 + i) * kp + col0) = o;
-      if (c8 == 0) a.q_scale[(((long long)(kb >> 2) * a.rows) + row0 + i) * 4 + (kb & 3)] = (unsigned char)sc;
+      *reinterpret_cast<uint2*>(tile + (r8 * 8 + i) * PITCH + c8 * 8) = v[i].quant(scale_value(sc));
+      if (c8 == 0 && row0 + i < a.rows) a.q_scale[(((long long)(kb >> 2) * a.rows) + row0 + i) * 4 + (kb & 3)] = (unsigned char)sc;
     }
+    __syncthreads();
+    const long long left = a.rows - mb * 128;
+    write_tiles<PITCH>(tile, a.q, mb * 8, left < 128 ? (int)(left + 15) / 16 : 8, a.col_blocks, kb);
+    if (a.qt) __syncthreads();
   }
   if (a.qt) {
-    const long long mp = (long long)gridDim.y * 128;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int sc = block_scale(cmax[j]);
-      const float f = inv_scale(sc);
-      const uint2 o = make_uint2(pack4(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f),
-                                 pack4(v[4][j] * f, v[5][j] * f, v[6][j] * f, v[7][j] * f));
-      *reinterpret_cast<uint2*>(tile + (c8 * 8 + j) * PITCH + r8 * 8) = o;
+      const int sc = block_scale(BLOCK ? rmax[0] : R::col_bits(cmax, j));
+      *reinterpret_cast<uint2*>(tile + (c8 * 8 + j) * PITCH + r8 * 8) = R::quant_col(v, j, scale_value(sc));
       if (r8 == 0 && col0 + j < a.cols) a.qt_scale[((mb >> 2) * a.cols + col0 + j) * 4 + (mb & 3)] = (unsigned char)sc;
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = i * 16 + r8;
-      if (kb * 128 + c < a.cols)
-        *reinterpret_cast<uint2*>(a.qt + (long long)(kb * 128 + c) * mp + mb * 128 + c8 * 8) =
-            *reinterpret_cast<const uint2*>(tile + c * PITCH + c8 * 8);
-    }
+    const int left = a.cols - kb * 128;
+    write_tiles<PITCH>(tile, a.qt, (long long)kb * 8, left < 128 ? (left + 15) / 16 : 8, row_blocks, mb);
   }
   if (a.colsum) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[i][j];
+      for (int i = 0; i < 8; ++i) s += v[i].get(j);
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if ((tid & 48) == 0) wave_sum[wave][c8 * 8 + j] = s;
@@ -140,29 +152,36 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
   }
 }
 
-extern "C" int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q,
-                               void* q_scale, void* qt, void* qt_scale, float* colsum, void* stream) {
-  PN_CHECK_ARG(dtype == PN_DTYPE_F32 || dtype == PN_DTYPE_BF16, "pn_fp8_quantize: element type %d (fp32 or bf16)", dtype);
-  PN_CHECK_ARG(block_rows == 1 || block_rows == 128, "pn_fp8_quantize: blocks of %d rows (1 or 128)", block_rows);
-  PN_CHECK_ARG(rows >= 0 && cols >= 1 && rows <= 65535ll * 128, "pn_fp8_quantize: %lld x %d elements", rows, cols);
-  if (rows == 0) return PN_OK;
-  PN_CHECK_ARG(x && (rows == 1 || ldx >= cols), "pn_fp8_quantize: x missing or its row stride below the row length");
-  PN_CHECK_ARG((q && q_scale) || (qt && qt_scale), "pn_fp8_quantize: output missing");
-  PN_CHECK_ARG((!q || q_scale) && (!qt || qt_scale), "pn_fp8_quantize: bytes without scales");
-  PN_CHECK_ARG((((uintptr_t)q | (uintptr_t)qt | (uintptr_t)q_scale | (uintptr_t)qt_scale) & 15) == 0,
-               "pn_fp8_quantize: outputs must be 16-byte aligned");
-  QuantArgs a = {x, rows, ldx, cols, (unsigned char*)q, (unsigned char*)q_scale, (unsigned char*)qt, (unsigned char*)qt_scale, colsum};
-  const dim3 grid((cols + 127) / 128, (unsigned)((rows + 127) / 128)), wg(256);
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == PN_DTYPE_F32) {
-    if (block_rows == 1) hipLaunchKernelGGL((fp8_quantize_kernel<float, false>), grid, wg, 0, s, a);
+int fp8_quantize_launch(const Fp8QuantJob& j, hipStream_t s) {
+  const Fp8Operand q = fp8_operand(j.q, j.rows, j.cols), qt = fp8_operand(j.qt, j.cols, j.rows);
+  const int col_blocks = (j.cols + 127) / 128;
+  QuantArgs a = {j.x, j.rows, j.rows == 1 ? 0 : j.ldx, j.cols, col_blocks, (unsigned char*)q.q, (unsigned char*)q.scale,
+                 (unsigned char*)qt.q, (unsigned char*)qt.scale, j.colsum};
+  const dim3 grid((unsigned)((j.rows + 127) / 128 * col_blocks)), wg(256);
+  if (j.dtype == PN_DTYPE_F32) {
+    if (j.block_rows == 1) hipLaunchKernelGGL((fp8_quantize_kernel<float, false>), grid, wg, 0, s, a);
     else hipLaunchKernelGGL((fp8_quantize_kernel<float, true>), grid, wg, 0, s, a);
   } else {
-    if (block_rows == 1) hipLaunchKernelGGL((fp8_quantize_kernel<__bf16, false>), grid, wg, 0, s, a);
+    if (j.block_rows == 1) hipLaunchKernelGGL((fp8_quantize_kernel<__bf16, false>), grid, wg, 0, s, a);
     else hipLaunchKernelGGL((fp8_quantize_kernel<__bf16, true>), grid, wg, 0, s, a);
   }
   PN_CHECK_LAUNCH("fp8_quantize_kernel");
   return PN_OK;
+}
+
+extern "C" size_t pn_fp8_operand_bytes(long long rows, long long cols) { return rows < 0 || cols < 1 ? 0 : fp8_bytes(rows, cols); }
+
+extern "C" int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q, void* qt,
+                               float* colsum, void* stream) {
+  PN_CHECK_ARG(dtype == PN_DTYPE_F32 || dtype == PN_DTYPE_BF16, "pn_fp8_quantize: element type %d (fp32 or bf16)", dtype);
+  PN_CHECK_ARG(block_rows == 1 || block_rows == 128, "pn_fp8_quantize: blocks of %d rows (1 or 128)", block_rows);
+  PN_CHECK_ARG(rows >= 0 && cols >= 1 && (rows + 127) / 128 < (1ll << 31) / ((cols + 127) / 128), "pn_fp8_quantize: %lld x %d elements",
+               rows, cols);
+  if (rows == 0) return PN_OK;
+  PN_CHECK_ARG(x && (rows == 1 || ldx >= cols), "pn_fp8_quantize: x missing or its row stride below the row length");
+  PN_CHECK_ARG(q || qt || colsum, "pn_fp8_quantize: output missing");
+  PN_CHECK_ARG((((uintptr_t)q | (uintptr_t)qt) & 255) == 0, "pn_fp8_quantize: operands must be 256-byte aligned");
+  return fp8_quantize_launch(Fp8QuantJob{x, dtype, block_rows, rows, ldx, cols, q, qt, colsum}, (hipStream_t)stream);
 }
 
 // out[c] = sum of colsum over the row blocks, in a fixed order
@@ -180,11 +199,8 @@ __global__ __launch_bounds__(256) void fp8_colsum_kernel(const float* partial, l
     else reinterpret_cast<__bf16*>(out)[c] = (__bf16)s;
   }
 }
-extern "C" int pn_fp8_colsum(const float* partial, long long rows, int cols, int out_dtype, void* out, void* stream) {
-  PN_CHECK_ARG(out_dtype == PN_DTYPE_F32 || out_dtype == PN_DTYPE_BF16, "pn_fp8_colsum: output type %d (fp32 or bf16)", out_dtype);
-  PN_CHECK_ARG(rows >= 0 && cols >= 1 && out && (partial || rows == 0), "pn_fp8_colsum: null pointer or empty row");
-  hipLaunchKernelGGL(fp8_colsum_kernel, dim3((cols + 63) / 64), dim3(256), 0, (hipStream_t)stream, partial, (rows + 127) / 128, cols, out,
-                     out_dtype);
+int fp8_colsum_launch(const float* partial, long long rows, int cols, int out_dtype, void* out, hipStream_t s) {
+  hipLaunchKernelGGL(fp8_colsum_kernel, dim3((cols + 63) / 64), dim3(256), 0, s, partial, (rows + 127) / 128, cols, out, out_dtype);
   PN_CHECK_LAUNCH("fp8_colsum_kernel");
   return PN_OK;
 }

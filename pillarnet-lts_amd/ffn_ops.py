@@ -303,55 +303,68 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
 
 # ---- products in fp8 ---------------------------------------------------------------------------------------------------
 class Fp8Rows:
-    """[rows, cols] in e4m3 with block scales, as pn_fp8_quantize lays them out: q uint8 [rows, kp], scale uint8
-    [ceil(kp / 512), rows, 4]."""
-    __slots__ = ("q", "scale", "rows", "cols")
+    """[rows, cols] in e4m3 with block scales, laid out for products along cols (the layout: pn_fp8_quantize)."""
+    __slots__ = ("data", "rows", "cols")
 
     def __init__(self, rows, cols, device):
-        kp = -(-cols // 128) * 128
         self.rows, self.cols = rows, cols
-        self.q = torch.empty((rows, kp), dtype=torch.uint8, device=device)
-        self.scale = torch.empty((-(-kp // 512), rows, 4), dtype=torch.uint8, device=device)
+        self.data = torch.empty(_lib.lib().pn_fp8_operand_bytes(rows, cols), dtype=torch.uint8, device=device)
+
+    def _parts(self):
+        """(bytes [groups, blocks, plane, quarter, row, 16], scale bytes [words, rows, 4]) as views."""
+        g, b = -(-self.rows // 16), -(-self.cols // 128)
+        n = g * b * 2048
+        return (self.data[:n].view(g, b, 2, 4, 16, 16), self.data[n: n + -(-b // 4) * self.rows * 4].view(-1, self.rows, 4))
+
+    def bytes_and_exponents(self):
+        """(uint8 [rows, cols rounded up to 128], int32 [rows, blocks]): e4m3 bytes, and the exponent of each block."""
+        q, s = self._parts()
+        g, b = q.shape[:2]
+        rows = q.permute(0, 4, 1, 3, 2, 5).reshape(g * 16, b * 128)[: self.rows]
+        return rows, s.permute(1, 0, 2).reshape(self.rows, -1)[:, :b].to(torch.int32) - 127
 
     def values(self):
         """What the bytes stand for, fp32 [rows, cols] (for tests and inspection)."""
-        kp = self.q.shape[1]
-        e = self.scale.permute(1, 0, 2).reshape(self.rows, -1)[:, : kp // 128].to(torch.int32)
-        s = (e << 23).view(torch.float32).repeat_interleave(128, 1)
-        return (self.q.view(torch.float8_e4m3fn).float() * s)[:, : self.cols]
+        q, e = self.bytes_and_exponents()
+        s = ((e + 127) << 23).view(torch.float32).repeat_interleave(128, 1)
+        return (q.view(torch.float8_e4m3fn).float() * s)[:, : self.cols]
 
 
-def fp8_quantize(x, block_rows=1, rows=True, transposed=False, colsum=False):
-    """x [..., C] -> (Fp8Rows of x or None, Fp8Rows of its transpose or None, column-sum partials or None), in one pass.
-    block_rows 1: a scale for each 128 elements along the contraction (the row, or the column for the transpose);
-    128: one for each 128 x 128 tile (weights)."""
+def fp8_quantize(x, block_rows=1, rows=True, transposed=False):
+    """x [..., C] -> (Fp8Rows of x or None, Fp8Rows of its transpose or None), in one pass.  block_rows 1: a scale for each 128
+    elements along the contraction (the row, or the column for the transpose); 128: one for each 128 x 128 tile (weights)."""
     _check("fp8_quantize", x)
     _require(x.dim() >= 1 and x.shape[-1] >= 1, "fp8_quantize: empty rows")
     _require(block_rows in (1, 128), f"fp8_quantize: blocks of {block_rows} rows (1 or 128)")
     _require(rows or transposed, "fp8_quantize: nothing asked for")
     v = _rows(x.detach())
     M, C = v.shape
+    _require(M > 0 or not transposed, "fp8_quantize: no rows to transpose")
     q = Fp8Rows(M, C, x.device) if rows else None
     qt = Fp8Rows(C, M, x.device) if transposed else None
-    cs = torch.empty((-(-M // 128), C), dtype=torch.float32, device=x.device) if colsum else None
-    _call("pn_fp8_quantize", x.device, _DTYPES[x.dtype], v.data_ptr(), M, C, v.stride(0), block_rows, _ptr(q and q.q),
-          _ptr(q and q.scale), _ptr(qt and qt.q), _ptr(qt and qt.scale), _ptr(cs))
-    return q, qt, cs
+    _call("pn_fp8_quantize", x.device, _DTYPES[x.dtype], v.data_ptr(), M, C, v.stride(0), block_rows, q and q.data.data_ptr(),
+          qt and qt.data.data_ptr(), None)
+    return q, qt
+
+
+def _bias_of(what, bias, n, device):
+    if bias is None:
+        return None, 0
+    _check(what, bias)
+    _require(bias.shape == (n,) and bias.device == device, f"{what}: the bias has shape [{n}] and lives with the weight")
+    return bias.detach().contiguous(), _DTYPES[bias.dtype]
 
 
 def fp8_matmul(x, w, bias=None, act="none", out_dtype=torch.bfloat16):
     """x, w: Fp8Rows with the same contraction -> act(x @ w.T + bias) [x.rows, w.rows]."""
-    _require(x.cols == w.cols, f"fp8_matmul: contractions of {x.cols} and {w.cols}")
+    _require(isinstance(x, Fp8Rows) and isinstance(w, Fp8Rows) and x.cols == w.cols, "fp8_matmul: two Fp8Rows with one contraction")
     _require(out_dtype in _DTYPES and act in _lib.PN_ACT, f"fp8_matmul: output {out_dtype}, activation {act!r}")
-    _require(x.q.device == w.q.device, f"fp8_matmul: operands on {x.q.device} and {w.q.device}")
-    if bias is not None:
-        _check("fp8_matmul", bias)
-        _require(bias.shape == (w.rows,) and bias.device == x.q.device, f"fp8_matmul: the bias has shape [{w.rows}]")
-        bias = bias.contiguous()
-    out = torch.empty((x.rows, w.rows), dtype=out_dtype, device=x.q.device)
-    _call("pn_fp8_gemm", out.device, x.q.data_ptr(), x.scale.data_ptr(), x.rows, w.q.data_ptr(), w.scale.data_ptr(), w.rows,
-          x.cols, _ptr(bias), _DTYPES[bias.dtype] if bias is not None else 0, _lib.PN_ACT[act], _DTYPES[out_dtype], out.data_ptr(),
-          w.rows)
+    dev = x.data.device
+    _require(dev == w.data.device, f"fp8_matmul: operands on {dev} and {w.data.device}")
+    bias, bd = _bias_of("fp8_matmul", bias, w.rows, dev)
+    out = torch.empty((x.rows, w.rows), dtype=out_dtype, device=dev)
+    _call("pn_fp8_gemm", dev, x.data.data_ptr(), x.rows, w.data.data_ptr(), w.rows, x.cols, _ptr(bias), bd, _lib.PN_ACT[act],
+          _DTYPES[out_dtype], out.data_ptr(), w.rows)
     return out
 
 
@@ -360,18 +373,12 @@ class Fp8Weight:
 
     def __init__(self, weight, bias=None):
         _check("Fp8Weight", weight)
-        _require(weight.dim() == 2 and weight.shape[0] >= 1, "Fp8Weight: a weight [out_features, in_features]")
-        self.data = fp8_quantize(weight.detach(), 128)[0]
-        self._set_bias(bias)
+        _require(weight.dim() == 2 and min(weight.shape) >= 1, "Fp8Weight: a weight [out_features, in_features]")
+        self._set(fp8_quantize(weight, 128)[0], bias)
 
-    def _set_bias(self, bias):
-        self.out_features, self.in_features = self.data.rows, self.data.cols
-        if bias is not None:
-            _check("Fp8Weight", bias)
-            _require(bias.shape == (self.out_features,) and bias.device == self.data.q.device,
-                     f"Fp8Weight: the bias has shape [{self.out_features}]")
-            bias = bias.detach().contiguous()
-        self.bias = bias
+    def _set(self, data, bias):
+        self.data, self.out_features, self.in_features = data, data.rows, data.cols
+        self.bias, self.bias_dtype = _bias_of("Fp8Weight", bias, data.rows, data.data.device)
 
     @classmethod
     def from_blocks(cls, values, exponents, bias=None):
@@ -384,12 +391,13 @@ class Fp8Weight:
         N, K = values.shape
         nb, kb = -(-N // 128), -(-K // 128)
         _require(exponents.shape == (nb, kb) and not exponents.is_floating_point(), f"Fp8Weight: exponents are integers [{nb}, {kb}]")
-        self = cls.__new__(cls)
-        d = self.data = Fp8Rows(N, K, values.device)
-        d.q.zero_()[:, :K] = values.view(torch.uint8)
-        bytes_ = torch.nn.functional.pad((exponents + 127).clamp(1, 254).to(torch.uint8), (0, d.scale.shape[0] * 4 - kb))
-        d.scale.copy_(bytes_.repeat_interleave(128, 0)[:N].view(N, -1, 4).permute(1, 0, 2))
-        self._set_bias(bias)
+        self, data = cls.__new__(cls), Fp8Rows(N, K, values.device)
+        q, s = data._parts()
+        pad = torch.nn.functional.pad(values.view(torch.uint8), (0, kb * 128 - K, 0, q.shape[0] * 16 - N))
+        q.copy_(pad.view(q.shape[0], 16, kb, 4, 2, 16).permute(0, 2, 4, 3, 1, 5))
+        e = torch.nn.functional.pad((exponents + 127).clamp(1, 254).to(torch.uint8), (0, s.shape[0] * 4 - kb))
+        s.copy_(e.repeat_interleave(128, 0)[:N].view(N, -1, 4).permute(1, 0, 2))
+        self._set(data, bias)
         return self
 
 
@@ -398,22 +406,40 @@ def fp8_linear(x, weight, act="none", out_dtype=None):
     out_dtype: fp32 or bf16 (default: x's).  Forward only; fp8_linear_train is the form with gradients."""
     _check("fp8_linear", x)
     _require(isinstance(weight, Fp8Weight), "fp8_linear: the weight is an Fp8Weight")
-    _require(x.shape[-1] == weight.in_features, f"fp8_linear: rows of {x.shape[-1]} for a weight of {weight.in_features}")
-    _require(x.device == weight.data.q.device, f"fp8_linear: x on {x.device}, the weight on {weight.data.q.device}")
+    N, K, dev = weight.out_features, weight.in_features, x.device
+    _require(x.dim() >= 1 and x.shape[-1] == K, f"fp8_linear: rows of {tuple(x.shape)} for a weight of {K}")
+    _require(dev == weight.data.data.device, f"fp8_linear: x on {dev}, the weight on {weight.data.data.device}")
     _require(not _wants_grad(x), "fp8_linear: forward only (fp8_linear_train has gradients)")
-    q = fp8_quantize(x)[0]
-    out = fp8_matmul(q, weight.data, weight.bias, act, x.dtype if out_dtype is None else out_dtype)
-    return out.view(*x.shape[:-1], weight.out_features)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _require(out_dtype in _DTYPES and act in _lib.PN_ACT, f"fp8_linear: output {out_dtype}, activation {act!r}")
+    v = _rows(x.detach())
+    M = v.shape[0]
+    out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
+    size = _lib.lib().pn_fp8_linear_workspace_bytes(M, N, K)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call("pn_fp8_linear", dev, _DTYPES[x.dtype], v.data_ptr(), M, v.stride(0), weight.data.data.data_ptr(), N, K, _ptr(weight.bias),
+          weight.bias_dtype, _lib.PN_ACT[act], _DTYPES[out_dtype], out.data_ptr(), N, _ptr(ws), size)
+    return out
 
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w, need_b = ctx.needs_input_grad
-        xq, xt, _ = fp8_quantize(x, 1, True, need_w)
-        wq, wt, _ = fp8_quantize(weight, 128, True, need_x)
-        y = fp8_matmul(xq, wq, bias, "none", x.dtype).view(*x.shape[:-1], weight.shape[0])
-        ctx.x_t, ctx.w_t = xt, wt              # one byte an element; x and the weight themselves are not kept
+        need_x, need_w, _ = ctx.needs_input_grad
+        L, dev = _lib.lib(), x.device
+        v, wv = _rows(x), _rows(weight)
+        (M, K), N = v.shape, wv.shape[0]
+        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        saved = None
+        if M:
+            # the transposed operands that the backward pass reads: a byte an element; x and the weight are not kept
+            saved = torch.empty(L.pn_fp8_train_saved_bytes(M, N, K), dtype=torch.uint8, device=dev)
+            ws = torch.empty(L.pn_fp8_train_workspace_bytes(M, N, K, 0), dtype=torch.uint8, device=dev)
+            b = None if bias is None else bias.contiguous()
+            _call("pn_fp8_train_forward", dev, _DTYPES[x.dtype], v.data_ptr(), M, v.stride(0), _DTYPES[weight.dtype], wv.data_ptr(), N, K,
+                  wv.stride(0), _ptr(b), 0 if b is None else _DTYPES[b.dtype], y.data_ptr(), int(need_w), int(need_x), saved.data_ptr(),
+                  ws.data_ptr())
+        ctx.save_for_backward(saved)
         ctx.meta = (x.shape, weight.dtype, None if bias is None else bias.dtype)
         return y
 
@@ -421,24 +447,18 @@ class _Fp8Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         need_x, need_w, need_b = ctx.needs_input_grad
+        (saved,) = ctx.saved_tensors
         shape, w_dtype, b_dtype = ctx.meta
-        dx = dw = db = None
-        gv = _rows(g)
-        M, N = gv.shape
-        if need_x or need_w:
-            gq, gt, cs = fp8_quantize(gv, 1, need_x, need_w, need_b)
-        elif need_b:
-            cs = fp8_quantize(gv, 1, True, False, True)[2]
-        if need_x:
-            dx = fp8_matmul(gq, ctx.w_t, None, "none", g.dtype).view(shape)
-        if need_w:
-            if M == 0:
-                dw = torch.zeros((N, shape[-1]), dtype=w_dtype, device=g.device)
-            else:
-                dw = fp8_matmul(gt, ctx.x_t, None, "none", w_dtype)
-        if need_b:
-            db = torch.empty(N, dtype=b_dtype, device=g.device)
-            _call("pn_fp8_colsum", g.device, cs.data_ptr(), M, N, _DTYPES[b_dtype], db.data_ptr())
+        dev, gv = g.device, _rows(g)
+        (M, N), K = gv.shape, shape[-1]
+        dx = torch.empty(shape, dtype=g.dtype, device=dev) if need_x else None
+        dw = torch.empty((N, K), dtype=w_dtype, device=dev) if need_w else None
+        db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
+        if M == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+        ws = torch.empty(_lib.lib().pn_fp8_train_workspace_bytes(M, N, K, 1), dtype=torch.uint8, device=dev)
+        _call("pn_fp8_train_backward", dev, _DTYPES[g.dtype], gv.data_ptr(), M, gv.stride(0), _DTYPES[w_dtype], N, K, saved.data_ptr(),
+              _ptr(dx), _ptr(dw), _ptr(db), _DTYPES[b_dtype] if need_b else 0, ws.data_ptr())
         return dx, dw, db
 
 
@@ -451,4 +471,5 @@ def fp8_linear_train(x, weight, bias=None):
     _require(x.dim() >= 1 and weight.dim() == 2 and min(weight.shape) >= 1 and x.shape[-1] == weight.shape[1],
              f"fp8_linear_train: x {tuple(x.shape)} for a weight {tuple(weight.shape)}")
     _require(bias is None or bias.shape == (weight.shape[0],), f"fp8_linear_train: the bias has shape [{weight.shape[0]}]")
+    _require(max(x.numel() // x.shape[-1], *weight.shape) <= 1 << 22, "fp8_linear_train: more than 2^22 rows or features")
     return _Fp8Linear.apply(x, weight, bias)

@@ -109,17 +109,33 @@ def test_dropout_and_fp8_arguments_are_checked_before_the_gpu():
     assert L.pn_act_dropout_backward(0, 16, None, 2, 8, 8, 8, 2, 5, 16, 0, 16, None) == -1      # gelu needs x
     assert L.pn_act_dropout_backward(0, None, 16, 2, 8, 8, 8, 1, 5, 16, 0, 16, None) == -1
     assert L.pn_dropout_draw(None, 16, None) == -1
-    q = lambda dt=0, x=16, r=4, c=8, ld=8, b=1, q=16, s=16, qt=None, st=None: L.pn_fp8_quantize(dt, x, r, c, ld, b, q, s, qt, st, None, None)
-    for bad in (dict(dt=2), dict(x=None), dict(r=-1), dict(c=0), dict(ld=7), dict(b=64), dict(q=None), dict(s=None), dict(qt=16),
-                dict(q=24)):
+    q = lambda dt=0, x=16, r=4, c=8, ld=8, b=1, q=256, t=None: L.pn_fp8_quantize(dt, x, r, c, ld, b, q, t, None, None)
+    for bad in (dict(dt=2), dict(x=None), dict(r=-1), dict(c=0), dict(ld=7), dict(b=64), dict(q=None), dict(q=24), dict(t=16)):
         assert q(**bad) == -1
     assert q(r=0) == 0
-    g = lambda x=16, m=4, w=16, n=8, k=8, act=0, od=0, out=16, ldo=8: L.pn_fp8_gemm(x, 16, m, w, 16, n, k, None, 0, act, od, out, ldo, None)
+    g = lambda x=256, m=4, w=256, n=8, k=8, act=0, od=0, out=16, ldo=8: L.pn_fp8_gemm(x, m, w, n, k, None, 0, act, od, out, ldo, None)
     for bad in (dict(x=None), dict(m=-1), dict(w=None), dict(n=0), dict(k=0), dict(act=3), dict(od=2), dict(out=None), dict(ldo=7),
-                dict(x=24)):
+                dict(x=24), dict(w=16), dict(k=(1 << 22) + 1)):
         assert g(**bad) == -1
     assert g(m=0) == 0
-    assert L.pn_fp8_colsum(None, 4, 8, 0, 16, None) == -1 and L.pn_fp8_colsum(16, 4, 8, 5, 16, None) == -1
+    f = lambda dt=0, x=16, m=5000, ld=256, w=256, n=256, k=256, ws=256, nb=1 << 30: L.pn_fp8_linear(dt, x, m, ld, w, n, k, None, 0, 0, 0, 16, n,
+                                                                                                  ws, nb, None)
+    assert L.pn_fp8_linear_workspace_bytes(5000, 256, 256) == L.pn_fp8_operand_bytes(5000, 256) > 5000 * 256
+    assert L.pn_fp8_linear_workspace_bytes(16, 256, 256) == 0 == L.pn_fp8_operand_bytes(-1, 8)
+    for bad in (dict(dt=4), dict(x=None), dict(ld=255), dict(w=None), dict(ws=8)):
+        assert f(**bad) == -1
+    assert f(ws=None) == -2 and f(nb=100) == -2
+    tf = lambda dt=0, x=16, m=4, ld=8, wd=0, w=16, n=8, k=8, lw=8, y=16, sv=256, ws=256: L.pn_fp8_train_forward(
+        dt, x, m, ld, wd, w, n, k, lw, None, 0, y, 1, 1, sv, ws, None)
+    for bad in (dict(dt=2), dict(wd=3), dict(x=None), dict(m=0), dict(ld=7), dict(lw=7), dict(w=None), dict(y=None), dict(sv=None), dict(ws=8),
+                dict(k=1 << 23)):
+        assert tf(**bad) == -1
+    tb = lambda dt=0, g=16, m=4, ld=8, wd=0, sv=256, dx=None, db=None, bd=0, ws=256: L.pn_fp8_train_backward(
+        dt, g, m, ld, wd, 8, 8, sv, dx, None, db, bd, ws, None)
+    for bad in (dict(dt=2), dict(g=None), dict(m=0), dict(ld=7), dict(sv=16), dict(ws=None), dict(db=16, bd=7)):
+        assert tb(**bad) == -1
+    assert tb() == 0                                                            # nothing asked for, nothing launched
+    assert L.pn_fp8_train_saved_bytes(0, 8, 8) == 0 and L.pn_fp8_train_workspace_bytes(4, 8, 8, 1) >= 4 * 8
 
 
 def test_struct_layout_matches_header():

@@ -417,23 +417,21 @@ def _values(rs, R, C, dtype):
 @pytest.mark.parametrize("R,C", [(1, 1), (1, 128), (3, 129), (127, 64), (128, 128), (129, 300), (700, 515), (260, 1024)])
 def test_fp8_quantize_is_exact(cuda, dtype, block_rows, R, C):
     x = _values(np.random.RandomState(R + C), R, C, dtype)
-    q, qt, cs = ffn_ops.fp8_quantize(x.to(cuda), block_rows, True, True, True)
+    q, qt = ffn_ops.fp8_quantize(x.to(cuda), block_rows, True, True)
     want = fo.quantise(d(x), block_rows)
     wt = fo.quantise(d(x).T, 1) if block_rows == 1 else want.T
     np.testing.assert_array_equal(d(q.values()), want)
     np.testing.assert_array_equal(d(qt.values()), wt)
-    assert (q.q[:, C:] == 0).all() and (qt.q[:, R:] == 0).all()               # padding that products run over
-    e = fo.block_exponents(d(x), block_rows).repeat(block_rows, 0)[:R] + 127
-    got = q.scale.permute(1, 0, 2).reshape(R, -1)[:, : e.shape[1]].cpu().numpy()
-    np.testing.assert_array_equal(got, e)
-    blocks = np.add.reduceat(np.abs(d(x)), np.arange(0, R, 128), 0)
-    within(cs, np.add.reduceat(d(x), np.arange(0, R, 128), 0), 128 * U32 * blocks, "column sums")
-    q2 = ffn_ops.fp8_quantize(x.to(cuda), block_rows)[0]
-    assert torch.equal(q2.q, q.q)
+    for o, exps in ((q, fo.block_exponents(d(x), block_rows)), (qt, fo.block_exponents(d(x).T, block_rows))):
+        bytes_, e = o.bytes_and_exponents()
+        assert (bytes_[:, o.cols:] == 0).all()                                 # padding that products run over
+        np.testing.assert_array_equal(e.cpu().numpy(), exps.repeat(block_rows, 0)[: o.rows])
+    same = lambda a, b: torch.equal(a.values(), b.values())
+    assert same(ffn_ops.fp8_quantize(x.to(cuda), block_rows)[0], q) and same(ffn_ops.fp8_quantize(x.to(cuda), block_rows, False, True)[1], qt)
     wide = torch.zeros(R, C + 7, dtype=dtype, device=cuda)
     wide[:, 3:3 + C] = x.to(cuda)
     q3 = ffn_ops.fp8_quantize(wide[:, 3:3 + C], block_rows, True, True)
-    assert torch.equal(q3[0].q, q.q) and torch.equal(q3[1].q, qt.q)
+    assert same(q3[0], q) and same(q3[1], qt)
 
 
 @BOTH
@@ -492,6 +490,8 @@ def test_fp8_linear_against_64_bits(cuda, dtype, M, K, N):
     for act in ("none", "relu", "gelu"):
         want = fo.act(pre, act)
         tol = 1.13 * (_product_tol(xq, wq, dtype, 0 * pre) + 8 * U32 * np.abs(pre) + U32 * np.abs(d(b))) + 4 * U32 * np.abs(pre) + U[dtype] * np.abs(want)   # |gelu'| <= 1.13
+        if act == "gelu" and dtype == torch.bfloat16:       # the tail Phi(-|x|) of a bf16 result is a fit to 2.6e-4 relative
+            tol = tol + 2.6e-4 * np.abs(pre) * (0.5 - 0.5 * fo._erf(np.abs(pre) / math.sqrt(2)))
         got = ffn_ops.fp8_linear(x.to(cuda), plan, act)
         assert got.dtype == dtype
         within(got, want, tol, act)
@@ -507,7 +507,7 @@ def test_fp8_weight_from_blocks_and_infinities(cuda):
     e = torch.from_numpy(fo.block_exponents(d(w), 128)).to(cuda)
     v = (w * torch.exp2(-e.float()).repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)[:, :300]).to(torch.float8_e4m3fn)
     b = ffn_ops.Fp8Weight.from_blocks(v, e)
-    assert torch.equal(a.data.q, b.data.q) and torch.equal(a.data.values(), b.data.values())
+    assert all(torch.equal(p, q) for p, q in zip(a.data.bytes_and_exponents(), b.data.bytes_and_exponents()))
     x = torch.randn(5, 300, device=cuda)
     x[2, 17] = math.inf
     y = ffn_ops.fp8_linear(x, b)
