@@ -50,28 +50,75 @@ template <int L, int NT> struct RowSum {
   }
 };
 
-__device__ __forceinline__ void load_param(const void* p, int dtype, int col, int n, float (&o)[8], float fill) {
-  if (!p) {
+// Columns of a thread: K pieces of eight.  EXACT: the row is L * 8 * K wide, every thread owns all of its pieces.  RAGGED (at
+// least 8 wide): a piece that would reach past the row's end is moved back onto its last eight columns; the columns that it then
+// shares with its neighbour are computed twice and counted once.  So every load is whole and unconditional: a load behind a branch
+// of its own waits for the one before it.  TINY: fewer than eight columns, all of them the first thread's.
+enum { EXACT, RAGGED, TINY };
+template <int L, int K, int MODE> struct Cols {
+  int c[K], dup[K];          // first column, columns that another thread owns
+  int n;
+  __device__ __forceinline__ Cols(int t, int C) : n(C) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int at = (k * L + t) * 8;
+      c[k] = MODE == EXACT ? at : MODE == RAGGED ? min(at, C - 8) : 0;
+      dup[k] = MODE == EXACT ? 0 : MODE == RAGGED ? at - c[k] : t == 0 ? 0 : 8;
+    }
+  }
+  __device__ __forceinline__ bool mine(int k, int i) const {
+    return MODE == EXACT ? true : MODE == RAGGED ? i >= dup[k] : dup[k] == 0 && i < n;
+  }
+  __device__ __forceinline__ bool any(int k) const { return MODE == EXACT ? true : dup[k] < 8; }
+  template <typename T> __device__ __forceinline__ void raw(const T* row, int k, Raw8<T>& o) const {
+    if (MODE == TINY) o.load_part(row, n);
+    else o.load(row + c[k]);
+  }
+  template <typename T> __device__ __forceinline__ void store(T* row, int k, const float (&v)[8]) const {
+    if (MODE != TINY) Piece8<T>::store(row + c[k], v);
+    else store8(row, n, v);
+  }
+  template <typename P> __device__ __forceinline__ void param(const void* p, int k, float (&o)[8], float fill) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = fill;
-  } else if (dtype == PN_DTYPE_F32) {
-    load8(reinterpret_cast<const float*>(p) + col, n, o);
-  } else {
-    load8(reinterpret_cast<const __bf16*>(p) + col, n, o);
+    if (!p) return;
+    Raw8<P> r;
+    raw(reinterpret_cast<const P*>(p), k, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = r.get(i);
   }
-}
+};
 
-// mean and 1 / sqrt(var + eps) of the row held as v[K][8] (elements from `cols` on are not part of it)
-template <int K, typename Sum>
-__device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, float eps, int cols, int c0, int cstep, Sum& sum) {
+// The gate's row of a row that advances by `step` rows at a time: no division in the loop.
+struct GateRow {
+  long long row, rest, by, by_rest, per;
+  __device__ __forceinline__ GateRow(long long first, long long step, long long rows_per_gate) : per(rows_per_gate) {
+    row = first / per;
+    rest = first - row * per;
+    by = step / per;
+    by_rest = step - by * per;
+  }
+  __device__ __forceinline__ void next() {
+    row += by;
+    rest += by_rest;
+    if (rest >= per) {
+      rest -= per;
+      ++row;
+    }
+  }
+};
+
+// mean and 1 / sqrt(var + eps) of the row held as v[K][8]
+template <int K, typename Own, typename Sum>
+__device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, float eps, const Own& own, Sum& sum) {
   if (kind != PN_NORM_LAYER && kind != PN_NORM_RMS) return make_float2(0.f, 1.f);
   float mean = 0.f, s = 0.f;
   if (kind == PN_NORM_LAYER) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[k][i];
-    mean = sum(s, 0.f).x / (float)cols;
+      for (int i = 0; i < 8; ++i) s += own.mine(k, i) ? v[k][i] : 0.f;
+    mean = sum(s, 0.f).x / (float)own.n;
   }
   s = 0.f;
 #pragma unroll
@@ -79,83 +126,104 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, fl
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float d = v[k][i] - mean;
-      if (c0 + k * cstep + i < cols) s = fmaf(d, d, s);
+      s = own.mine(k, i) ? fmaf(d, d, s) : s;
     }
-  const float var = sum(s, 0.f).x / (float)cols;
+  const float var = sum(s, 0.f).x / (float)own.n;
   return make_float2(mean, 1.f / sqrtf(var + eps));
 }
 
-template <typename T, int L, int K, int NT>
+// FULL: the branch passes a post norm or dropout (with the registers that takes); otherwise gate and scale only.
+template <typename T, typename P, int L, int K, int NT, int MODE, bool FULL>
 __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
   constexpr int SLOTS = NT / L;
   __shared__ float2 lds[2 * (NT / 64)];
   RowSum<L, NT> sum{lds};
   const pnResidualNorm& p = a.p;
-  const int slot = threadIdx.x / L, t = threadIdx.x % L, C = p.cols;
+  const int slot = threadIdx.x / L, C = p.cols;
+  const Cols<L, K, MODE> own(threadIdx.x % L, C);
   const T* X = reinterpret_cast<const T*>(p.x);
   const T* F = reinterpret_cast<const T*>(p.branch);
+  const P* G = reinterpret_cast<const P*>(p.gate);
   T* H = reinterpret_cast<T*>(a.h);
   T* Y = reinterpret_cast<T*>(a.y);
   PhiloxKey key{};
-  if (p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
-  for (long long base = (long long)blockIdx.x * SLOTS; base < p.rows; base += (long long)gridDim.x * SLOTS) {
+  if (FULL && p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
+  float nw[K][8], nb[K][8], pw[FULL ? K : 1][8], pb[FULL ? K : 1][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    own.template param<P>(p.norm_weight, k, nw[k], 1.f);
+    own.template param<P>(p.norm_bias, k, nb[k], 0.f);
+    if (FULL) {
+      own.template param<P>(p.post_weight, k, pw[k], 1.f);
+      own.template param<P>(p.post_bias, k, pb[k], 0.f);
+    }
+  }
+  // The next row (and its gate) is on its way while this one is worked on; nothing is loaded in between, as waiting for a
+  // later load would wait for these too.  Past the last row the loads repeat it.
+  const long long step = (long long)gridDim.x * SLOTS, first = (long long)blockIdx.x * SLOTS + slot;
+  GateRow gate(first, step, p.rows_per_gate);
+  Raw8<T> nx[K], nf[K];
+  Raw8<P> ng[K];
+  auto fetch = [&](long long row) {
+    const bool in = row < p.rows;
+    row = in ? row : p.rows - 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) own.raw(X + row * p.ldx, k, nx[k]);
+    if (F) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) own.raw(F + row * p.ldb, k, nf[k]);
+    }
+    if (G) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) own.raw(G + (in ? gate.row * C : 0), k, ng[k]);
+    }
+  };
+  fetch(first);
+  for (long long base = (long long)blockIdx.x * SLOTS; base < p.rows; base += step) {
     const bool live = base + slot < p.rows;
     const long long row = live ? base + slot : p.rows - 1;
-    float h[K][8];
+    float h[K][8], f[K][8], g[K][8];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * L + t) * 8;
-      load8(X + row * p.ldx + c, C - c, h[k]);
-    }
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[k][i] = nx[k].get(i);
+        f[k][i] = F ? nf[k].get(i) : 0.f;
+        g[k][i] = G ? p.scale * ng[k].get(i) : p.scale;
+      }
+    gate.next();
+    if (base + step < p.rows) fetch(base + step + slot);
     float2 fs = make_float2(0.f, 1.f);
     if (F) {
-      float f[K][8];
+      if (FULL) fs = row_stats<K>(f, p.post_kind, p.post_eps, own, sum);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        load8(F + row * p.ldb + c, C - c, f[k]);
-      }
-      fs = row_stats<K>(f, p.post_kind, p.post_eps, C, t * 8, L * 8, sum);
-      const char* gate = reinterpret_cast<const char*>(p.gate);
-      if (gate) gate += row / p.rows_per_gate * C * (p.param_dtype == PN_DTYPE_F32 ? 4 : 2);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        float w[8], b[8], g[8];
-        load_param(p.post_weight, p.param_dtype, c, C - c, w, 1.f);
-        load_param(p.post_bias, p.param_dtype, c, C - c, b, 0.f);
-        load_param(gate, p.param_dtype, c, C - c, g, 1.f);
         uint32_t keep = 0xffu;
-        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + c, p.threshold);
+        if (FULL && p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + own.c[k], p.threshold);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float u = f[k][i];
-          if (p.post_kind != PN_NORM_NONE) u = fmaf((u - fs.x) * fs.y, w[i], b[i]);
-          u = (keep >> i & 1) ? u * a.keep_scale : 0.f;
-          h[k][i] = (float)(T)fmaf(p.scale * g[i], u, h[k][i]);
+          if (FULL) {
+            if (p.post_kind != PN_NORM_NONE) u = fmaf((u - fs.x) * fs.y, pw[k][i], pb[k][i]);
+            u = (keep >> i & 1) ? u * a.keep_scale : 0.f;
+          }
+          h[k][i] = (float)(T)fmaf(g[k][i], u, h[k][i]);
         }
-        if (live) store8(H + row * C + c, C - c, h[k]);
-        // what lies behind the row's end must not enter the norm's sums
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i >= C) h[k][i] = 0.f;
+        if (live && own.any(k)) own.store(H + row * C, k, h[k]);
       }
     }
     float2 hs = make_float2(0.f, 1.f);
     if (Y) {
-      hs = row_stats<K>(h, p.norm_kind, p.norm_eps, C, t * 8, L * 8, sum);
+      hs = row_stats<K>(h, p.norm_kind, p.norm_eps, own, sum);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        float w[8], b[8];
-        load_param(p.norm_weight, p.param_dtype, c, C - c, w, 1.f);
-        load_param(p.norm_bias, p.param_dtype, c, C - c, b, 0.f);
+        float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = act_f(fmaf((h[k][i] - hs.x) * hs.y, w[i], b[i]), p.act);
-        if (live) store8(Y + row * C + c, C - c, w);
+        for (int i = 0; i < 8; ++i) o[i] = act_f(fmaf((h[k][i] - hs.x) * hs.y, nw[k][i], nb[k][i]), p.act);
+        if (live && own.any(k)) own.store(Y + row * C, k, o);
       }
     }
-    if (a.stats && live && t == 0)
+    if (a.stats && live && threadIdx.x % L == 0)
       *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(hs.x, hs.y, fs.x, fs.y);
   }
 }
@@ -165,7 +233,7 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
 // order: no atomics, the same bits on every run.
 static constexpr int NSUM_NORM = 2, NSUM_ALL = 5;      // weight, bias | post weight, post bias, gate
 
-template <typename T, int L, int K, int NT, bool BRANCH>
+template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH>
 __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
   constexpr int SLOTS = NT / L, NS = BRANCH ? NSUM_ALL : NSUM_NORM;
   __shared__ float2 lds[2 * (NT / 64)];
@@ -173,6 +241,7 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
   RowSum<L, NT> sum{lds};
   const pnResidualNorm& p = a.p;
   const int slot = threadIdx.x / L, t = threadIdx.x % L, C = p.cols;
+  const Cols<L, K, MODE> own(t, C);
   const int group = blockIdx.x / a.chunks_per_group, chunk = blockIdx.x % a.chunks_per_group;
   const long long g_begin = (long long)group * a.group_rows, g_end = min(g_begin + a.group_rows, (long long)p.rows);
   const long long r_begin = g_begin + (long long)chunk * a.chunk_rows, r_end = min(r_begin + a.chunk_rows, g_end);
@@ -183,54 +252,94 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
   const T* GY = reinterpret_cast<const T*>(a.gy);
   PhiloxKey key{};
   if (BRANCH && p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
-  const char* gate_row = reinterpret_cast<const char*>(p.gate);
   const float inv_c = 1.f / (float)C;
-  float acc[NS][K][8];
+  const bool relu = p.act == PN_ACT_RELU;
+  const P* G = reinterpret_cast<const P*>(p.gate);
+  float acc[NS][K][8], nw[K][8], nb[K][8], pw[BRANCH ? K : 1][8], pb[BRANCH ? K : 1][8];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[s][k][i] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    own.template param<P>(p.norm_weight, k, nw[k], 1.f);
+    own.template param<P>(relu ? p.norm_bias : nullptr, k, nb[k], 0.f);
+    if (BRANCH) {
+      own.template param<P>(p.post_weight, k, pw[k], 1.f);
+      own.template param<P>(p.post_bias, k, pb[k], 0.f);
+    }
+  }
 
+  Raw8<T> ngh[K], ngy[K], nh[K], nf[K];
+  Raw8<P> ng[K];
+  float4 nst = make_float4(0.f, 1.f, 0.f, 1.f);
+  GateRow gate(min(r_begin + slot, r_end - 1), SLOTS, p.rows_per_gate);
+  auto fetch = [&](long long row) {                      // as in the forward pass, a row ahead
+    const bool in = row < r_end;
+    row = in ? row : r_end - 1;
+    if (BRANCH && G) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) own.raw(G + (in ? gate.row * C : 0), k, ng[k]);
+    }
+    if (GY) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        own.raw(GY + row * C, k, ngy[k]);
+        own.raw(H + row * ldh, k, nh[k]);
+      }
+    }
+    if (GH) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) own.raw(GH + row * C, k, ngh[k]);
+    }
+    if (BRANCH) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) own.raw(F + row * p.ldb, k, nf[k]);
+    }
+    if (a.stats) nst = *reinterpret_cast<const float4*>(a.stats + row * 4);
+  };
+  if (r_begin < r_end) fetch(r_begin + slot);
   for (long long base = r_begin; base < r_end; base += SLOTS) {
     const bool live = base + slot < r_end;
     const long long row = live ? base + slot : r_end - 1;
-    const float4 st = a.stats ? *reinterpret_cast<const float4*>(a.stats + row * 4) : make_float4(0.f, 1.f, 0.f, 1.f);
-    float dh[K][8];
+    Raw8<T> rgh[K], rgy[K], rh[K], rf[K];
+    Raw8<P> rg[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * L + t) * 8;
-      if (GH) {
-        load8(GH + row * C + c, C - c, dh[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dh[k][i] = 0.f;
-      }
+      rgh[k] = ngh[k];
+      rgy[k] = ngy[k];
+      rh[k] = nh[k];
+      rf[k] = nf[k];
+      rg[k] = ng[k];
     }
+    const float4 st = nst;
+    gate.next();
+    if (base + SLOTS < r_end) fetch(base + SLOTS + slot);
+    float dh[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dh[k][i] = GH ? rgh[k].get(i) : 0.f;
     if (GY) {
       float tw[K][8], hh[K][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        float w[8], b[8];
-        load8(GY + row * C + c, C - c, tw[k]);
-        load8(H + row * ldh + c, C - c, hh[k]);
-        load_param(p.norm_weight, p.param_dtype, c, C - c, w, 1.f);
-        if (p.act == PN_ACT_RELU) load_param(p.norm_bias, p.param_dtype, c, C - c, b, 0.f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          hh[k][i] = (hh[k][i] - st.x) * st.y;
-          if (c + i >= C) hh[k][i] = 0.f;
-          float g = tw[k][i];
-          if (p.act == PN_ACT_RELU && fmaf(hh[k][i], w[i], b[i]) <= 0.f) g = 0.f;
-          if (live) {
+          hh[k][i] = (rh[k].get(i) - st.x) * st.y;
+          float g = rgy[k].get(i);
+          if (relu && fmaf(hh[k][i], nw[k][i], nb[k][i]) <= 0.f) g = 0.f;
+          tw[k][i] = g * nw[k][i];
+          if (live && own.mine(k, i)) {
             acc[0][k][i] = fmaf(g, hh[k][i], acc[0][k][i]);
             acc[1][k][i] += g;
           }
-          tw[k][i] = g * w[i];
-          s1 += tw[k][i];
-          s2 = fmaf(tw[k][i], hh[k][i], s2);
+          if (own.mine(k, i)) {
+            s1 += tw[k][i];
+            s2 = fmaf(tw[k][i], hh[k][i], s2);
+          }
         }
       }
       if (p.norm_kind == PN_NORM_LAYER || p.norm_kind == PN_NORM_RMS) {
@@ -249,46 +358,37 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
     }
     if (a.dx) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        if (live) store8(reinterpret_cast<T*>(a.dx) + row * C + c, C - c, dh[k]);
-      }
+      for (int k = 0; k < K; ++k)
+        if (live && own.any(k)) own.store(reinterpret_cast<T*>(a.dx) + row * C, k, dh[k]);
     }
     if constexpr (BRANCH) {
-      const char* gate = gate_row ? gate_row + row / p.rows_per_gate * C * (p.param_dtype == PN_DTYPE_F32 ? 4 : 2) : nullptr;
       float fh[K][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        float w[8], b[8], g[8], dg[8];
-        load8(F + row * p.ldb + c, C - c, fh[k]);
-        load_param(p.post_weight, p.param_dtype, c, C - c, w, 1.f);
-        load_param(p.post_bias, p.param_dtype, c, C - c, b, 0.f);
-        load_param(gate, p.param_dtype, c, C - c, g, 1.f);
+        float dg[8];
         uint32_t keep = 0xffu;
-        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + c, p.threshold);
+        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + own.c[k], p.threshold);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          fh[k][i] = (fh[k][i] - st.z) * st.w;
-          if (c + i >= C) fh[k][i] = 0.f;
-          const float u = p.post_kind != PN_NORM_NONE ? fmaf(fh[k][i], w[i], b[i]) : fh[k][i];
+          fh[k][i] = (rf[k].get(i) - st.z) * st.w;
+          const float u = p.post_kind != PN_NORM_NONE ? fmaf(fh[k][i], pw[k][i], pb[k][i]) : fh[k][i];
           const bool kept = keep >> i & 1;
-          const float sd = p.scale * dh[k][i];
-          const float du = kept ? g[i] * sd * a.keep_scale : 0.f;
-          const float v = kept ? u * a.keep_scale : 0.f;
+          const float sd = p.scale * dh[k][i], v = kept ? u * a.keep_scale : 0.f;
+          const float du = kept ? (G ? rg[k].get(i) : 1.f) * sd * a.keep_scale : 0.f;
           dg[i] = sd * v;
-          if (live && c + i < C) {
+          if (live && own.mine(k, i)) {
             acc[NS - 1][k][i] += dg[i];
             acc[NS - 3][k][i] = fmaf(du, fh[k][i], acc[NS - 3][k][i]);
             acc[NS - 2][k][i] += du;
           }
-          dh[k][i] = p.post_kind != PN_NORM_NONE ? du * w[i] : du;
-          s1 += dh[k][i];
-          s2 = fmaf(dh[k][i], fh[k][i], s2);
+          dh[k][i] = p.post_kind != PN_NORM_NONE ? du * pw[k][i] : du;
+          if (own.mine(k, i)) {
+            s1 += dh[k][i];
+            s2 = fmaf(dh[k][i], fh[k][i], s2);
+          }
         }
-        if (a.dgate_rows && live) {
-          if (p.param_dtype == PN_DTYPE_F32) store8(reinterpret_cast<float*>(a.dgate_rows) + row * C + c, C - c, dg);
-          else store8(reinterpret_cast<__bf16*>(a.dgate_rows) + row * C + c, C - c, dg);
+        if (a.dgate_rows && live && own.any(k)) {
+          own.store(reinterpret_cast<P*>(a.dgate_rows) + row * C, k, dg);
         }
       }
       if (p.post_kind == PN_NORM_LAYER || p.post_kind == PN_NORM_RMS) {
@@ -301,38 +401,38 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
       }
       if (a.df) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int c = (k * L + t) * 8;
-          if (live) store8(reinterpret_cast<T*>(a.df) + row * C + c, C - c, dh[k]);
-        }
+        for (int k = 0; k < K; ++k)
+          if (live && own.any(k)) own.store(reinterpret_cast<T*>(a.df) + row * C, k, dh[k]);
       }
     }
   }
 
+  // the chunk's sums: add the workgroup's row slots, in order, every thread a share of the columns
   float* out = a.partial + (size_t)blockIdx.x * NS * C;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    if (SLOTS == 1) {
+  for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * L + t) * 8;
-        store8(out + s * C + c, C - c, acc[s][k]);
-      }
-    } else {                                     // add the workgroup's row slots, in order
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < K; ++k) {
+      if (SLOTS > 1) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cols_lds[slot * L * 8 + t * 8 + i] = acc[s][k][i];
+        for (int i = 0; i < 8; ++i) cols_lds[(slot * 8 + i) * L + t] = own.mine(k, i) ? acc[s][k][i] : 0.f;
         __syncthreads();
-        for (int c = threadIdx.x; c < L * 8; c += NT) {
+        // L * 8 columns, in the order (i, t) in which they lie; the columns that two threads share are the last one's to count
+        for (int q = threadIdx.x; q < L * 8; q += NT) {
+          const int i = q / L, tt = q % L;
+          const Cols<L, K, MODE> theirs(tt, C);
           float v = 0.f;
-          for (int q = 0; q < SLOTS; ++q) v += cols_lds[q * L * 8 + c];
-          if (k * L * 8 + c < C) out[s * C + k * L * 8 + c] = v;
+#pragma unroll 8
+          for (int z = 0; z < SLOTS; ++z) v += cols_lds[z * L * 8 + q];
+          if (theirs.mine(k, i)) out[s * C + theirs.c[k] + i] = v;
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (own.mine(k, i)) out[s * C + own.c[k] + i] = acc[s][k][i];
       }
     }
-  }
 }
 
 // out[v][c] = sum over the chunks of vector v: blockIdx.x picks the vector (weight, bias, post weight, post bias, then
@@ -353,6 +453,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
   float acc = 0.f;
   if (c < a.cols) {
     const float* p = a.partial + ((size_t)first * a.sums + s) * a.cols + c;
+#pragma unroll 8
     for (int i = w; i < count; i += 16) acc += p[(size_t)i * a.sums * a.cols];
   }
   lds[w][lane] = acc;
@@ -372,6 +473,7 @@ static int norm_check(const pnResidualNorm* p) {
   PN_CHECK_ARG(p->dtype == PN_DTYPE_F32 || p->dtype == PN_DTYPE_BF16, "residual_norm: element type %d (fp32 or bf16)", p->dtype);
   PN_CHECK_ARG(p->param_dtype == PN_DTYPE_F32 || p->param_dtype == PN_DTYPE_BF16, "residual_norm: parameter type %d (fp32 or bf16)",
                p->param_dtype);
+  PN_CHECK_ARG(p->dtype == PN_DTYPE_BF16 || p->param_dtype == PN_DTYPE_F32, "residual_norm: fp32 rows take fp32 parameters");
   PN_CHECK_ARG(p->cols >= 1 && p->cols <= PN_NORM_MAX_COLS, "residual_norm: %d columns (1..%d)", p->cols, PN_NORM_MAX_COLS);
   PN_CHECK_ARG(p->rows >= 0 && p->rows < (1ll << 40) / p->cols, "residual_norm: %lld rows", (long long)p->rows);
   PN_CHECK_ARG(p->post_kind >= PN_NORM_NONE && p->post_kind <= PN_NORM_RMS, "residual_norm: post norm %d (none, layer, rms)",
@@ -398,19 +500,35 @@ static NormArgs norm_args(const pnResidualNorm* p) {
   return a;
 }
 
+static constexpr int FWD_WAVES = 8192;                  // 32 a CU: what the forward kernel keeps resident
+
 // Threads per row: the fewest that hold the row at eight elements each, so that a narrow row does not idle a wave.
 #define NORM_BY_COLS(C, GO)                                                      \
   (C) <= 64 ? GO(8, 1, 256) : (C) <= 128 ? GO(16, 1, 256) : (C) <= 256 ? GO(32, 1, 256) : (C) <= 512 ? GO(64, 1, 256) \
   : (C) <= 1024 ? GO(128, 1, 256) : (C) <= 2048 ? GO(256, 1, 256) : (C) <= 4096 ? GO(512, 1, 512)              \
   : (C) <= 8192 ? GO(1024, 1, 1024) : GO(1024, 2, 1024)
 
-template <typename T, int L, int K, int NT> static int norm_fwd(const NormArgs& a, hipStream_t s) {
-  const long long need = (a.p.rows + NT / L - 1) / (NT / L);
-  const unsigned grid = (unsigned)(need < (1 << 30) ? need : (1 << 30));
-  hipLaunchKernelGGL((residual_norm_fwd_kernel<T, L, K, NT>), dim3(grid), dim3(NT), 0, s, a);
+template <typename T, typename P, int L, int K, int NT> static int norm_fwd(const NormArgs& a, hipStream_t s) {
+  const bool full = a.p.post_kind != PN_NORM_NONE || a.p.threshold;
+#define FWD(MODE, L_, K_, NT_)                                                                                                \
+  do {                                                                                                                       \
+    const long long need = (a.p.rows + NT_ / L_ - 1) / (NT_ / L_), most = FWD_WAVES / (NT_ / 64);                            \
+    const dim3 grid((unsigned)(need < most ? need : most)), wg(NT_);                                                         \
+    if (full) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, true>), grid, wg, 0, s, a);              \
+    else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, false>), grid, wg, 0, s, a);                  \
+  } while (0)
+  if (a.p.cols == L * K * 8) FWD(EXACT, L, K, NT);
+  else if (a.p.cols >= 8) FWD(RAGGED, L, K, NT);
+  else FWD(TINY, 8, 1, 256);
+#undef FWD
   PN_CHECK_LAUNCH("residual_norm_fwd_kernel");
   return PN_OK;
 }
+
+// element type and parameter type: fp32 rows go with fp32 parameters, bf16 rows with either
+#define NORM_BY_TYPE(DTYPE, PTYPE, COLS, GO)                                                       \
+  ((DTYPE) == PN_DTYPE_F32 ? (NORM_BY_COLS(COLS, GO##_F32)) : (PTYPE) == PN_DTYPE_F32 ? (NORM_BY_COLS(COLS, GO##_MIX)) \
+                                                                                       : (NORM_BY_COLS(COLS, GO##_BF16)))
 
 extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* y, float* stats, void* stream) {
   const int rc = norm_check(p);
@@ -423,16 +541,17 @@ extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* 
   a.y = p->norm_kind == PN_NORM_NONE ? nullptr : y;
   a.stats = stats;
   hipStream_t s = (hipStream_t)stream;
-#define GO_F32(L, K, NT) norm_fwd<float, L, K, NT>(a, s)
-#define GO_BF16(L, K, NT) norm_fwd<__bf16, L, K, NT>(a, s)
-  if (p->dtype == PN_DTYPE_F32) return NORM_BY_COLS(p->cols, GO_F32);
-  return NORM_BY_COLS(p->cols, GO_BF16);
+#define GO_F32(L, K, NT) norm_fwd<float, float, L, K, NT>(a, s)
+#define GO_MIX(L, K, NT) norm_fwd<__bf16, float, L, K, NT>(a, s)
+#define GO_BF16(L, K, NT) norm_fwd<__bf16, __bf16, L, K, NT>(a, s)
+  return NORM_BY_TYPE(p->dtype, p->param_dtype, p->cols, GO);
 #undef GO_F32
+#undef GO_MIX
 #undef GO_BF16
 }
 
 // Chunks of the backward pass: about NORM_WGS workgroups in all, whole passes over the row slots, none across two gates.
-static constexpr int NORM_WGS = 1024;
+static constexpr int NORM_WGS = 512;
 struct NormChunks { long long groups, group_rows; int per_group, rows, sums; };
 static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
   NormChunks c;
@@ -460,9 +579,16 @@ extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
   return (size_t)c.groups * c.per_group * c.sums * p->cols * sizeof(float);
 }
 
-template <typename T, int L, int K, int NT> static int norm_bwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
-  if (branch) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, L, K, NT, true>), dim3(grid), dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, L, K, NT, false>), dim3(grid), dim3(NT), 0, s, a);
+template <typename T, typename P, int L, int K, int NT> static int norm_bwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
+#define BWD(MODE, L_, K_, NT_)                                                                                              \
+  do {                                                                                                                     \
+    if (branch) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, P, L_, K_, NT_, MODE, true>), dim3(grid), dim3(NT_), 0, s, a); \
+    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, P, L_, K_, NT_, MODE, false>), dim3(grid), dim3(NT_), 0, s, a);       \
+  } while (0)
+  if (a.p.cols == L * K * 8) BWD(EXACT, L, K, NT);
+  else if (a.p.cols >= 8) BWD(RAGGED, L, K, NT);
+  else BWD(TINY, 8, 1, 256);
+#undef BWD
   PN_CHECK_LAUNCH("residual_norm_bwd_kernel");
   return PN_OK;
 }
@@ -506,10 +632,12 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
     a.chunk_rows = c.rows;
     a.chunks_per_group = c.per_group;
     a.group_rows = c.group_rows;
-#define GO_F32(L, K, NT) norm_bwd<float, L, K, NT>(a, branch, (unsigned)chunks, s)
-#define GO_BF16(L, K, NT) norm_bwd<__bf16, L, K, NT>(a, branch, (unsigned)chunks, s)
-    const int r = p->dtype == PN_DTYPE_F32 ? (NORM_BY_COLS(p->cols, GO_F32)) : (NORM_BY_COLS(p->cols, GO_BF16));
+#define GO_F32(L, K, NT) norm_bwd<float, float, L, K, NT>(a, branch, (unsigned)chunks, s)
+#define GO_MIX(L, K, NT) norm_bwd<__bf16, float, L, K, NT>(a, branch, (unsigned)chunks, s)
+#define GO_BF16(L, K, NT) norm_bwd<__bf16, __bf16, L, K, NT>(a, branch, (unsigned)chunks, s)
+    const int r = NORM_BY_TYPE(p->dtype, p->param_dtype, p->cols, GO);
 #undef GO_F32
+#undef GO_MIX
 #undef GO_BF16
     if (r != PN_OK) return r;
   }

@@ -277,22 +277,25 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8GemmArgs a) {
 #endif
 }
 
-// 256 x 256 tiles for large products: eight waves of 128 x 64 in two groups of four, one wave of each group on every SIMD,
-// half a block apart.  While one group multiplies its block from registers, the other reads its own from LDS (the first also
+// Large products: 256 x 256 tiles, eight waves of 128 x 64 (WIDE: 128 x 256 tiles, waves of 64 x 64) in two groups of four, one
+// wave of each group on every SIMD, half a block apart.  While one group multiplies its block from registers, the other reads its own from LDS (the first also
 // sends for the block after); then they change places (two barriers a block).  The matrix pipe of a SIMD always has a wave that needs
 // nothing else.
-struct Fp8Pair {
-  static constexpr int BM = 256, BN = 256, NW = 8, FM = 8, FN = 4, XBYTES = BM * 128, BUF = (BM + BN) * 128, SBUF = (BM + BN) * 4;
-  static constexpr int PROWS = 16, PARK = PROWS * 64 * 2, LDS = 2 * BUF + 2 * SBUF + NW * PARK;
+// WIDE, the widening to bf16 is part of the reading half: two vector instructions for each matrix instruction that would otherwise
+// wait for them (8192^3: 933 us with all waves in step).
+template <bool WIDE> struct Fp8Pair {
+  static constexpr int BM = WIDE ? 128 : 256, BN = 256, NW = 8, FM = BM / 32, FN = 4, XBYTES = BM * 128, BUF = (BM + BN) * 128;
+  static constexpr int SBUF = 2048, PARK = WIDE ? 0 : 16 * 64 * 2, LDS = 2 * BUF + 2 * SBUF + NW * PARK;   // scale words: 256 rows of x, 256 of w
 };
+template <bool WIDE>
 __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  typedef Fp8Pair C;
+  typedef Fp8Pair<WIDE> C;
   constexpr int NW = C::NW, FM = C::FM, FN = C::FN, BUF = C::BUF, XBYTES = C::XBYTES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lk = lane >> 4;
   const int group = wave >> 2;                            // waves 0-3 and 4-7: one of each on every SIMD
-  const int wm = group * 128, wn = (wave & 3) * 64;
+  const int wm = group * (C::BM / 2), wn = (wave & 3) * 64;
   const unsigned strip = (unsigned)a.kblocks * 2048u;     // bytes of a group of 16 rows
   const int total = a.tiles_m * a.tiles_n, per = (total + 7) / 8;
   const int end = min((int)(blockIdx.x & 7) * per + per, total), step = (int)gridDim.x >> 3;
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
   auto stage = [&](int kb) {
     char* base = smem + (kb & 1) * BUF + wave * 1024;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < C::BM / 32; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(base + j * 4096), 16, voff + j * 2 * strip,
                                                kb * 2048, 0, 0);
 #pragma unroll
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
   enter(lin);
   if (!group) stage(0);
   bool stores_behind = false;
-  constexpr int STORES = FM * 16 / 8;
+  constexpr int STORES = WIDE ? FM * FN : FM * 2;
   while (true) {
     fp8_f32x4 acc[FM][FN];
 #pragma unroll
@@ -361,31 +364,50 @@ __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
     for (int kb = 0; kb < a.kblocks; ++kb) {
       // reading; nobody reads block kb - 1 any more, so block kb + 1 may land in its place
       if (!group && kb + 1 < a.kblocks) stage(kb + 1);
-      const char* bx = smem + (kb & 1) * BUF + wm * 128 + lane * 16;
-      const char* bw = smem + (kb & 1) * BUF + XBYTES + wn * 128 + lane * 16;
+      const char* lx = smem + (kb & 1) * BUF + wm * 128 + lane * 16;
+      const char* lw = smem + (kb & 1) * BUF + XBYTES + wn * 128 + lane * 16;
       const unsigned char* sc = reinterpret_cast<const unsigned char*>(smem) + 2 * BUF + ((kb >> 2) & 1) * C::SBUF + (kb & 3);
       i32x8 fx[FM], fw[FN];
       uint32_t sx[FM], sw[FN];
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        const i32x4 lo = *reinterpret_cast<const i32x4*>(bw + j * 2048), hi = *reinterpret_cast<const i32x4*>(bw + j * 2048 + 1024);
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(lw + j * 2048), hi = *reinterpret_cast<const i32x4*>(lw + j * 2048 + 1024);
         fw[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        sw[j] = sc[(C::BM + wn + j * 16 + lr) * 4];
+        sw[j] = sc[(256 + wn + j * 16 + lr) * 4];
       }
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const i32x4 lo = *reinterpret_cast<const i32x4*>(bx + i * 2048), hi = *reinterpret_cast<const i32x4*>(bx + i * 2048 + 1024);
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(lx + i * 2048), hi = *reinterpret_cast<const i32x4*>(lx + i * 2048 + 1024);
         fx[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         sx[i] = sc[(wm + i * 16 + lr) * 4];
       }
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_waitcnt(0xc07f);                 // lgkmcnt(0): the reads are done
+      fp8_bf16x8 bx[WIDE ? FM : 1][4], bw_[WIDE ? FN : 1][4];
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int j = 0; j < FN; ++j) bw_[j][e] = widen8(fw[j][2 * e], fw[j][2 * e + 1], scale_of(sw[j]));
+#pragma unroll
+          for (int i = 0; i < FM; ++i) bx[i][e] = widen8(fx[i][2 * e], fx[i][2 * e + 1], scale_of(sx[i]));
+        }
+      }
       PAIR_BARRIER();
       __builtin_amdgcn_s_setprio(1);
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_fp8(fw[j], fx[i], acc[i][j], sw[j], sx[i]);   // D[n][m]
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw_[j][e], bx[i][e], acc[i][j], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma_fp8(fw[j], fx[i], acc[i][j], sw[j], sx[i]);   // D[n][m]
+      }
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
       asm volatile("" ::: "memory");
@@ -413,36 +435,56 @@ __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    char* park = smem + 2 * BUF + 2 * C::SBUF + wave * C::PARK;
-    __bf16* out = reinterpret_cast<__bf16*>(a.out) + om * a.ldo + on;
+    if constexpr (WIDE) {
+      float* out = reinterpret_cast<float*>(a.out) + om * a.ldo + on;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        typedef __attribute__((ext_vector_type(4))) __bf16 V4;
-        V4 o;
+        for (int j = 0; j < FN; ++j) {
+          struct __attribute__((packed, aligned(4))) Raw { float v[4]; } q;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (__bf16)act_bf16(acc[i][j][e] + bias[j][e], a.act);
-        const int at = j * 32 + ek * 8;
-        *reinterpret_cast<V4*>(park + er * 128 + (((at >> 4) ^ (er >> 1)) << 4) + (at & 15)) = o;
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the wave's own rows: no other wave touches them
+          for (int e = 0; e < 4; ++e) q.v[e] = act_f(acc[i][j][e] + bias[j][e], a.act);
+          float* o = out + (i * 16 + er) * a.ldo + j * 16 + ek * 4;
+          if (whole) {
+            *reinterpret_cast<Raw*>(o) = q;
+          } else if (i * 16 + er < left_m) {
 #pragma unroll
-      for (int r = 0; r < 16; r += 8) {
-        const int row = r + (el >> 3), ch = el & 7;
-        const uint4 v = *reinterpret_cast<const uint4*>(park + row * 128 + ((ch ^ (row >> 1)) << 4));
-        struct __attribute__((packed, aligned(2))) Raw { __bf16 v[8]; };    // rows of odd length start at any element
-        const Raw q = __builtin_bit_cast(Raw, v);
-        __bf16* o = out + (i * 16 + row) * a.ldo + ch * 8;
-        if (whole) {
-          *reinterpret_cast<Raw*>(o) = q;
-        } else if (i * 16 + row < left_m) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (ch * 8 + e < left_n) o[e] = q.v[e];
+            for (int e = 0; e < 4; ++e)
+              if (j * 16 + ek * 4 + e < left_n) o[e] = q.v[e];
+          }
         }
+    } else {
+      char* park = smem + 2 * BUF + 2 * C::SBUF + wave * C::PARK;
+      __bf16* out = reinterpret_cast<__bf16*>(a.out) + om * a.ldo + on;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          typedef __attribute__((ext_vector_type(4))) __bf16 V4;
+          V4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = (__bf16)act_bf16(acc[i][j][e] + bias[j][e], a.act);
+          const int at = j * 32 + ek * 8;
+          *reinterpret_cast<V4*>(park + er * 128 + (((at >> 4) ^ (er >> 1)) << 4) + (at & 15)) = o;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the wave's own rows: no other wave touches them
+#pragma unroll
+        for (int r = 0; r < 16; r += 8) {
+          const int row = r + (el >> 3), ch = el & 7;
+          const uint4 v = *reinterpret_cast<const uint4*>(park + row * 128 + ((ch ^ (row >> 1)) << 4));
+          struct __attribute__((packed, aligned(2))) Raw { __bf16 v[8]; };    // rows of odd length start at any element
+          const Raw q = __builtin_bit_cast(Raw, v);
+          __bf16* o = out + (i * 16 + row) * a.ldo + ch * 8;
+          if (whole) {
+            *reinterpret_cast<Raw*>(o) = q;
+          } else if (i * 16 + row < left_m) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (ch * 8 + e < left_n) o[e] = q.v[e];
+          }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // read before the next rows overwrite them
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // read before the next rows overwrite them
     }
     if (!more) break;
     stores_behind = whole;
@@ -507,9 +549,17 @@ template <> struct RawRows<float> {
   }
 };
 
+struct Fp8Laid {};         // x is an operand already
+template <> struct RawRows<Fp8Laid> {
+  static constexpr int LOADS = 2, LANES = 16, EACH = 8;
+  i32x4 v[2];
+  uint32_t scale;
+};
+
 template <typename T, int FN, int NW, int DEPTH, bool WIDE>
 __global__ __launch_bounds__(NW * 64) void fp8_direct_kernel(Fp8DirectArgs d) {
   typedef RawRows<T> R;
+  constexpr bool LAID = std::is_same<T, Fp8Laid>::value;
   constexpr int OWN = 2048 + 16;                          // a wave's part of LDS: a block's bytes and its rows' scales
   const Fp8GemmArgs& a = d.g;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -524,8 +574,11 @@ __global__ __launch_bounds__(NW * 64) void fp8_direct_kernel(Fp8DirectArgs d) {
   // lane's rows of x: row j * (64 / LANES) + lane / LANES of the strip, EACH elements from (lane % LANES) * EACH on; rows past the
   // end repeat the last one (their outputs are not stored)
   const T* px[R::LOADS];
+  const unsigned char* qx = a.x + (size_t)tm * a.kblocks * 2048 + lane * 16;
+  const unsigned char* qs = reinterpret_cast<const unsigned char*>(a.xs + (m0 + lr < a.M ? m0 + lr : a.M - 1));
 #pragma unroll
   for (int j = 0; j < R::LOADS; ++j) {
+    if (LAID) break;
     const long long m = m0 + j * (64 / R::LANES) + lane / R::LANES;
     px[j] = reinterpret_cast<const T*>(d.x) + (m < a.M ? m : a.M - 1) * d.ldx + (lane % R::LANES) * R::EACH;
   }
@@ -556,8 +609,14 @@ __global__ __launch_bounds__(NW * 64) void fp8_direct_kernel(Fp8DirectArgs d) {
       nw[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       ns[j] = ps[j][(long long)(kb >> 2) * a.N * 4 + (kb & 3)];
     }
+    if constexpr (LAID) {
 #pragma unroll
-    for (int j = 0; j < R::LOADS; ++j) nx.load(j, px[j] + min(kb * 128, tail));
+      for (int j = 0; j < 2; ++j) nx.v[j] = *reinterpret_cast<const i32x4*>(qx + (size_t)kb * 2048 + j * 1024);
+      nx.scale = qs[(long long)(kb >> 2) * a.x_rows * 4 + (kb & 3)];
+    } else {
+#pragma unroll
+      for (int j = 0; j < R::LOADS; ++j) nx.load(j, px[j] + min(kb * 128, tail));
+    }
     __builtin_amdgcn_sched_barrier(0);                    // the loads of a block stay together, in order
   };
 #pragma unroll
@@ -567,41 +626,50 @@ __global__ __launch_bounds__(NW * 64) void fp8_direct_kernel(Fp8DirectArgs d) {
     for (int s = 0; s < DEPTH; ++s) {
       const int kb = kb0 + s * NW;
       if (kb >= a.kblocks) break;
-      // element e of the 128 that were read is k = e - shift of the block; those before the block are dropped
-      const int shift = kb * 128 > tail ? kb * 128 - tail : 0;
-      uint32_t mag[R::LOADS], any = 0;
-      if (shift) {
+      i32x4 lo, hi;
+      uint32_t sx;
+      if constexpr (LAID) {
+        lo = x[s].v[0];
+        hi = x[s].v[1];
+        sx = x[s].scale;
+      } else {
+        // element e of the 128 that were read is k = e - shift of the block; those before the block are dropped
+        const int shift = kb * 128 > tail ? kb * 128 - tail : 0;
+        uint32_t mag[R::LOADS], any = 0;
+        if (shift) {
 #pragma unroll
-        for (int j = 0; j < R::LOADS; ++j) x[s].drop(j, shift - k_own);
-      }
-#pragma unroll
-      for (int j = 0; j < R::LOADS; ++j) {
-        mag[j] = x[s].template mag<false>(j);
-        any = Raw8<T>::mag_max(any, mag[j]);
-      }
-      if (Raw8<T>::mag_inf(any)) {                        // rare: leave out what is not finite
-#pragma unroll
-        for (int j = 0; j < R::LOADS; ++j) mag[j] = x[s].template mag<true>(j);
-      }
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int j = 0; j < R::LOADS; ++j) {
-        const int sc = block_scale(R::row_max(mag[j])), row = j * (64 / R::LANES) + lane / R::LANES;
-        const uint2 o = x[s].quant(j, scale_value((uint32_t)sc));
-        auto place = [&](int k) { return own + ((k >> 4) & 1) * 1024 + ((k >> 5) * 16 + row) * 16 + (k & 15); };
-        if (!shift) {
-          if (R::EACH == 8) *reinterpret_cast<uint2*>(place(k_own)) = o;
-          else *reinterpret_cast<uint32_t*>(place(k_own)) = o.x;
-        } else {                                          // byte by byte; the dropped elements' zeros fill the block's end
-#pragma unroll
-          for (int i = 0; i < R::EACH; ++i) *place((k_own + i - shift) & 127) = (char)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
+          for (int j = 0; j < R::LOADS; ++j) x[s].drop(j, shift - k_own);
         }
-        if (lane % R::LANES == 0) own[2048 + row] = (char)sc;
+#pragma unroll
+        for (int j = 0; j < R::LOADS; ++j) {
+          mag[j] = x[s].template mag<false>(j);
+          any = Raw8<T>::mag_max(any, mag[j]);
+        }
+        if (Raw8<T>::mag_inf(any)) {                        // rare: leave out what is not finite
+#pragma unroll
+          for (int j = 0; j < R::LOADS; ++j) mag[j] = x[s].template mag<true>(j);
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < R::LOADS; ++j) {
+          const int sc = block_scale(R::row_max(mag[j])), row = j * (64 / R::LANES) + lane / R::LANES;
+          const uint2 o = x[s].quant(j, scale_value((uint32_t)sc));
+          auto place = [&](int k) { return own + ((k >> 4) & 1) * 1024 + ((k >> 5) * 16 + row) * 16 + (k & 15); };
+          if (!shift) {
+            if (R::EACH == 8) *reinterpret_cast<uint2*>(place(k_own)) = o;
+            else *reinterpret_cast<uint32_t*>(place(k_own)) = o.x;
+          } else {                                          // byte by byte; the dropped elements' zeros fill the block's end
+#pragma unroll
+            for (int i = 0; i < R::EACH; ++i) *place((k_own + i - shift) & 127) = (char)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
+          }
+          if (lane % R::LANES == 0) own[2048 + row] = (char)sc;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own part: no other wave touches it
+        lo = *reinterpret_cast<const i32x4*>(own + lane * 16);
+        hi = *reinterpret_cast<const i32x4*>(own + 1024 + lane * 16);
+        sx = (unsigned char)own[2048 + lr];
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own part: no other wave touches it
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(own + lane * 16), hi = *reinterpret_cast<const i32x4*>(own + 1024 + lane * 16);
       const i32x8 q = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      const uint32_t sx = (unsigned char)own[2048 + lr];
       if (WIDE) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -690,60 +758,15 @@ template <int BM, int BN, int WM, int WN, int RING, bool WIDE> static int fp8_ti
   return PN_OK;
 }
 
-static int fp8_pair(Fp8GemmArgs a, hipStream_t s) {
-  typedef Fp8Pair C;
+template <bool WIDE> static int fp8_pair(Fp8GemmArgs a, hipStream_t s) {
+  typedef Fp8Pair<WIDE> C;
   static bool raised = false;
-  const int rc = fp8_raise_lds((const void*)fp8_pair_kernel, C::LDS, &raised);
+  const int rc = fp8_raise_lds((const void*)fp8_pair_kernel<WIDE>, C::LDS, &raised);
   if (rc != PN_OK) return rc;
   const unsigned grid = fp8_grid(a, C::BM, C::BN, 1);
-  hipLaunchKernelGGL(fp8_pair_kernel, dim3(grid), dim3(512), C::LDS, s, a);
+  hipLaunchKernelGGL(fp8_pair_kernel<WIDE>, dim3(grid), dim3(512), C::LDS, s, a);
   PN_CHECK_LAUNCH("fp8_pair_kernel");
   return PN_OK;
-}
-
-// Time of a product by tiles, in us: whole rounds of the workgroups that fit on the device, each a cost per block and one per
-// tile.  Measured on 256 CUs (8192^3 and 16384 x 4096 x 8192: rounds of 64 and 32 blocks; 512 x 3136 x 256: 25 blocks, a tile or
-// less a CU): 256 x 256 in pairs 398 / 450 us, 128 x 128 523 / 562 (fp32 outputs 944 / 990), 64 x 64 764 / 884 (1239 / 1327).
-struct Fp8Cost { int bm, resident; float round_block, round_tile, lone_block, lone_tile; };
-static const Fp8Cost FP8_PAIR = {256, 1, 1.35f, 13.f, 1.35f, 13.f};
-static const Fp8Cost FP8_128[2] = {{128, 2, 0.95f, 4.8f, 0.78f, 3.f}, {128, 2, 1.75f, 5.8f, 1.25f, 3.f}};       // bf16, fp32 outputs
-static const Fp8Cost FP8_64[2] = {{64, 4, 0.63f, 5.f, 0.35f, 2.6f}, {64, 4, 1.12f, 5.6f, 0.52f, 2.6f}};
-static float fp8_cost(const Fp8Cost& c, long long m, int n, int kblocks, int cus) {
-  const long long tiles = (m + c.bm - 1) / c.bm * ((n + c.bm - 1) / c.bm);
-  if (tiles <= cus) return c.lone_block * kblocks + c.lone_tile;
-  return (float)((tiles + cus * c.resident - 1) / (cus * c.resident)) * (c.round_block * kblocks + c.round_tile);
-}
-
-template <bool WIDE> static int fp8_small(const Fp8GemmArgs& a, int cus, hipStream_t s) {
-  if (fp8_cost(FP8_64[WIDE], a.M, a.N, a.kblocks, cus) <= fp8_cost(FP8_128[WIDE], a.M, a.N, a.kblocks, cus))
-    return fp8_tile<64, 64, 2, 2, 2, WIDE>(a, s);
-  return fp8_tile<128, 128, 2, 2, 2, WIDE>(a, s);
-}
-
-int fp8_gemm_launch(const Fp8Gemm& g, hipStream_t s) {
-  Fp8GemmArgs a = {g.x.q, g.w.q, g.x.scale, g.w.scale, g.M, g.M, g.N, (g.K + 127) / 128, (g.K + 511) / 512, 0, 0,
-                   g.bias, g.bias_dtype, g.act, g.out_dtype, g.out, g.ldo};
-  const int cus = fp8_cus(), kb = a.kblocks;
-  if (g.out_dtype == PN_DTYPE_F32) return fp8_small<true>(a, cus, s);
-  auto small = [&](long long m) {
-    const float c64 = fp8_cost(FP8_64[0], m, g.N, kb, cus), c128 = fp8_cost(FP8_128[0], m, g.N, kb, cus);
-    return c64 < c128 ? c64 : c128;
-  };
-  const float by_small = small(g.M), by_pair = fp8_cost(FP8_PAIR, g.M, g.N, kb, cus);
-  // Rows that fill whole 256-row tiles, and the few behind them in a launch of their own: 8200 x 2048 x 4096 takes 94 us as
-  // three rounds of 256 x 256, 90 us in 128 x 128, and two rounds and a strip of 8 rows
-  const long long whole = g.M & ~255ll;
-  const float by_split = whole && whole < g.M ? fp8_cost(FP8_PAIR, whole, g.N, kb, cus) + small(g.M - whole) : 1e30f;
-  if (by_small <= by_pair && by_small <= by_split) return fp8_small<false>(a, cus, s);
-  if (by_pair <= by_split) return fp8_pair(a, s);
-  Fp8GemmArgs t = a;
-  a.M = whole;
-  t.M = g.M - whole;
-  t.x += (size_t)(whole / 16) * kb * 2048;
-  t.xs += whole;
-  t.out = reinterpret_cast<__bf16*>(g.out) + whole * g.ldo;
-  const int rc = fp8_pair(a, s);
-  return rc != PN_OK ? rc : fp8_small<false>(t, cus, s);
 }
 
 template <typename T, int FN, int NW, int DEPTH> static int fp8_direct(Fp8DirectArgs d, hipStream_t s) {
@@ -756,6 +779,64 @@ template <typename T, int FN, int NW, int DEPTH> static int fp8_direct(Fp8Direct
   else hipLaunchKernelGGL((fp8_direct_kernel<T, FN, NW, DEPTH, false>), grid, wg, LDS, s, d);
   PN_CHECK_LAUNCH("fp8_direct_kernel");
   return PN_OK;
+}
+
+// Time of a product by tiles, in us: whole rounds of the workgroups that fit on the device, each a cost per block and one per
+// tile.  Measured on 256 CUs (8192^3 and 16384 x 4096 x 8192: rounds of 64 and 32 blocks; 512 x 3136 x 256: 25 blocks, a tile or
+// less a CU): pairs, 256 x 256, 398 / 450 us (fp32 outputs, 128 x 256: 865 / 940); 128 x 128 523 / 562 (1000 / 998); 64 x 64
+// 764 / 884 (1239 / 1327).
+struct Fp8Cost { int bm, bn, resident; float round_block, round_tile, lone_block, lone_tile; };
+static const Fp8Cost FP8_PAIR[2] = {{256, 256, 1, 1.35f, 13.f, 1.35f, 13.f}, {128, 256, 1, 1.6f, 14.f, 1.6f, 14.f}};  // bf16, fp32 outputs
+static const Fp8Cost FP8_128[2] = {{128, 128, 2, 0.95f, 4.8f, 0.78f, 3.f}, {128, 128, 2, 1.85f, 6.f, 1.25f, 7.f}};
+static const Fp8Cost FP8_64[2] = {{64, 64, 4, 0.63f, 5.f, 0.35f, 2.6f}, {64, 64, 4, 1.12f, 5.6f, 0.52f, 2.6f}};
+static float fp8_cost(const Fp8Cost& c, long long m, int n, int kblocks, int cus) {
+  const long long tiles = (m + c.bm - 1) / c.bm * ((n + c.bn - 1) / c.bn);
+  if (tiles <= cus) return c.lone_block * kblocks + c.lone_tile;
+  return (float)((tiles + cus * c.resident - 1) / (cus * c.resident)) * (c.round_block * kblocks + c.round_tile);
+}
+
+// Few tiles and a long contraction: a CU takes 64 x 64 x 128 in 0.35 us however few of them there are (what it loads), so the
+// work is spread over more CUs by 16 rows x 32 or 64 columns, the blocks dealt to a workgroup's waves (512 x 3136 x 256: 6 us
+// against 11).
+static bool fp8_spread(long long m, int n, int k) { return k >= 1024 && (m + 15) / 16 * ((n + 63) / 64) <= 256; }
+template <typename T> static int fp8_direct_by_size(const Fp8DirectArgs& d, hipStream_t s) {
+  return (d.g.M + 15) / 16 * ((d.g.N + 31) / 32) <= 256 ? fp8_direct<T, 2, 8, 2>(d, s) : fp8_direct<T, 4, 8, 2>(d, s);
+}
+
+template <bool WIDE> static int fp8_small(const Fp8GemmArgs& a, int cus, hipStream_t s) {
+  if (fp8_spread(a.M, a.N, a.kblocks * 128)) return fp8_direct_by_size<Fp8Laid>(Fp8DirectArgs{a, nullptr, 0, a.kblocks * 128}, s);
+  if (fp8_cost(FP8_64[WIDE], a.M, a.N, a.kblocks, cus) <= fp8_cost(FP8_128[WIDE], a.M, a.N, a.kblocks, cus))
+    return fp8_tile<64, 64, 2, 2, 2, WIDE>(a, s);
+  return fp8_tile<128, 128, 2, 2, 2, WIDE>(a, s);
+}
+
+template <bool WIDE> static int fp8_gemm_by_size(Fp8GemmArgs a, hipStream_t s) {
+  const int cus = fp8_cus(), kb = a.kblocks, bm = FP8_PAIR[WIDE].bm;
+  auto small = [&](long long m) {
+    const float c64 = fp8_cost(FP8_64[WIDE], m, a.N, kb, cus), c128 = fp8_cost(FP8_128[WIDE], m, a.N, kb, cus);
+    return c64 < c128 ? c64 : c128;
+  };
+  const float by_small = small(a.M), by_pair = fp8_cost(FP8_PAIR[WIDE], a.M, a.N, kb, cus);
+  // Rows that fill whole tiles of the pair kernel, and the few behind them in a launch of their own: 8200 x 2048 x 4096 takes
+  // 94 us as three rounds of 256 x 256, 90 us in 128 x 128, 72 us as two rounds and 8 for a strip of 8 rows
+  const long long whole = a.M / bm * bm;
+  const float by_split = whole && whole < a.M ? fp8_cost(FP8_PAIR[WIDE], whole, a.N, kb, cus) + small(a.M - whole) : 1e30f;
+  if (by_small <= by_pair && by_small <= by_split) return fp8_small<WIDE>(a, cus, s);
+  if (by_pair <= by_split) return fp8_pair<WIDE>(a, s);
+  Fp8GemmArgs t = a;
+  a.M = whole;
+  t.M -= whole;
+  t.x += (size_t)(whole / 16) * kb * 2048;
+  t.xs += whole;
+  t.out = (char*)t.out + whole * t.ldo * (WIDE ? 4 : 2);
+  const int rc = fp8_pair<WIDE>(a, s);
+  return rc != PN_OK ? rc : fp8_small<WIDE>(t, cus, s);
+}
+
+int fp8_gemm_launch(const Fp8Gemm& g, hipStream_t s) {
+  const Fp8GemmArgs a = {g.x.q, g.w.q, g.x.scale, g.w.scale, g.M, g.M, g.N, (g.K + 127) / 128, (g.K + 511) / 512, 0, 0,
+                         g.bias, g.bias_dtype, g.act, g.out_dtype, g.out, g.ldo};
+  return g.out_dtype == PN_DTYPE_F32 ? fp8_gemm_by_size<true>(a, s) : fp8_gemm_by_size<false>(a, s);
 }
 
 static int fp8_check(const void* w, long long m, int n, int k, const void* bias, int bias_dtype, int act, int out_dtype, void* out, long long ldo) {
@@ -799,9 +880,7 @@ extern "C" int pn_fp8_linear(int dtype, const void* x, long long m, long long ld
   if (fp8_is_direct(m, n, k)) {
     Fp8DirectArgs d = {{nullptr, (const unsigned char*)w, nullptr, fp8_operand(w, n, k).scale, m, m, n, (k + 127) / 128, (k + 511) / 512, 0, 0,
                         bias, bias_dtype, act, out_dtype, out, ldo}, x, m == 1 ? 0 : ldx, k};
-    const bool narrow = (m + 15) / 16 * ((n + 31) / 32) <= 256;
-    if (dtype == PN_DTYPE_F32) return narrow ? fp8_direct<float, 2, 8, 2>(d, s) : fp8_direct<float, 4, 8, 2>(d, s);
-    return narrow ? fp8_direct<__bf16, 2, 8, 2>(d, s) : fp8_direct<__bf16, 4, 8, 2>(d, s);
+    return dtype == PN_DTYPE_F32 ? fp8_direct_by_size<float>(d, s) : fp8_direct_by_size<__bf16>(d, s);
   }
   if (ws_bytes < fp8_bytes(m, k) || !ws) {
     pn_set_error("pn_fp8_linear: workspace of %zu bytes is too small", ws_bytes);

@@ -189,8 +189,10 @@ __global__ __launch_bounds__(256) void fp8_colsum_kernel(const float* partial, l
   __shared__ float lds[4][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (long long i = w; i < blocks; i += 4) s += partial[i * cols + c];
+  }
   lds[w][lane] = s;
   __syncthreads();
   if (w == 0 && c < cols) {

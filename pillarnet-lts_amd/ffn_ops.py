@@ -289,7 +289,8 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
             rng, call = None, 0
     params = [gate, pw, pb, w, b]
     kinds = {t.dtype for t in params if t is not None}
-    if len(kinds) > 1:                  # the kernels read parameters of one type
+    if len(kinds) > 1 or (kinds and x.dtype == torch.float32 and torch.bfloat16 in kinds):
+        # the kernels read parameters of one type, of fp32 where the rows are
         params = [None if t is None else t.float() for t in params]
     gate, pw, pb, w, b = [None if t is None else t.contiguous() for t in params]
     cfg = _JoinCfg(_lib.PN_NORM[post_norm.kind] if post_norm is not None else 0, _lib.PN_NORM[norm.kind] if norm is not None else 0,

@@ -68,7 +68,7 @@ def _join(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=2), dict(param_dtype=7), dict(cols=0), dict(cols=16385), dict(rows=-1), dict(post_kind=3), dict(norm_kind=4),
+    dict(dtype=2), dict(param_dtype=7), dict(param_dtype=1), dict(cols=0), dict(cols=16385), dict(rows=-1), dict(post_kind=3), dict(norm_kind=4),
     dict(act=2), dict(branch=None, gate=16), dict(branch=None, post_kind=1), dict(branch=None, threshold=5, rng=16),
     dict(branch=None, norm_kind=0), dict(threshold=65537, rng=16), dict(threshold=1), dict(call=65536), dict(x=None),
     dict(ldx=7), dict(ldb=7), dict(gate=16, rows_per_gate=3), dict(gate=16, rows_per_gate=0)])
