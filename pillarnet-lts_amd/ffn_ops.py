@@ -38,14 +38,22 @@ def _check(what, *tensors):
             raise PillarnetHipError(f"{what}: {t.dtype} (fp32 or bf16)")
 
 
+_FN = {}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _call(name, device, *args):
     """One C entry on `device`'s current stream, with `device` current during the launch."""
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.lib(), name)
+    i = device.index
+    if i == _current_device():
+        rc = fn(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
     if rc:
         _lib.check(rc, name)
 
@@ -58,7 +66,7 @@ def _rows(x):
     """x as [rows, cols] with unit column stride and a row stride >= cols; a copy only where no view has them."""
     C = x.shape[-1]
     if x.is_contiguous():
-        return x.view(-1, C) if C else x.reshape(0, 0)
+        return x if x.dim() == 2 else x.view(-1, C) if C else x.reshape(0, 0)
     try:
         v = x.view(-1, C)
         if v.stride(1) == 1 and (v.shape[0] <= 1 or v.stride(0) >= C):
@@ -69,7 +77,21 @@ def _rows(x):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _backward(fn):
+    """A backward pass that is not itself differentiable: the guard against a second derivative is only put up where one could
+    be asked for (create_graph), as it costs as much host time as a launch."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return staticmethod(backward)
 
 
 # ---- activation + dropout ----------------------------------------------------------------------------------------------
@@ -105,10 +127,11 @@ def _check_rng(what, rng, device, call):
 
 
 def _act_dropout_forward(x, threshold, rng, call, act):
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     v = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), v.shape[0], v.shape[1], v.stride(0), act, threshold,
-          _ptr(rng), call, y.data_ptr())
+    R, C = v.shape
+    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), R, C, v.stride(0), act, threshold, _ptr(rng), call,
+          y.data_ptr())
     return y
 
 
@@ -120,16 +143,16 @@ class _ActDropout(torch.autograd.Function):
         ctx.args = (threshold, call, act)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, g):
         rng, saved = ctx.saved_tensors
         threshold, call, act = ctx.args
+        dx = torch.empty_like(g, memory_format=torch.contiguous_format)
         gv = _rows(g)
         sv = None if saved is None else _rows(saved)
-        dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), gv.shape[0], gv.shape[1],
-              gv.stride(0), 0 if sv is None else sv.stride(0), act, threshold, _ptr(rng), call, dx.data_ptr())
+        R, C = gv.shape
+        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), R, C, gv.stride(0),
+              0 if sv is None else sv.stride(0), act, threshold, _ptr(rng), call, dx.data_ptr())
         return dx, None, None, None, None
 
 
@@ -187,8 +210,8 @@ def _join_struct(cfg, x, f, gate, pw, pb, w, b, rng):
 
 def _join_forward(cfg, x, f, gate, pw, pb, w, b, rng, want_stats):
     s, keep = _join_struct(cfg, x, f, gate, pw, pb, w, b, rng)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if cfg.norm else None
+    h = torch.empty_like(x, memory_format=torch.contiguous_format) if f is not None else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if cfg.norm else None
     stats = torch.empty((s.rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
     if s.rows:                          # (an empty tensor has no address to tell the branch by)
         _call("pn_residual_norm_forward", x.device, byref(s), _ptr(h), _ptr(y), _ptr(stats))
@@ -206,8 +229,7 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return (h, y) if f is not None and cfg.norm else h if f is not None else y
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, *grads):
         cfg = ctx.cfg
         rng, h, f, gate, pw, pb, w, b, stats = ctx.saved_tensors
@@ -223,6 +245,8 @@ class _ResidualNorm(torch.autograd.Function):
         s, keep = _join_struct(cfg, h, (f if ctx.reads_f else h) if ctx.has_branch else None, gate, pw, pb, w, b, rng)
         gh = None if gh is None else gh.contiguous()
         gy = None if gy is None else gy.contiguous()
+        if gy is None and ctx.has_branch and not ctx.reads_f:
+            return None, None, gh if need[0] else None, gh if need[1] else None, None, None, None, None, None
         dx = torch.empty(shape, dtype=dt, device=dev) if need[0] or (need[1] and not ctx.reads_f) else None
         df = torch.empty(shape, dtype=dt, device=dev) if need[1] and ctx.reads_f else None
         sums = [torch.empty_like(t, memory_format=torch.contiguous_format) if n and t is not None else None
@@ -287,12 +311,15 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
             _check_rng(what, rng, x.device, call)
         else:
             rng, call = None, 0
-    params = [gate, pw, pb, w, b]
-    kinds = {t.dtype for t in params if t is not None}
-    if len(kinds) > 1 or (kinds and x.dtype == torch.float32 and torch.bfloat16 in kinds):
-        # the kernels read parameters of one type, of fp32 where the rows are
-        params = [None if t is None else t.float() for t in params]
-    gate, pw, pb, w, b = [None if t is None else t.contiguous() for t in params]
+    first = None
+    for t in (gate, pw, pb, w, b):
+        if t is not None and (first is not None and t.dtype != first or t.dtype != torch.float32 and x.dtype == torch.float32
+                              or not t.is_contiguous()):
+            # the kernels read dense parameters of one type, of fp32 where the rows are
+            same = x.dtype == torch.bfloat16 and len({q.dtype for q in (gate, pw, pb, w, b) if q is not None}) == 1
+            gate, pw, pb, w, b = [None if q is None else (q if same else q.float()).contiguous() for q in (gate, pw, pb, w, b)]
+            break
+        first = first if t is None else t.dtype
     cfg = _JoinCfg(_lib.PN_NORM[post_norm.kind] if post_norm is not None else 0, _lib.PN_NORM[norm.kind] if norm is not None else 0,
                    post_norm.eps if post_norm is not None else 0.0, norm.eps if norm is not None else 0.0, float(scale), threshold, call,
                    _lib.PN_ACT[act], rows_per_gate)
@@ -444,8 +471,7 @@ class _Fp8Linear(torch.autograd.Function):
         ctx.meta = (x.shape, weight.dtype, None if bias is None else bias.dtype)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, g):
         need_x, need_w, need_b = ctx.needs_input_grad
         (saved,) = ctx.saved_tensors
