@@ -15,7 +15,7 @@ import torch.nn as nn
 
 import torch.nn.functional as Fn
 
-from . import _lib, builder, dense_hip, iou3d_nms
+from . import _lib, builder, dense_hip, ffn_ops, iou3d_nms
 from .detectors import BaseDetector
 from .nn_utils import build_norm_layer
 from .registry import DETECTORS, POINT_HEAD, ROI_HEAD, SECOND_STAGE
@@ -122,11 +122,16 @@ def roi_grid_pool_torch(rois, feature_map, grid, cell_size, x_min, y_min):
     return out.view(B, R, grid * grid, C), pts
 
 
+FP8_PLANS = dense_hip.PlanCache()      # weights laid out for fp8 products (PLANS holds the same modules' fp32 plans)
+
+
 class FoldedMLP:
     """Eval-mode stack of (Conv1d(k=1) | Linear) + BatchNorm1d + ReLU [+ Dropout] ... as plain fp32
-    `relu(x @ W' + b')` launches with the norm folded into W', b'."""
+    `relu(x @ W' + b')` launches with the norm folded into W', b'; `fp8`: the products in e4m3 with block scales
+    (ffn_ops.fp8_linear), fp32 in between."""
 
-    def __init__(self, layers):
+    def __init__(self, layers, fp8=False):
+        self.fp8 = fp8
         mods = [m for m in layers if not isinstance(m, nn.Dropout)]
         self.steps, i = [], 0
         while i < len(mods):
@@ -143,11 +148,17 @@ class FoldedMLP:
                 j += 1
             if j < len(mods) and isinstance(mods[j], nn.ReLU):
                 relu, j = True, j + 1
-            self.steps.append((w.t().float().contiguous(), b.float().contiguous(), relu))
+            if fp8:
+                self.steps.append((ffn_ops.Fp8Weight(w.float(), b.float()), None, relu))
+            else:
+                self.steps.append((w.t().float().contiguous(), b.float().contiguous(), relu))
             i = j
 
     def __call__(self, x):
         for wt, b, relu in self.steps:
+            if self.fp8:
+                x = ffn_ops.fp8_linear(x, wt, "relu" if relu else "none")
+                continue
             x = torch.addmm(b, x, wt)
             if relu:
                 x = torch.relu_(x)
@@ -528,6 +539,14 @@ class MLPMixer(nn.Module):
         x = self.token_mixer(x) + x
         return self.channel_mixer(x) + x
 
+    def forward_fused(self, x, linear):
+        """The same with the norms, residuals and activations on the fused kernels; `linear`: how a Linear is run."""
+        ln1, conv1, _, conv2 = self.token_mixer
+        ln2, fc1, _, fc2 = self.channel_mixer
+        t = conv2(ffn_ops.act_dropout(conv1(ffn_ops.residual_norm(x, norm=ffn_ops.Norm.of(ln1))), 0.0, act="gelu"))
+        x, n = ffn_ops.residual_norm(x, t, norm=ffn_ops.Norm.of(ln2))
+        return ffn_ops.residual_norm(x, linear(fc2, linear(fc1, n, "gelu")))
+
 
 class _Affine(nn.Module):
     def __init__(self, dim):
@@ -560,6 +579,14 @@ class ResMLPLayer(nn.Module):
         x = x + self.channel_scale * self.channel_mixer(x)
         return self.post_aff(x)
 
+    def forward_fused(self, x, linear):
+        """The same with every affine, layer scale and residual on the fused kernels; `linear`: how a Linear is run."""
+        aff = lambda m: ffn_ops.Norm("affine", m.alpha.view(-1), m.beta.view(-1))
+        fc1, _, fc2 = self.channel_mixer
+        x = ffn_ops.residual_norm(x, norm=aff(self.token_aff))
+        _, x = ffn_ops.residual_norm(x, self.token_mixer(x), gate=self.token_scale, norm=aff(self.channel_aff))
+        return ffn_ops.residual_norm(x, linear(fc2, linear(fc1, x, "gelu")), gate=self.channel_scale, norm=aff(self.post_aff))[1]
+
 
 def _fc_stack(cfg_list, cin, cout, dp_ratio, conv=True):
     layers, pre = [], cin
@@ -581,6 +608,59 @@ class RoIHeadTemplate(nn.Module):
         self.model_cfg, self.num_class = model_cfg, num_class
         self.proposal_target_layer = ProposalTargetLayer(model_cfg["TARGET_CONFIG"]) if "TARGET_CONFIG" in model_cfg else None
         self.use_iou, self.forward_ret_dict = False, None
+        self.use_fused(False)
+
+    def use_fused(self, fused_ops=True, fp8=False, dropout_seed=None):
+        """fused_ops: the head's norms, residuals, activations and dropouts run on ffn_ops (the dropouts then draw from a
+        counter-based generator of their own instead of torch's: other masks, the same distribution).  fp8 (implies fused_ops):
+        its Linear / 1x1 layers too, as products in e4m3 with block scales, forward and backward.  dropout_seed: the
+        generator's seed (default torch.initial_seed(); data-parallel ranks add their rank)."""
+        self.fused_ops, self.fp8, self.dropout_seed, self._dropout_state = bool(fused_ops or fp8), bool(fp8), dropout_seed, None
+        return self
+
+    def draw_dropout(self, device):
+        """The generator's state for one pass of this head (None outside of training)."""
+        if not self.training:
+            return None
+        if self._dropout_state is None or self._dropout_state.state.device != device:
+            seed = torch.initial_seed() if self.dropout_seed is None else int(self.dropout_seed)
+            if torch.distributed.is_available() and torch.distributed.is_initialized():
+                seed += torch.distributed.get_rank()
+            self._dropout_state = ffn_ops.DropoutState(seed, device)
+        return self._dropout_state.draw()
+
+    def fused_linear(self, m, x, act="none"):
+        """A Linear or a Conv1d of kernel size 1 on rows [..., C], then the activation."""
+        w = m.weight.flatten(1)
+        grads = torch.is_grad_enabled() and (x.requires_grad or m.weight.requires_grad or (m.bias is not None and m.bias.requires_grad))
+        if self.fp8 and not grads:
+            plan = FP8_PLANS.get(m, lambda m: ffn_ops.Fp8Weight(m.weight.flatten(1), m.bias))
+            return ffn_ops.fp8_linear(x.detach(), plan, act)
+        y = ffn_ops.fp8_linear_train(x, w, m.bias) if self.fp8 else Fn.linear(x, w, m.bias)
+        return y if act == "none" else ffn_ops.act_dropout(y, 0.0, act=act)
+
+    def fused_stack(self, layers, x, rng=None, call=0):
+        """Conv1d(k=1) | Linear, BatchNorm1d / LayerNorm, ReLU, Dropout ... on rows [N, C]; a ReLU and the Dropout behind it are one
+        launch, so are a LayerNorm and the ReLU behind it.  -> (rows, the next dropout's call number)."""
+        mods, i = list(layers), 0
+        follows = lambda kind: i + 1 < len(mods) and isinstance(mods[i + 1], kind)
+        while i < len(mods):
+            m = mods[i]
+            if isinstance(m, (nn.Conv1d, nn.Linear)):
+                x = self.fused_linear(m, x)
+            elif isinstance(m, nn.LayerNorm):
+                relu = follows(nn.ReLU)
+                x, i = ffn_ops.residual_norm(x, norm=ffn_ops.Norm.of(m), act="relu" if relu else "none"), i + relu
+            elif isinstance(m, (nn.ReLU, nn.Dropout)):
+                relu = isinstance(m, nn.ReLU)
+                drop = (mods[i + 1] if follows(nn.Dropout) else None) if relu else m
+                p = drop.p if drop is not None and self.training else 0.0
+                x = ffn_ops.act_dropout(x, p, rng, call, "relu" if relu else "none")
+                call, i = call + (p > 0), i + (relu and drop is not None)
+            else:
+                x = m(x)
+            i += 1
+        return x, call
 
     def make_fc_layers(self, input_channels, output_channels, fc_list):
         """roi_head_template.py:23-39."""
@@ -689,8 +769,9 @@ class RoIMIXHead(RoIHeadTemplate):
     """roi_mix_head.py:17-122 on the shared template (roi_head_template.py)."""
 
     def __init__(self, in_channels=None, model_cfg=None, num_class=1, code_size=7, add_box_param=False, test_cfg=None,
-                 mixer_type=None, num_patches=49, **kwargs):
+                 mixer_type=None, num_patches=49, fused_ops=False, fp8=False, dropout_seed=None, **kwargs):
         super().__init__(num_class=num_class, model_cfg=model_cfg)
+        self.use_fused(fused_ops, fp8, dropout_seed)
         if in_channels is None:
             in_channels = kwargs.pop("input_channels")          # the legacy configs' name for it
         self.test_cfg = test_cfg
@@ -718,6 +799,10 @@ class RoIMIXHead(RoIHeadTemplate):
                     nn.init.constant_(m.bias, 0)
         nn.init.normal_(self.reg_layers[-1].weight, mean=0, std=0.001)
 
+    def _mix(self, x):
+        fused = self.fused_ops and isinstance(self.mlp_mixer, (MLPMixer, ResMLPLayer))
+        return self.mlp_mixer.forward_fused(x, self.fused_linear) if fused else self.mlp_mixer(x)
+
     def _forward_train(self, batch_dict):
         """roi_mix_head.py:81-121 with training=True: the module path (BatchNorm statistics, Dropout)."""
         td = batch_dict.get("roi_targets_dict", None)
@@ -725,9 +810,16 @@ class RoIMIXHead(RoIHeadTemplate):
             td = self.assign_targets(batch_dict)
             batch_dict["rois"], batch_dict["roi_labels"], batch_dict["roi_scores"] = td["rois"], td["roi_labels"], td["roi_scores"]
         B, R = batch_dict["rois"].shape[:2]
-        feats = self.mlp_mixer(batch_dict["roi_features"].view(B * R, self.num_patches, -1))
+        feats = self._mix(batch_dict["roi_features"].view(B * R, self.num_patches, -1))
         if self.add_box_param:
             feats = torch.cat([feats, batch_dict["rois"], batch_dict["roi_scores"].unsqueeze(-1)], dim=-1)
+        if self.fused_ops:
+            rng = self.draw_dropout(feats.device)
+            x, call = self.fused_stack(self.shared_fc_layer, feats.reshape(B * R, -1), rng)
+            td["rcnn_cls"], call = self.fused_stack(self.cls_layers, x, rng, call)
+            td["rcnn_reg"], _ = self.fused_stack(self.reg_layers, x, rng, call)
+            self.forward_ret_dict = td
+            return batch_dict
         x = self.shared_fc_layer(feats.reshape(B * R, -1, 1))
         td["rcnn_cls"] = self.cls_layers(x).transpose(1, 2).contiguous().squeeze(dim=1)
         td["rcnn_reg"] = self.reg_layers(x).transpose(1, 2).contiguous().squeeze(dim=1)
@@ -739,11 +831,11 @@ class RoIMIXHead(RoIHeadTemplate):
             return self._forward_train(batch_dict)
         B = len(batch_dict["rois"])
         R = batch_dict["rois"].shape[1]
-        feats = self.mlp_mixer(batch_dict["roi_features"].view(B * R, self.num_patches, -1))
+        feats = self._mix(batch_dict["roi_features"].view(B * R, self.num_patches, -1))
         if self.add_box_param:
             feats = torch.cat([feats, batch_dict["rois"], batch_dict["roi_scores"].unsqueeze(-1)], dim=-1)
-        shared, cls_mlp, reg_mlp = dense_hip.PLANS.get(self, lambda m: (
-            FoldedMLP(m.shared_fc_layer), FoldedMLP(m.cls_layers), FoldedMLP(m.reg_layers)))
+        shared, cls_mlp, reg_mlp = (FP8_PLANS if self.fp8 else dense_hip.PLANS).get(self, lambda m: tuple(
+            FoldedMLP(f, m.fp8) for f in (m.shared_fc_layer, m.cls_layers, m.reg_layers)))
         x = shared(feats.reshape(B * R, -1).float())
         cls, reg = cls_mlp(x), reg_mlp(x)
         c, b = self.generate_predicted_boxes(batch_dict["batch_size"], batch_dict["rois"], cls, reg)
@@ -790,8 +882,10 @@ class RoIFFNHead(RoIHeadTemplate):
 
     def __init__(self, model_cfg, num_cls_fcs=1, num_reg_fcs=1, num_iou_fcs=1, feedforward_channels=2048,
                  content_dim=256, num_ffn_fcs=2, dropout=0.0, ffn_act_cfg=dict(type="ReLU", inplace=True),
-                 num_class=1, code_size=7, test_cfg=None, init_bias=-2.19, add_box_param=False):
+                 num_class=1, code_size=7, test_cfg=None, init_bias=-2.19, add_box_param=False, fused_ops=False, fp8=False,
+                 dropout_seed=None):
         super().__init__(num_class=num_class, model_cfg=model_cfg)
+        self.use_fused(fused_ops, fp8, dropout_seed)
         self.test_cfg, self.code_size, self.add_box_param, self.init_bias = test_cfg, code_size, add_box_param, init_bias
         self.use_iou = num_iou_fcs > 0
         self.ffn = FFN(content_dim, feedforward_channels, num_ffn_fcs, act_cfg=ffn_act_cfg, dropout=dropout)
@@ -827,6 +921,21 @@ class RoIFFNHead(RoIHeadTemplate):
             nn.init.zeros_(self.fc_iou.weight)
             nn.init.zeros_(self.fc_iou.bias)
 
+    def _query_fused(self, x):
+        """ffn_norm(x + dropout(ffn layers(x))): the widening layers' activation and dropout are one launch each, the residual, the
+        last dropout and the norm another."""
+        p, f = self.ffn.dropout.p if self.training else 0.0, x
+        rng = self.draw_dropout(x.device) if p > 0 else None
+        *wide, last = self.ffn.layers
+        for call, (fc, act, _) in enumerate(wide):
+            kind = "relu" if isinstance(act, nn.ReLU) else "gelu"
+            f = ffn_ops.act_dropout(self.fused_linear(fc, f), p, rng, call, kind) if p > 0 else self.fused_linear(fc, f, kind)
+        f = self.fused_linear(last, f)
+        norm = ffn_ops.Norm.of(self.ffn_norm)
+        if not self.ffn.add_residual:
+            return ffn_ops.residual_norm(ffn_ops.act_dropout(f, p, rng, len(wide)), norm=norm)
+        return ffn_ops.residual_norm(x, f, norm=norm, dropout=(p, rng, len(wide)) if p > 0 else None)[1]
+
     def forward(self, batch_dict, training=True):
         """roi_ffn_head.py:81-140."""
         if training:
@@ -838,16 +947,18 @@ class RoIFFNHead(RoIHeadTemplate):
             batch_dict["roi_features"] = torch.cat([batch_dict["roi_features"], batch_dict["rois"],
                                                     batch_dict["roi_scores"].unsqueeze(-1)], dim=-1)
         batch_dict["roi_features"] = batch_dict["roi_features"].view(-1, batch_dict["roi_features"].shape[-1])
-        query = self.ffn_norm(self.ffn(batch_dict["roi_features"]))
+        query = self._query_fused(batch_dict["roi_features"]) if self.fused_ops else self.ffn_norm(self.ffn(batch_dict["roi_features"]))
 
-        def run(layers, x):
-            for m in layers:
+        def run(layers, last, x):
+            if self.fused_ops:
+                return self.fused_stack([*layers, last], x)[0]
+            for m in [*layers, last]:
                 x = m(x)
             return x
 
-        rcnn_cls = self.fc_cls(run(self.cls_fcs, query))
-        rcnn_reg = self.fc_reg(run(self.reg_fcs, query))
-        rcnn_iou = self.fc_iou(run(self.iou_fcs, query)) if self.use_iou else None
+        rcnn_cls = run(self.cls_fcs, self.fc_cls, query)
+        rcnn_reg = run(self.reg_fcs, self.fc_reg, query)
+        rcnn_iou = run(self.iou_fcs, self.fc_iou, query) if self.use_iou else None
         if not training:
             c, b = self.generate_predicted_boxes(batch_dict["batch_size"], batch_dict["rois"], rcnn_cls, rcnn_reg)
             batch_dict["batch_cls_preds"], batch_dict["batch_box_preds"] = c, b
@@ -953,8 +1064,11 @@ class PillarRCNN(BaseDetector):
         self.point_head = builder.build_point_head(point_head) if point_head is not None else None
         self.roi_head = builder.build_roi_head(roi_head)
 
-    def to_inference(self, dtype=torch.bfloat16, device="cuda", dense_backend="hip"):
+    def to_inference(self, dtype=torch.bfloat16, device="cuda", dense_backend="hip", roi_fp8=False):
+        """roi_fp8: the RoI head's layers as products in fp8 with block scales (RoIHeadTemplate.use_fused)."""
         self.single_det.to_inference(dtype, device, dense_backend)
+        if roi_fp8:
+            self.roi_head.use_fused(fp8=True)
         self.eval().to(device)
         for m in list(self.second_stage) + [self.point_head, self.roi_head]:
             if m is not None:
