@@ -81,23 +81,38 @@ __device__ __forceinline__ void philox(const PhiloxKey& k, unsigned long long gr
     k1 += 0xBB67AE85u;
   }
 }
-__device__ __forceinline__ uint32_t philox_u16(const uint32_t (&c)[4], int i) { return (c[i >> 1] >> (16 * (i & 1))) & 0xffffu; }
 
-// keep decisions of the eight elements that start at linear index e (a group boundary or not): bit i set = kept
-__device__ __forceinline__ uint32_t keep_bits8(const PhiloxKey& k, unsigned long long e, uint32_t threshold) {
-  uint32_t c[4], bits = 0;
-  philox(k, e >> 3, c);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bits |= (philox_u16(c, i) >= threshold ? 1u : 0u) << i;
+// Keep decisions of eight elements: element i is kept if its 16 bits are >= threshold, compared in the upper half of a word, so
+// that every second one needs no shift.  `past` = (threshold - 1) << 16 | 0xffff: > past means the half is >= threshold.
+struct Keep8 {
+  uint32_t c[4], past;
+  __device__ __forceinline__ bool operator()(int i) const { return (i & 1 ? c[i >> 1] : c[i >> 1] << 16) > past; }
+};
+// threshold 1 .. 65536; without dropping (0) the caller takes the others' branch: everything is kept
+__device__ __forceinline__ uint32_t keep_past(uint32_t threshold) { return (threshold - 1) << 16 | 0xffffu; }
+__device__ __forceinline__ Keep8 keep_all() { return Keep8{{~0u, ~0u, ~0u, ~0u}, 0x80000000u}; }
+__device__ __forceinline__ Keep8 keep8_group(const PhiloxKey& k, unsigned long long group, uint32_t threshold) {
+  Keep8 o;
+  o.past = keep_past(threshold);
+  philox(k, group, o.c);
+  return o;
+}
+// ... that start at linear index e, a group's first element or not: bits of two groups, spread to whole halves (0xffff is kept)
+__device__ __forceinline__ Keep8 keep8_at(const PhiloxKey& k, unsigned long long e, uint32_t threshold) {
+  Keep8 o = keep8_group(k, e >> 3, threshold);
   const int sh = (int)(e & 7);
   if (sh) {
-    uint32_t hi = 0;
-    philox(k, (e >> 3) + 1, c);
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi |= (philox_u16(c, i) >= threshold ? 1u : 0u) << i;
-    bits = ((bits | hi << 8) >> sh) & 0xffu;
+    for (int i = 0; i < 8; ++i) bits |= o(i) ? 1u << i : 0u;
+    philox(k, (e >> 3) + 1, o.c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits |= o(i) ? 256u << i : 0u;
+    bits >>= sh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.c[i] = (bits >> (2 * i) & 1) * 0xffffu | (bits >> (2 * i + 1) & 1) * 0xffff0000u;
   }
-  return bits;
+  return o;
 }
 
 // GELU from the normal distribution's tail: with z = |x| / sqrt(2), q = Phi(-|x|) = exp(-z^2) * erfcx(z) / 2, and
@@ -185,6 +200,19 @@ template <> struct Raw8<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
   }
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f;
+  }
+  __device__ __forceinline__ uint4 words(int j) const {
+    return make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+  }
+  __device__ __forceinline__ void set_words(int j, uint4 w) {
+    v[4 * j] = __uint_as_float(w.x);
+    v[4 * j + 1] = __uint_as_float(w.y);
+    v[4 * j + 2] = __uint_as_float(w.z);
+    v[4 * j + 3] = __uint_as_float(w.w);
+  }
   __device__ __forceinline__ float get(int i) const { return v[i]; }
   template <bool FINITE> __device__ __forceinline__ uint32_t mag(int i) const {
     const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
@@ -237,6 +265,17 @@ template <> struct Raw8<__bf16> {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = 0u;
+  }
+  __device__ __forceinline__ void fill(float f) {          // f: a bf16 value
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(f) >> 16) * 0x10001u;
+  }
+  __device__ __forceinline__ uint4 words(int) const { return make_uint4(v[0], v[1], v[2], v[3]); }
+  __device__ __forceinline__ void set_words(int, uint4 w) {
+    v[0] = w.x;
+    v[1] = w.y;
+    v[2] = w.z;
+    v[3] = w.w;
   }
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
   template <bool FINITE> __device__ __forceinline__ uint32_t mag(int i) const {

@@ -47,17 +47,17 @@ __global__ __launch_bounds__(256) void act_dropout_kernel(DropArgs a) {
   const T* xp = reinterpret_cast<const T*>(a.x);
   if (!BWD || ACT != PN_ACT_NONE) load8_view(xp, a.ldx, a.cols, e, n, x);
   if (BWD) load8_view(reinterpret_cast<const T*>(a.g), a.ldg, a.cols, e, n, g);
-  uint32_t keep = 0xffu;
-  if (a.threshold && !(BWD && ACT == PN_ACT_RELU)) keep = keep_bits8(philox_key(a.rng, a.call), e, a.threshold);
+  Keep8 keep = keep_all();
+  if (a.threshold && !(BWD && ACT == PN_ACT_RELU)) keep = keep8_group(philox_key(a.rng, a.call), e >> 3, a.threshold);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (!BWD) {
-      o[i] = (keep >> i & 1) ? act_f(x[i], ACT) * a.scale : 0.f;
+      o[i] = keep(i) ? act_f(x[i], ACT) * a.scale : 0.f;
     } else if (ACT == PN_ACT_RELU) {
       o[i] = x[i] <= 0.f ? 0.f : g[i] * a.scale;
     } else {
       const float d = ACT == PN_ACT_GELU ? gelu_grad_f(x[i]) : 1.f;
-      o[i] = (keep >> i & 1) ? g[i] * a.scale * d : 0.f;
+      o[i] = keep(i) ? g[i] * a.scale * d : 0.f;
     }
   }
   store8(reinterpret_cast<T*>(a.out) + e, n, o);

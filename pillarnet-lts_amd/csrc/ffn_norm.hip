@@ -20,48 +20,75 @@ struct NormArgs {
   float keep_scale;
 };
 
-// sums over the L threads that share a row (L <= 64: shuffles; more: one LDS exchange, two buffers so that one barrier is
-// enough).  The order of the additions depends on L alone.
+// a + its neighbour's: lanes 1, 2, 4, 8 apart by DPP (past the first two as mirrored half and whole rows of 16, whose quads agree by
+// then), rows 16 and 32 apart by the swap of two registers' rows.  No trip through LDS, where a shuffle takes some 100 cycles.
+template <int O> __device__ __forceinline__ float add_across(float v) {
+  const int i = __float_as_int(v);
+  if constexpr (O <= 8) {
+    constexpr int CTRL = O == 1 ? 0xB1 : O == 2 ? 0x4E : O == 4 ? 0x141 : 0x140;
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, i, CTRL, 0xf, 0xf, true));
+  } else if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
+}
+template <int W> __device__ __forceinline__ float lanes_sum(float v) {
+  if (W > 1) v = add_across<1>(v);
+  if (W > 2) v = add_across<2>(v);
+  if (W > 4) v = add_across<4>(v);
+  if (W > 8) v = add_across<8>(v);
+  if (W > 16) v = add_across<16>(v);
+  if (W > 32) v = add_across<32>(v);
+  return v;
+}
+
+// Sums over the L threads that share a row (L <= 64: across the lanes; more, or L = 0 for the whole workgroup: one LDS exchange,
+// two buffers so that one barrier is enough).  The order of the additions depends on L (or the workgroup's size) alone.
 template <int L, int NT> struct RowSum {
-  float2* lds;             // [2][NT / 64]
+  static constexpr int SLOTS = 16;
+  float2* lds;             // [2][SLOTS]
   int turn = 0;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
-    constexpr int W = L < 64 ? L : 64;
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-      a += __shfl_xor(a, o);
-      b += __shfl_xor(b, o);
+  __device__ __forceinline__ explicit RowSum(float2* buf) : lds(buf) {
+    if (L == 0) {          // the places of the waves that there are not
+      if (threadIdx.x < 2 * SLOTS) lds[threadIdx.x] = make_float2(0.f, 0.f);
+      __syncthreads();
     }
-    if (L > 64) {
-      float2* buf = lds + turn * (NT / 64);
+  }
+  template <bool TWO> __device__ __forceinline__ float2 sums(float a, float b) {
+    constexpr int W = L >= 1 && L < 64 ? L : 64, WAVES = L == 0 ? SLOTS : L > 64 ? L / 64 : 1;
+    a = lanes_sum<W>(a);
+    if (TWO) b = lanes_sum<W>(b);
+    if (WAVES > 1) {
+      float2* buf = lds + turn * SLOTS;
       turn ^= 1;
-      const int wave = threadIdx.x >> 6, first = wave & ~(L / 64 - 1);
+      const int wave = threadIdx.x >> 6;
       if ((threadIdx.x & 63) == 0) buf[wave] = make_float2(a, b);
       __syncthreads();
-      a = b = 0.f;
-#pragma unroll
-      for (int i = 0; i < (L >= 64 ? L / 64 : 1); ++i) {
-        const float2 v = buf[first + i];
-        a += v.x;
-        b += v.y;
-      }
+      const float2 v = buf[(L == 0 ? 0 : wave & ~(WAVES - 1)) + (threadIdx.x & (WAVES - 1))];
+      a = lanes_sum<WAVES>(v.x);
+      if (TWO) b = lanes_sum<WAVES>(v.y);
     }
     return make_float2(a, b);
   }
+  __device__ __forceinline__ float2 operator()(float a, float b) { return sums<true>(a, b); }
+  __device__ __forceinline__ float operator()(float a) { return sums<false>(a, 0.f).x; }
 };
 
-// Columns of a thread: K pieces of eight.  EXACT: the row is L * 8 * K wide, every thread owns all of its pieces.  RAGGED (at
+// Columns of a thread: K pieces of eight, l threads a row.  EXACT: the row is l * 8 * K wide, every thread owns all of its pieces.  RAGGED (at
 // least 8 wide): a piece that would reach past the row's end is moved back onto its last eight columns; the columns that it then
 // shares with its neighbour are computed twice and counted once.  So every load is whole and unconditional: a load behind a branch
 // of its own waits for the one before it.  TINY: fewer than eight columns, all of them the first thread's.
 enum { EXACT, RAGGED, TINY };
-template <int L, int K, int MODE> struct Cols {
+template <int K, int MODE> struct Cols {
   int c[K], dup[K];          // first column, columns that another thread owns
   int n;
-  __device__ __forceinline__ Cols(int t, int C) : n(C) {
+  __device__ __forceinline__ Cols(int t, int l, int C) : n(C) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int at = (k * L + t) * 8;
+      const int at = (k * l + t) * 8;
       c[k] = MODE == EXACT ? at : MODE == RAGGED ? min(at, C - 8) : 0;
       dup[k] = MODE == EXACT ? 0 : MODE == RAGGED ? at - c[k] : t == 0 ? 0 : 8;
     }
@@ -78,14 +105,9 @@ template <int L, int K, int MODE> struct Cols {
     if (MODE != TINY) Piece8<T>::store(row + c[k], v);
     else store8(row, n, v);
   }
-  template <typename P> __device__ __forceinline__ void param(const void* p, int k, float (&o)[8], float fill) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fill;
-    if (!p) return;
-    Raw8<P> r;
-    raw(reinterpret_cast<const P*>(p), k, r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = r.get(i);
+  template <typename P> __device__ __forceinline__ void param(const void* p, int k, Raw8<P>& o, float fill) const {
+    o.fill(fill);
+    if (p) raw(reinterpret_cast<const P*>(p), k, o);
   }
 };
 
@@ -118,7 +140,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, fl
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += own.mine(k, i) ? v[k][i] : 0.f;
-    mean = sum(s, 0.f).x / (float)own.n;
+    mean = sum(s) / (float)own.n;
   }
   s = 0.f;
 #pragma unroll
@@ -128,19 +150,20 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[K][8], int kind, fl
       const float d = v[k][i] - mean;
       s = own.mine(k, i) ? fmaf(d, d, s) : s;
     }
-  const float var = sum(s, 0.f).x / (float)own.n;
+  const float var = sum(s) / (float)own.n;
   return make_float2(mean, 1.f / sqrtf(var + eps));
 }
 
+// L threads a row, NT a workgroup; L = 0: the workgroup, of up to NT threads, has one row.
 // FULL: the branch passes a post norm or dropout (with the registers that takes); otherwise gate and scale only.
 template <typename T, typename P, int L, int K, int NT, int MODE, bool FULL>
 __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
-  constexpr int SLOTS = NT / L;
-  __shared__ float2 lds[2 * (NT / 64)];
-  RowSum<L, NT> sum{lds};
+  constexpr int SLOTS = L ? NT / L : 1;
+  __shared__ float2 lds[2 * RowSum<L, NT>::SLOTS];
+  RowSum<L, NT> sum(lds);
   const pnResidualNorm& p = a.p;
-  const int slot = threadIdx.x / L, C = p.cols;
-  const Cols<L, K, MODE> own(threadIdx.x % L, C);
+  const int slot = L ? threadIdx.x / L : 0, t = L ? threadIdx.x % L : threadIdx.x, C = p.cols;
+  const Cols<K, MODE> own(t, L ? L : blockDim.x, C);
   const T* X = reinterpret_cast<const T*>(p.x);
   const T* F = reinterpret_cast<const T*>(p.branch);
   const P* G = reinterpret_cast<const P*>(p.gate);
@@ -148,14 +171,18 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
   T* Y = reinterpret_cast<T*>(a.y);
   PhiloxKey key{};
   if (FULL && p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
-  float nw[K][8], nb[K][8], pw[FULL ? K : 1][8], pb[FULL ? K : 1][8];
+  auto draw = [&](long long row, int c) {                 // rows of whole pieces start at a group of the generator
+    const unsigned long long e = (unsigned long long)row * C + c;
+    return MODE == EXACT || (C & 7) == 0 ? keep8_group(key, e >> 3, p.threshold) : keep8_at(key, e, p.threshold);
+  };
+  Raw8<P> nw[K], nb[K], pw[FULL ? K : 1], pb[FULL ? K : 1];     // as they are stored: bf16 takes half the registers
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    own.template param<P>(p.norm_weight, k, nw[k], 1.f);
-    own.template param<P>(p.norm_bias, k, nb[k], 0.f);
+    own.param(p.norm_weight, k, nw[k], 1.f);
+    own.param(p.norm_bias, k, nb[k], 0.f);
     if (FULL) {
-      own.template param<P>(p.post_weight, k, pw[k], 1.f);
-      own.template param<P>(p.post_bias, k, pb[k], 0.f);
+      own.param(p.post_weight, k, pw[k], 1.f);
+      own.param(p.post_bias, k, pb[k], 0.f);
     }
   }
   // The next row (and its gate) is on its way while this one is worked on; nothing is loaded in between, as waiting for a
@@ -198,14 +225,14 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
       if (FULL) fs = row_stats<K>(f, p.post_kind, p.post_eps, own, sum);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        uint32_t keep = 0xffu;
-        if (FULL && p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + own.c[k], p.threshold);
+        Keep8 keep = keep_all();
+        if (FULL && p.threshold) keep = draw(row, own.c[k]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float u = f[k][i];
           if (FULL) {
-            if (p.post_kind != PN_NORM_NONE) u = fmaf((u - fs.x) * fs.y, pw[k][i], pb[k][i]);
-            u = (keep >> i & 1) ? u * a.keep_scale : 0.f;
+            if (p.post_kind != PN_NORM_NONE) u = fmaf((u - fs.x) * fs.y, pw[k].get(i), pb[k].get(i));
+            u = keep(i) ? u * a.keep_scale : 0.f;
           }
           h[k][i] = (float)(T)fmaf(g[k][i], u, h[k][i]);
         }
@@ -219,11 +246,11 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
       for (int k = 0; k < K; ++k) {
         float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = act_f(fmaf((h[k][i] - hs.x) * hs.y, nw[k][i], nb[k][i]), p.act);
+        for (int i = 0; i < 8; ++i) o[i] = act_f(fmaf((h[k][i] - hs.x) * hs.y, nw[k].get(i), nb[k].get(i)), p.act);
         if (live && own.any(k)) own.store(Y + row * C, k, o);
       }
     }
-    if (a.stats && live && threadIdx.x % L == 0)
+    if (a.stats && live && t == 0)
       *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(hs.x, hs.y, fs.x, fs.y);
   }
 }
@@ -231,17 +258,23 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
 // Backward.  A workgroup owns a chunk of consecutive rows and keeps the column sums (gradients of weights, biases and gate)
 // in registers over the whole chunk; its partial sums go to memory once, and residual_norm_sum_kernel adds the chunks in
 // order: no atomics, the same bits on every run.
+//
+// Rows over 4096 wide with a branch, 16 columns a thread (at eight, 1024 threads leave 128 registers each: the sums alone are 40,
+// and spilled ones wait for the next row's loads): the parameters wait in LDS, and no row is fetched ahead.
+static constexpr __host__ __device__ bool bwd_parks(int L, int K, int NT, bool branch) { return branch && L == 0 && K == 2 && NT == 512; }
 static constexpr int NSUM_NORM = 2, NSUM_ALL = 5;      // weight, bias | post weight, post bias, gate
 
 template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH>
 __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
-  constexpr int SLOTS = NT / L, NS = BRANCH ? NSUM_ALL : NSUM_NORM;
-  __shared__ float2 lds[2 * (NT / 64)];
+  constexpr int SLOTS = L ? NT / L : 1, NS = BRANCH ? NSUM_ALL : NSUM_NORM;
+  constexpr bool PARK = bwd_parks(L, K, NT, BRANCH), AHEAD = !PARK;
+  __shared__ float2 lds[2 * RowSum<L, NT>::SLOTS];
   __shared__ float cols_lds[SLOTS > 1 ? NT * 8 : 1];
-  RowSum<L, NT> sum{lds};
+  extern __shared__ __attribute__((aligned(16))) char parked[];
+  RowSum<L, NT> sum(lds);
   const pnResidualNorm& p = a.p;
-  const int slot = threadIdx.x / L, t = threadIdx.x % L, C = p.cols;
-  const Cols<L, K, MODE> own(t, C);
+  const int threads = L ? L : blockDim.x, slot = L ? threadIdx.x / L : 0, t = L ? threadIdx.x % L : threadIdx.x, C = p.cols;
+  const Cols<K, MODE> own(t, threads, C);
   const int group = blockIdx.x / a.chunks_per_group, chunk = blockIdx.x % a.chunks_per_group;
   const long long g_begin = (long long)group * a.group_rows, g_end = min(g_begin + a.group_rows, (long long)p.rows);
   const long long r_begin = g_begin + (long long)chunk * a.chunk_rows, r_end = min(r_begin + a.chunk_rows, g_end);
@@ -252,25 +285,43 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
   const T* GY = reinterpret_cast<const T*>(a.gy);
   PhiloxKey key{};
   if (BRANCH && p.threshold) key = philox_key(reinterpret_cast<const unsigned long long*>(p.rng), p.call);
+  auto draw = [&](long long row, int c) {                 // rows of whole pieces start at a group of the generator
+    const unsigned long long e = (unsigned long long)row * C + c;
+    return MODE == EXACT || (C & 7) == 0 ? keep8_group(key, e >> 3, p.threshold) : keep8_at(key, e, p.threshold);
+  };
   const float inv_c = 1.f / (float)C;
   const bool relu = p.act == PN_ACT_RELU;
   const P* G = reinterpret_cast<const P*>(p.gate);
-  float acc[NS][K][8], nw[K][8], nb[K][8], pw[BRANCH ? K : 1][8], pb[BRANCH ? K : 1][8];
+  float acc[NS][K][8];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[s][k][i] = 0.f;
+  constexpr int VECS = BRANCH ? 4 : 2, WORDS = sizeof(Raw8<P>) / 16;
+  Raw8<P> held[PARK ? 1 : VECS][K];
+  uint4* park = reinterpret_cast<uint4*>(parked) + t;     // [VECS][K][WORDS][threads]: a thread's own places
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    own.template param<P>(p.norm_weight, k, nw[k], 1.f);
-    own.template param<P>(relu ? p.norm_bias : nullptr, k, nb[k], 0.f);
-    if (BRANCH) {
-      own.template param<P>(p.post_weight, k, pw[k], 1.f);
-      own.template param<P>(p.post_bias, k, pb[k], 0.f);
+  for (int v = 0; v < VECS; ++v)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      Raw8<P> r;
+      own.param(v == 0 ? p.norm_weight : v == 1 ? (relu ? p.norm_bias : nullptr) : v == 2 ? p.post_weight : p.post_bias, k, r, v & 1 ? 0.f : 1.f);
+      if (PARK) {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) park[((v * K + k) * WORDS + j) * threads] = r.words(j);
+      } else {
+        held[PARK ? 0 : v][k] = r;
+      }
     }
-  }
+  auto param = [&](int v, int k) {
+    if (!PARK) return held[PARK ? 0 : v][k];
+    Raw8<P> r;
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) r.set_words(j, park[((v * K + k) * WORDS + j) * threads]);
+    return r;
+  };
 
   Raw8<T> ngh[K], ngy[K], nh[K], nf[K];
   Raw8<P> ng[K];
@@ -300,8 +351,9 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
     }
     if (a.stats) nst = *reinterpret_cast<const float4*>(a.stats + row * 4);
   };
-  if (r_begin < r_end) fetch(r_begin + slot);
+  if (AHEAD && r_begin < r_end) fetch(r_begin + slot);
   for (long long base = r_begin; base < r_end; base += SLOTS) {
+    if (!AHEAD) fetch(base + slot);
     const bool live = base + slot < r_end;
     const long long row = live ? base + slot : r_end - 1;
     Raw8<T> rgh[K], rgy[K], rh[K], rf[K];
@@ -316,7 +368,7 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
     }
     const float4 st = nst;
     gate.next();
-    if (base + SLOTS < r_end) fetch(base + SLOTS + slot);
+    if (AHEAD && base + SLOTS < r_end) fetch(base + SLOTS + slot);
     float dh[K][8];
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -326,12 +378,16 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
       float tw[K][8], hh[K][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
+        const Raw8<P> nw = param(0, k);
+        Raw8<P> nb;
+        if (relu) nb = param(1, k);
+        else nb.fill(0.f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           hh[k][i] = (rh[k].get(i) - st.x) * st.y;
           float g = rgy[k].get(i);
-          if (relu && fmaf(hh[k][i], nw[k][i], nb[k][i]) <= 0.f) g = 0.f;
-          tw[k][i] = g * nw[k][i];
+          if (relu && fmaf(hh[k][i], nw.get(i), nb.get(i)) <= 0.f) g = 0.f;
+          tw[k][i] = g * nw.get(i);
           if (live && own.mine(k, i)) {
             acc[0][k][i] = fmaf(g, hh[k][i], acc[0][k][i]);
             acc[1][k][i] += g;
@@ -366,13 +422,14 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float dg[8];
-        uint32_t keep = 0xffu;
-        if (p.threshold) keep = keep_bits8(key, (unsigned long long)row * C + own.c[k], p.threshold);
+        Keep8 keep = keep_all();
+        if (p.threshold) keep = draw(row, own.c[k]);
+        const Raw8<P> pw = param(2, k), pb = param(3, k);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           fh[k][i] = (rf[k].get(i) - st.z) * st.w;
-          const float u = p.post_kind != PN_NORM_NONE ? fmaf(fh[k][i], pw[k][i], pb[k][i]) : fh[k][i];
-          const bool kept = keep >> i & 1;
+          const float u = p.post_kind != PN_NORM_NONE ? fmaf(fh[k][i], pw.get(i), pb.get(i)) : fh[k][i];
+          const bool kept = keep(i);
           const float sd = p.scale * dh[k][i], v = kept ? u * a.keep_scale : 0.f;
           const float du = kept ? (G ? rg[k].get(i) : 1.f) * sd * a.keep_scale : 0.f;
           dg[i] = sd * v;
@@ -381,7 +438,7 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
             acc[NS - 3][k][i] = fmaf(du, fh[k][i], acc[NS - 3][k][i]);
             acc[NS - 2][k][i] += du;
           }
-          dh[k][i] = p.post_kind != PN_NORM_NONE ? du * pw[k][i] : du;
+          dh[k][i] = p.post_kind != PN_NORM_NONE ? du * pw.get(i) : du;
           if (own.mine(k, i)) {
             s1 += dh[k][i];
             s2 = fmaf(dh[k][i], fh[k][i], s2);
@@ -416,15 +473,15 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
       if (SLOTS > 1) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cols_lds[(slot * 8 + i) * L + t] = own.mine(k, i) ? acc[s][k][i] : 0.f;
+        for (int i = 0; i < 8; ++i) cols_lds[(slot * 8 + i) * threads + t] = own.mine(k, i) ? acc[s][k][i] : 0.f;
         __syncthreads();
         // L * 8 columns, in the order (i, t) in which they lie; the columns that two threads share are the last one's to count
-        for (int q = threadIdx.x; q < L * 8; q += NT) {
-          const int i = q / L, tt = q % L;
-          const Cols<L, K, MODE> theirs(tt, C);
+        for (int q = threadIdx.x; q < threads * 8; q += NT) {
+          const int i = q / threads, tt = q % threads;
+          const Cols<K, MODE> theirs(tt, threads, C);
           float v = 0.f;
 #pragma unroll 8
-          for (int z = 0; z < SLOTS; ++z) v += cols_lds[z * L * 8 + q];
+          for (int z = 0; z < SLOTS; ++z) v += cols_lds[z * threads * 8 + q];
           if (theirs.mine(k, i)) out[s * C + theirs.c[k] + i] = v;
         }
       } else {
@@ -502,22 +559,24 @@ static NormArgs norm_args(const pnResidualNorm* p) {
 
 static constexpr int FWD_WAVES = 8192;                  // 32 a CU: what the forward kernel keeps resident
 
-// Threads per row: the fewest that hold the row at eight elements each, so that a narrow row does not idle a wave.
-#define NORM_BY_COLS(C, GO)                                                      \
+// Threads per row: the fewest that hold the row at eight elements each (K pieces of eight over 8192 columns, and in the backward
+// pass with a branch over 4096), so that a narrow row does not idle a wave; over 1024 columns the workgroup is as large as its row.
+#define NORM_BY_COLS(C, WIDE, GO)                                                \
   (C) <= 64 ? GO(8, 1, 256) : (C) <= 128 ? GO(16, 1, 256) : (C) <= 256 ? GO(32, 1, 256) : (C) <= 512 ? GO(64, 1, 256) \
-  : (C) <= 1024 ? GO(128, 1, 256) : (C) <= 2048 ? GO(256, 1, 256) : (C) <= 4096 ? GO(512, 1, 512)              \
-  : (C) <= 8192 ? GO(1024, 1, 1024) : GO(1024, 2, 1024)
+  : (C) <= 1024 ? GO(128, 1, 256) : (C) <= 4096 ? GO(0, 1, 512) : (C) <= 8192 ? WIDE : GO(0, 2, 1024)
+static int norm_threads(int C, int L, int K, int NT) { return L ? NT : ((C + 8 * K - 1) / (8 * K) + 63) / 64 * 64; }
 
 template <typename T, typename P, int L, int K, int NT> static int norm_fwd(const NormArgs& a, hipStream_t s) {
   const bool full = a.p.post_kind != PN_NORM_NONE || a.p.threshold;
 #define FWD(MODE, L_, K_, NT_)                                                                                                \
   do {                                                                                                                       \
-    const long long need = (a.p.rows + NT_ / L_ - 1) / (NT_ / L_), most = FWD_WAVES / (NT_ / 64);                            \
-    const dim3 grid((unsigned)(need < most ? need : most)), wg(NT_);                                                         \
+    const int threads = norm_threads(a.p.cols, L_, K_, NT_), slots = L_ ? NT_ / (L_ ? L_ : 1) : 1;                                \
+    const long long need = (a.p.rows + slots - 1) / slots, most = FWD_WAVES / (threads / 64);                            \
+    const dim3 grid((unsigned)(need < most ? need : most)), wg(threads);                                                         \
     if (full) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, true>), grid, wg, 0, s, a);              \
     else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, false>), grid, wg, 0, s, a);                  \
   } while (0)
-  if (a.p.cols == L * K * 8) FWD(EXACT, L, K, NT);
+  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT)) * K * 8) FWD(EXACT, L, K, NT);
   else if (a.p.cols >= 8) FWD(RAGGED, L, K, NT);
   else FWD(TINY, 8, 1, 256);
 #undef FWD
@@ -525,10 +584,11 @@ template <typename T, typename P, int L, int K, int NT> static int norm_fwd(cons
   return PN_OK;
 }
 
-// element type and parameter type: fp32 rows go with fp32 parameters, bf16 rows with either
-#define NORM_BY_TYPE(DTYPE, PTYPE, COLS, GO)                                                       \
-  ((DTYPE) == PN_DTYPE_F32 ? (NORM_BY_COLS(COLS, GO##_F32)) : (PTYPE) == PN_DTYPE_F32 ? (NORM_BY_COLS(COLS, GO##_MIX)) \
-                                                                                       : (NORM_BY_COLS(COLS, GO##_BF16)))
+template <typename T, typename P> static int norm_fwd_by_cols(const NormArgs& a, hipStream_t s) {
+#define GO(L, K, NT) norm_fwd<T, P, L, K, NT>(a, s)
+  return NORM_BY_COLS(a.p.cols, GO(0, 1, 1024), GO);
+#undef GO
+}
 
 extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* y, float* stats, void* stream) {
   const int rc = norm_check(p);
@@ -541,28 +601,28 @@ extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* 
   a.y = p->norm_kind == PN_NORM_NONE ? nullptr : y;
   a.stats = stats;
   hipStream_t s = (hipStream_t)stream;
-#define GO_F32(L, K, NT) norm_fwd<float, float, L, K, NT>(a, s)
-#define GO_MIX(L, K, NT) norm_fwd<__bf16, float, L, K, NT>(a, s)
-#define GO_BF16(L, K, NT) norm_fwd<__bf16, __bf16, L, K, NT>(a, s)
-  return NORM_BY_TYPE(p->dtype, p->param_dtype, p->cols, GO);
-#undef GO_F32
-#undef GO_MIX
-#undef GO_BF16
+  // fp32 rows go with fp32 parameters, bf16 rows with either
+  if (p->dtype == PN_DTYPE_F32) return norm_fwd_by_cols<float, float>(a, s);
+  return p->param_dtype == PN_DTYPE_F32 ? norm_fwd_by_cols<__bf16, float>(a, s) : norm_fwd_by_cols<__bf16, __bf16>(a, s);
 }
 
-// Chunks of the backward pass: about NORM_WGS workgroups in all, whole passes over the row slots, none across two gates.
-static constexpr int NORM_WGS = 512;
+// Chunks of the backward pass: about BWD_WAVES waves in all (8 a CU: what the kernel with a branch keeps resident; a workgroup a CU at the least), whole passes
+// over the row slots, none across two gates.
+static constexpr int BWD_WAVES = 2048;
 struct NormChunks { long long groups, group_rows; int per_group, rows, sums; };
 static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
   NormChunks c;
   c.groups = p->gate && p->rows_per_gate > 1 ? p->rows / p->rows_per_gate : 1;
   if (c.groups < 1) c.groups = 1;
   c.group_rows = c.groups > 1 ? p->rows_per_gate : p->rows;
-#define SLOTS_OF(L, K, NT) (NT / L)
-  const int slots = NORM_BY_COLS(p->cols, SLOTS_OF);
+#define SLOTS_OF(L, K, NT) (L ? NT / (L ? L : 1) : 1)
+#define WAVES_OF(L, K, NT) (norm_threads(p->cols, L, K, NT) / 64)
+  const int slots = NORM_BY_COLS(p->cols, 1, SLOTS_OF), waves = NORM_BY_COLS(p->cols, (branch ? WAVES_OF(0, 2, 512) : WAVES_OF(0, 1, 1024)), WAVES_OF);
 #undef SLOTS_OF
+#undef WAVES_OF
   const long long passes = (c.group_rows + slots - 1) / slots;
-  long long want = (NORM_WGS + c.groups - 1) / c.groups;
+  const int wgs = waves > 8 ? 256 : BWD_WAVES / waves;
+  long long want = (wgs + c.groups - 1) / c.groups;
   if (want > passes) want = passes;
   if (want < 1) want = 1;
   const long long per = (passes + want - 1) / want;
@@ -579,18 +639,35 @@ extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
   return (size_t)c.groups * c.per_group * c.sums * p->cols * sizeof(float);
 }
 
-template <typename T, typename P, int L, int K, int NT> static int norm_bwd(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
-#define BWD(MODE, L_, K_, NT_)                                                                                              \
-  do {                                                                                                                     \
-    if (branch) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, P, L_, K_, NT_, MODE, true>), dim3(grid), dim3(NT_), 0, s, a); \
-    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, P, L_, K_, NT_, MODE, false>), dim3(grid), dim3(NT_), 0, s, a);       \
-  } while (0)
-  if (a.p.cols == L * K * 8) BWD(EXACT, L, K, NT);
-  else if (a.p.cols >= 8) BWD(RAGGED, L, K, NT);
-  else BWD(TINY, 8, 1, 256);
-#undef BWD
+template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH> static int norm_bwd(const NormArgs& a, unsigned grid, hipStream_t s) {
+  const int threads = norm_threads(a.p.cols, L, K, NT);
+  size_t lds = 0;
+  if (bwd_parks(L, K, NT, BRANCH)) {
+    lds = (size_t)4 * K * 8 * sizeof(P) * threads;
+    static thread_local int raised_on = -1;                // the device that this thread allowed more than 64 KB on last
+    int d = 0;
+    PN_CHECK_HIP(hipGetDevice(&d));
+    if (d != raised_on) {
+      PN_CHECK_HIP(hipFuncSetAttribute((const void*)residual_norm_bwd_kernel<T, P, L, K, NT, MODE, BRANCH>,
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, 4 * K * 8 * (int)sizeof(P) * NT));
+      raised_on = d;
+    }
+  }
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<T, P, L, K, NT, MODE, BRANCH>), dim3(grid), dim3(threads), lds, s, a);
   PN_CHECK_LAUNCH("residual_norm_bwd_kernel");
   return PN_OK;
+}
+template <typename T, typename P, int L, int K, int NT, bool BRANCH> static int norm_bwd_by_mode(const NormArgs& a, unsigned grid, hipStream_t s) {
+  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT)) * K * 8) return norm_bwd<T, P, L, K, NT, EXACT, BRANCH>(a, grid, s);
+  return a.p.cols >= 8 ? norm_bwd<T, P, L, K, NT, RAGGED, BRANCH>(a, grid, s) : norm_bwd<T, P, 8, 1, 256, TINY, BRANCH>(a, grid, s);
+}
+template <typename T, typename P, bool BRANCH> static int norm_bwd_by_cols(const NormArgs& a, unsigned grid, hipStream_t s) {
+#define GO(L, K, NT) norm_bwd_by_mode<T, P, L, K, NT, BRANCH>(a, grid, s)
+  return NORM_BY_COLS(a.p.cols, GO(0, (BRANCH ? 2 : 1), (BRANCH ? 512 : 1024)), GO);
+#undef GO
+}
+template <typename T, typename P> static int norm_bwd_by_branch(const NormArgs& a, bool branch, unsigned grid, hipStream_t s) {
+  return branch ? norm_bwd_by_cols<T, P, true>(a, grid, s) : norm_bwd_by_cols<T, P, false>(a, grid, s);
 }
 
 extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const float* stats, const void* gh,
@@ -632,13 +709,10 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
     a.chunk_rows = c.rows;
     a.chunks_per_group = c.per_group;
     a.group_rows = c.group_rows;
-#define GO_F32(L, K, NT) norm_bwd<float, float, L, K, NT>(a, branch, (unsigned)chunks, s)
-#define GO_MIX(L, K, NT) norm_bwd<__bf16, float, L, K, NT>(a, branch, (unsigned)chunks, s)
-#define GO_BF16(L, K, NT) norm_bwd<__bf16, __bf16, L, K, NT>(a, branch, (unsigned)chunks, s)
-    const int r = NORM_BY_TYPE(p->dtype, p->param_dtype, p->cols, GO);
-#undef GO_F32
-#undef GO_MIX
-#undef GO_BF16
+    const unsigned grid = (unsigned)chunks;
+    const int r = p->dtype == PN_DTYPE_F32 ? norm_bwd_by_branch<float, float>(a, branch, grid, s)
+                  : p->param_dtype == PN_DTYPE_F32 ? norm_bwd_by_branch<__bf16, float>(a, branch, grid, s)
+                                                   : norm_bwd_by_branch<__bf16, __bf16>(a, branch, grid, s);
     if (r != PN_OK) return r;
   }
   if (dweight || dbias || dpost_weight || dpost_bias || dgate) {

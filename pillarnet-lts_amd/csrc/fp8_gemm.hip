@@ -732,11 +732,14 @@ static int fp8_cus() {                                    // compute units of th
   return cus;
 }
 
-static int fp8_raise_lds(const void* kernel, int bytes, bool* done) {
-  if (bytes > 65536 && !*done) {
-    PN_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    *done = true;
-  }
+// More than 64 KB of LDS has to be allowed for a kernel once on each device; `on`: the one that this thread allowed it on last
+static int fp8_raise_lds(const void* kernel, int bytes, int* on) {
+  int d = 0;
+  if (bytes <= 65536) return PN_OK;
+  PN_CHECK_HIP(hipGetDevice(&d));
+  if (d == *on) return PN_OK;
+  PN_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  *on = d;
   return PN_OK;
 }
 
@@ -749,8 +752,8 @@ static unsigned fp8_grid(Fp8GemmArgs& a, int bm, int bn, int resident) {
 
 template <int BM, int BN, int WM, int WN, int RING, bool WIDE> static int fp8_tile(Fp8GemmArgs a, hipStream_t s) {
   typedef Fp8Tile<BM, BN, WM, WN, RING, WIDE> C;
-  static bool raised = false;
-  const int rc = fp8_raise_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, RING, WIDE>, C::LDS, &raised);
+  static thread_local int raised_on = -1;
+  const int rc = fp8_raise_lds((const void*)fp8_tile_kernel<BM, BN, WM, WN, RING, WIDE>, C::LDS, &raised_on);
   if (rc != PN_OK) return rc;
   const unsigned grid = fp8_grid(a, BM, BN, 163840 / C::LDS < 16 / C::NW ? 163840 / C::LDS : 16 / C::NW);
   hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WM, WN, RING, WIDE>), dim3(grid), dim3(C::NW * 64), C::LDS, s, a);
@@ -760,8 +763,8 @@ template <int BM, int BN, int WM, int WN, int RING, bool WIDE> static int fp8_ti
 
 template <bool WIDE> static int fp8_pair(Fp8GemmArgs a, hipStream_t s) {
   typedef Fp8Pair<WIDE> C;
-  static bool raised = false;
-  const int rc = fp8_raise_lds((const void*)fp8_pair_kernel<WIDE>, C::LDS, &raised);
+  static thread_local int raised_on = -1;
+  const int rc = fp8_raise_lds((const void*)fp8_pair_kernel<WIDE>, C::LDS, &raised_on);
   if (rc != PN_OK) return rc;
   const unsigned grid = fp8_grid(a, C::BM, C::BN, 1);
   hipLaunchKernelGGL(fp8_pair_kernel<WIDE>, dim3(grid), dim3(512), C::LDS, s, a);
