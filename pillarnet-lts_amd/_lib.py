@@ -145,9 +145,10 @@ SIGNATURES = {
     "pn_act_dropout_backward": (c_int, [c_int, c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong, c_int,
                                         c_uint32, c_void_p, c_uint32, c_void_p, c_void_p]),
     "pn_dropout_draw": (c_int, [c_void_p, c_void_p, c_void_p]),
-    "pn_residual_norm_forward": (c_int, [POINTER(pnResidualNorm), c_void_p, c_void_p, c_void_p, c_void_p]),
-    "pn_residual_norm_workspace_bytes": (c_size_t, [POINTER(pnResidualNorm)]),
-    "pn_residual_norm_backward": (c_int, [POINTER(pnResidualNorm)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
+    # const pnResidualNorm* as an address: byref(pnResidualNorm(...)) or the packed bytes of one, a tenth of the host time
+    "pn_residual_norm_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pn_residual_norm_workspace_bytes": (c_size_t, [c_void_p]),
+    "pn_residual_norm_backward": (c_int, [c_void_p] * 13 + [c_size_t, c_void_p]),
     "pn_fp8_operand_bytes": (c_size_t, [c_longlong, c_longlong]),
     "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "pn_fp8_gemm": (c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong,

@@ -9,8 +9,8 @@ with Dropout of roi_head_template.py:23-39, the mixers of mlp_layers.py:24-117) 
 All take fp32 or bf16 tensors on the GPU, run on the current stream of the tensors' device, allocate through torch's
 caching allocator only and wait for nothing, so they can be captured into a HIP graph.  A graph that holds a backward pass
 is captured while no eager autograd graph over the same leaves is alive (torch's own rule for captured backward passes)."""
+import struct
 from collections import namedtuple
-from ctypes import byref
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -197,33 +197,48 @@ class Norm(namedtuple("Norm", "kind weight bias eps")):
 _JoinCfg = namedtuple("_JoinCfg", "post norm post_eps norm_eps scale threshold call act rows_per_gate")
 
 
-def _join_struct(cfg, x, f, gate, pw, pb, w, b, rng):
-    """(struct, row views that must outlive the launch)."""
-    xv, fv = _rows(x), None if f is None else _rows(f)
-    params = [t for t in (gate, pw, pb, w, b) if t is not None]
-    s = _lib.pnResidualNorm(
-        _DTYPES[x.dtype], _DTYPES[params[0].dtype] if params else _lib.PN_DTYPE_F32, cfg.post, cfg.norm, cfg.act, x.shape[-1],
-        xv.shape[0], cfg.rows_per_gate, xv.stride(0), 0 if fv is None else fv.stride(0), cfg.scale, cfg.post_eps, cfg.norm_eps,
-        cfg.threshold, cfg.call, _ptr(rng), xv.data_ptr(), _ptr(fv), _ptr(gate), _ptr(pw), _ptr(pb), _ptr(w), _ptr(b))
-    return s, (xv, fv)
+_JOIN = struct.Struct("@6i4q3f2I8Q")                     # pnResidualNorm, fields in order
 
 
-def _join_forward(cfg, x, f, gate, pw, pb, w, b, rng, want_stats):
-    s, keep = _join_struct(cfg, x, f, gate, pw, pb, w, b, rng)
+def _strided(x):
+    """(x or a copy of it, its row stride) as _rows, without a view where x is contiguous."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
+    x = _rows(x)
+    return x, x.stride(0)
+
+
+def _join_struct(cfg, rows, x, f, gate, pw, pb, w, b, rng):
+    """(packed struct, tensors that must outlive the launch)."""
+    x, ldx = _strided(x)
+    f, ldf = (None, 0) if f is None else _strided(f)
+    param = gate if gate is not None else pw if pw is not None else pb if pb is not None else w if w is not None else b
+    s = _JOIN.pack(
+        _DTYPES[x.dtype], _lib.PN_DTYPE_F32 if param is None else _DTYPES[param.dtype], cfg.post, cfg.norm, cfg.act, x.shape[-1],
+        rows, cfg.rows_per_gate, ldx, ldf, cfg.scale, cfg.post_eps, cfg.norm_eps, cfg.threshold, cfg.call,
+        0 if rng is None else rng.data_ptr(), x.data_ptr(), 0 if f is None else f.data_ptr(), 0 if gate is None else gate.data_ptr(),
+        0 if pw is None else pw.data_ptr(), 0 if pb is None else pb.data_ptr(), 0 if w is None else w.data_ptr(),
+        0 if b is None else b.data_ptr())
+    return s, (x, f)
+
+
+def _join_forward(cfg, rows, x, f, gate, pw, pb, w, b, rng, want_stats):
+    s, keep = _join_struct(cfg, rows, x, f, gate, pw, pb, w, b, rng)
     h = torch.empty_like(x, memory_format=torch.contiguous_format) if f is not None else None
     y = torch.empty_like(x, memory_format=torch.contiguous_format) if cfg.norm else None
-    stats = torch.empty((s.rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    if s.rows:                          # (an empty tensor has no address to tell the branch by)
-        _call("pn_residual_norm_forward", x.device, byref(s), _ptr(h), _ptr(y), _ptr(stats))
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
+    if rows:                            # (an empty tensor has no address to tell the branch by)
+        _call("pn_residual_norm_forward", x.device, s, None if h is None else h.data_ptr(), None if y is None else y.data_ptr(),
+              None if stats is None else stats.data_ptr())
     return h, y, stats
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, cfg, rng, x, f, gate, pw, pb, w, b):
-        h, y, stats = _join_forward(cfg, x, f, gate, pw, pb, w, b, rng, True)
+    def forward(ctx, cfg, rows, rng, x, f, gate, pw, pb, w, b):
+        h, y, stats = _join_forward(cfg, rows, x, f, gate, pw, pb, w, b, rng, True)
         reads_f = f is not None and (gate is not None or cfg.post or cfg.threshold or cfg.scale != 1.0)
-        ctx.cfg, ctx.has_branch, ctx.reads_f = cfg, f is not None, reads_f
+        ctx.cfg, ctx.rows, ctx.has_branch, ctx.reads_f = cfg, rows, f is not None, reads_f
         # the norm's backward reads the rows it normalised; x itself is needed only where it is those rows
         ctx.save_for_backward(rng, h if f is not None else x, f if reads_f else None, gate, pw, pb, w, b, stats)
         ctx.set_materialize_grads(False)
@@ -231,39 +246,39 @@ class _ResidualNorm(torch.autograd.Function):
 
     @_backward
     def backward(ctx, *grads):
-        cfg = ctx.cfg
+        cfg, rows, has_branch, reads_f = ctx.cfg, ctx.rows, ctx.has_branch, ctx.reads_f
         rng, h, f, gate, pw, pb, w, b, stats = ctx.saved_tensors
-        if ctx.has_branch:
+        if has_branch:
             gh, gy = grads if cfg.norm else (grads[0], None)
         else:
             gh, gy = None, grads[0]
         if gh is None and gy is None:
-            return (None,) * 9
-        dev, shape, dt = h.device, h.shape, h.dtype
-        need = ctx.needs_input_grad[2:]
-        # without reads_f the struct still needs a branch pointer to say that h is a stored tensor: h stands in, unread
-        s, keep = _join_struct(cfg, h, (f if ctx.reads_f else h) if ctx.has_branch else None, gate, pw, pb, w, b, rng)
+            return (None,) * 10
+        need_x, need_f, *need = ctx.needs_input_grad[3:]
         gh = None if gh is None else gh.contiguous()
         gy = None if gy is None else gy.contiguous()
-        if gy is None and ctx.has_branch and not ctx.reads_f:
-            return None, None, gh if need[0] else None, gh if need[1] else None, None, None, None, None, None
-        dx = torch.empty(shape, dtype=dt, device=dev) if need[0] or (need[1] and not ctx.reads_f) else None
-        df = torch.empty(shape, dtype=dt, device=dev) if need[1] and ctx.reads_f else None
-        sums = [torch.empty_like(t, memory_format=torch.contiguous_format) if n and t is not None else None
-                for t, n in zip((w, b, pw, pb, gate), (need[5], need[6], need[3], need[4], need[2]))]
-        if s.rows == 0:
+        if gy is None and has_branch and not reads_f:
+            return None, None, None, gh if need_x else None, gh if need_f else None, None, None, None, None, None
+        contiguous = torch.contiguous_format
+        dx = torch.empty_like(h, memory_format=contiguous) if need_x or (need_f and not reads_f) else None
+        df = torch.empty_like(h, memory_format=contiguous) if need_f and reads_f else None
+        sums = [torch.empty_like(t, memory_format=contiguous) if n and t is not None else None for t, n in zip((gate, pw, pb, w, b), need)]
+        if rows == 0:
             for t in sums:
                 if t is not None:
                     t.zero_()
         else:
-            size = _lib.lib().pn_residual_norm_workspace_bytes(byref(s))
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            _call("pn_residual_norm_backward", dev, byref(s), _ptr(h), _ptr(stats), _ptr(gh), _ptr(gy), _ptr(dx), _ptr(df),
-                  *[_ptr(t) for t in sums], ws.data_ptr(), size)
-        dw, db, dpw, dpb, dgate = sums
-        if ctx.has_branch and not ctx.reads_f:
-            df = dx if need[1] else None
-        return None, None, dx if need[0] else None, df, dgate, dpw, dpb, dw, db
+            # without reads_f the struct still needs a branch pointer to say that h is a stored tensor: h stands in, unread
+            s, keep = _join_struct(cfg, rows, h, (f if reads_f else h) if has_branch else None, gate, pw, pb, w, b, rng)
+            size = _lib.lib().pn_residual_norm_workspace_bytes(s)
+            ws = torch.empty(size, dtype=torch.uint8, device=h.device)
+            dgate, dpw, dpb, dw, db = [None if t is None else t.data_ptr() for t in sums]
+            _call("pn_residual_norm_backward", h.device, s, h.data_ptr(), stats.data_ptr(), None if gh is None else gh.data_ptr(),
+                  None if gy is None else gy.data_ptr(), None if dx is None else dx.data_ptr(), None if df is None else df.data_ptr(),
+                  dw, db, dpw, dpb, dgate, ws.data_ptr(), size)
+        if has_branch and not reads_f:
+            df = dx if need_f else None
+        return (None, None, None, dx if need_x else None, df, *sums)
 
 
 def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=None, dropout=None, act="none"):
@@ -324,8 +339,8 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
                    post_norm.eps if post_norm is not None else 0.0, norm.eps if norm is not None else 0.0, float(scale), threshold, call,
                    _lib.PN_ACT[act], rows_per_gate)
     if _wants_grad(x, branch, gate, pw, pb, w, b):
-        return _ResidualNorm.apply(cfg, rng, x, branch, gate, pw, pb, w, b)
-    h, y, _ = _join_forward(cfg, x, branch, gate, pw, pb, w, b, rng, False)
+        return _ResidualNorm.apply(cfg, R, rng, x, branch, gate, pw, pb, w, b)
+    h, y, _ = _join_forward(cfg, R, x, branch, gate, pw, pb, w, b, rng, False)
     return (h, y) if h is not None and y is not None else h if y is None else y
 
 
