@@ -249,13 +249,13 @@ def params_version(module):
 
 
 class PlanCache:
-    """plans keyed by module, invalidated when any parameter / buffer is modified in place."""
+    """plans keyed by module, invalidated when any parameter / buffer is modified in place (`version`: what is compared)."""
 
-    def __init__(self):
-        self._d = {}
+    def __init__(self, version=params_version):
+        self._d, self._version = {}, version
 
     def get(self, module, builder):
-        v = params_version(module)
+        v = self._version(module)
         hit = self._d.get(id(module))
         # id() values are recycled once a module is collected: the entry must belong to THIS module
         if hit is None or hit[0] != v or hit[2]() is not module:

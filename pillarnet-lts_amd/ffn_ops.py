@@ -426,7 +426,7 @@ class Fp8Weight:
     @classmethod
     def from_blocks(cls, values, exponents, bias=None):
         """values: float8_e4m3fn [N, K]; exponents: integers [ceil(N / 128), ceil(K / 128)], the weight of tile (i, j) being
-        values * 2^exponents[i, j] (-126 to 127)."""
+        values * 2^exponents[i, j] (-126 to 127; what lies beyond is taken to the nearer end)."""
         _require(values.device.type == "cuda" and exponents.device == values.device,
                  "Fp8Weight: tensors must live on the GPU (no CPU fallback)")
         _require(values.dtype == torch.float8_e4m3fn and values.dim() == 2 and min(values.shape) >= 1,
@@ -467,8 +467,8 @@ def fp8_linear(x, weight, act="none", out_dtype=None):
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        need_x, need_w, _ = ctx.needs_input_grad
+    def forward(ctx, x, weight, bias, grads):
+        need_x, need_w = grads and x.requires_grad, grads and weight.requires_grad
         L, dev = _lib.lib(), x.device
         v, wv = _rows(x), _rows(weight)
         (M, K), N = v.shape, wv.shape[0]
@@ -476,7 +476,8 @@ class _Fp8Linear(torch.autograd.Function):
         saved = None
         if M:
             # the transposed operands that the backward pass reads: a byte an element; x and the weight are not kept
-            saved = torch.empty(L.pn_fp8_train_saved_bytes(M, N, K), dtype=torch.uint8, device=dev)
+            # (one byte stands in where neither gradient is wanted)
+            saved = torch.empty(L.pn_fp8_train_saved_bytes(M, N, K) if need_x or need_w else 1, dtype=torch.uint8, device=dev)
             ws = torch.empty(L.pn_fp8_train_workspace_bytes(M, N, K, 0), dtype=torch.uint8, device=dev)
             b = None if bias is None else bias.contiguous()
             _call("pn_fp8_train_forward", dev, _DTYPES[x.dtype], v.data_ptr(), M, v.stride(0), _DTYPES[weight.dtype], wv.data_ptr(), N, K,
@@ -488,7 +489,7 @@ class _Fp8Linear(torch.autograd.Function):
 
     @_backward
     def backward(ctx, g):
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         (saved,) = ctx.saved_tensors
         shape, w_dtype, b_dtype = ctx.meta
         dev, gv = g.device, _rows(g)
@@ -497,11 +498,11 @@ class _Fp8Linear(torch.autograd.Function):
         dw = torch.empty((N, K), dtype=w_dtype, device=dev) if need_w else None
         db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
         if M == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None
         ws = torch.empty(_lib.lib().pn_fp8_train_workspace_bytes(M, N, K, 1), dtype=torch.uint8, device=dev)
         _call("pn_fp8_train_backward", dev, _DTYPES[g.dtype], gv.data_ptr(), M, gv.stride(0), _DTYPES[w_dtype], N, K, saved.data_ptr(),
               _ptr(dx), _ptr(dw), _ptr(db), _DTYPES[b_dtype] if need_b else 0, ws.data_ptr())
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 def fp8_linear_train(x, weight, bias=None):
@@ -514,4 +515,4 @@ def fp8_linear_train(x, weight, bias=None):
              f"fp8_linear_train: x {tuple(x.shape)} for a weight {tuple(weight.shape)}")
     _require(bias is None or bias.shape == (weight.shape[0],), f"fp8_linear_train: the bias has shape [{weight.shape[0]}]")
     _require(max(x.numel() // x.shape[-1], *weight.shape) <= 1 << 22, "fp8_linear_train: more than 2^22 rows or features")
-    return _Fp8Linear.apply(x, weight, bias)
+    return _Fp8Linear.apply(x, weight, bias, torch.is_grad_enabled())

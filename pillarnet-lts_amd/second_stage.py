@@ -122,7 +122,9 @@ def roi_grid_pool_torch(rois, feature_map, grid, cell_size, x_min, y_min):
     return out.view(B, R, grid * grid, C), pts
 
 
-FP8_PLANS = dense_hip.PlanCache()      # weights laid out for fp8 products (PLANS holds the same modules' fp32 plans)
+# weights laid out for fp8 products (PLANS holds the same modules' fp32 plans), anew where a weight was written in place or its
+# storage replaced
+FP8_PLANS = dense_hip.PlanCache(lambda m: (dense_hip.params_version(m), tuple(p.data_ptr() for p in m.parameters())))
 
 
 class FoldedMLP:
@@ -602,6 +604,7 @@ def _fc_stack(cfg_list, cin, cout, dp_ratio, conv=True):
 class RoIHeadTemplate(nn.Module):
     """roi_head_template.py:13-219: what every RoI head shares -- the proposal sampler, the RoI-frame target
     encoding, class / box / IoU losses and the decoding of residuals back into boxes."""
+    HAS_FUSED = False                      # whether the head's forward pass honours use_fused
 
     def __init__(self, num_class, model_cfg):
         super().__init__()
@@ -614,7 +617,10 @@ class RoIHeadTemplate(nn.Module):
         """fused_ops: the head's norms, residuals, activations and dropouts run on ffn_ops (the dropouts then draw from a
         counter-based generator of their own instead of torch's: other masks, the same distribution).  fp8 (implies fused_ops):
         its Linear / 1x1 layers too, as products in e4m3 with block scales, forward and backward.  dropout_seed: the
-        generator's seed (default torch.initial_seed(); data-parallel ranks add their rank)."""
+        generator's seed (default torch.initial_seed(); data-parallel ranks add their rank); its offset starts at 0 and is no part
+        of the state dict, so a resumed run takes another seed."""
+        if (fused_ops or fp8) and not self.HAS_FUSED:
+            raise _lib.PillarnetHipError(f"{type(self).__name__} has no fused path")
         self.fused_ops, self.fp8, self.dropout_seed, self._dropout_state = bool(fused_ops or fp8), bool(fp8), dropout_seed, None
         return self
 
@@ -767,6 +773,7 @@ class RoIHeadTemplate(nn.Module):
 @ROI_HEAD.register_module
 class RoIMIXHead(RoIHeadTemplate):
     """roi_mix_head.py:17-122 on the shared template (roi_head_template.py)."""
+    HAS_FUSED = True
 
     def __init__(self, in_channels=None, model_cfg=None, num_class=1, code_size=7, add_box_param=False, test_cfg=None,
                  mixer_type=None, num_patches=49, fused_ops=False, fp8=False, dropout_seed=None, **kwargs):
@@ -879,6 +886,7 @@ class FFN(nn.Module):
 class RoIFFNHead(RoIHeadTemplate):
     """roi_ffn_head.py:10-140: a transformer-style feed-forward block + LayerNorm over the flattened RoI feature,
     then Linear + LayerNorm + ReLU towers for class, box residual and (num_iou_fcs > 0) an IoU estimate."""
+    HAS_FUSED = True
 
     def __init__(self, model_cfg, num_cls_fcs=1, num_reg_fcs=1, num_iou_fcs=1, feedforward_channels=2048,
                  content_dim=256, num_ffn_fcs=2, dropout=0.0, ffn_act_cfg=dict(type="ReLU", inplace=True),

@@ -142,3 +142,12 @@ def test_struct_layout_matches_header():
     assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers
     values = [3, 1, 2, 1, 0, 64, 10, 5, 64, 64, 0.5, 1e-5, 1e-6, 77, 9, *range(1 << 33, (1 << 33) + 8)]
     assert ffn_ops._JOIN.pack(*values) == bytes(_lib.pnResidualNorm(*values))           # what ffn_ops hands over
+
+
+def test_a_head_without_a_fused_path_says_so():
+    from pillarnet_lts_amd import legacy
+    head = legacy.RoIHead(16, dict(SHARED_FC=[8], CLS_FC=[8], REG_FC=[8], DP_RATIO=0.0))
+    for kw in (dict(), dict(fused_ops=False, fp8=True)):
+        with pytest.raises(PillarnetHipError, match="RoIHead has no fused path"):
+            head.use_fused(**kw)
+    assert head.use_fused(False) is head and not head.fused_ops

@@ -1,11 +1,11 @@
 """Feed-forward operators on the GPU against oracle/ffn_oracle.py (64 bits).
 
 Tolerances are counted in half steps of the types, u = eps / 2 relative to the value a rounding acts on:
-  dropout      two fp32 roundings (scale, product) and the output's; GELU adds an absolute error of |x| * 4u (erff within
-               2 ulp = 4u of a value below 1, its argument's two roundings times max |t erf'(t)| = 0.49, the sum's rounding,
-               all halved by the factor 0.5: 3.5u).
-  norms        a sum over a row takes at most 8 K serial, 6 shuffle and 16 cross-wave additions (K <= 2): 38 roundings, and as
-               many for the second statistic, so every normalised value is within 96u of r * (|t| + mean |t|) + |n|; the
+  dropout      two fp32 roundings (scale, product) and the output's; GELU adds an absolute error of |x| * 4u (its tail q <= 1/2
+               from the fitted t P(t) e^(-z^2): t is within 3u, which the product's sensitivity of at most 2.26 to it takes to
+               6.8u of q, 3.4u |x|, and the last product's rounding).
+  norms        a sum over a row takes at most 8 K serial, 6 additions across lanes and 4 across waves (K <= 2): 26 roundings, and
+               as many for the second statistic, so every normalised value is within 96u of r * (|t| + mean |t|) + |n|; the
                gradients add two more such sums.
   column sums  R rows (and chunks) are added in fp32: (R + 64)u of the sum of magnitudes, plus what the summands are off.
   fp8          bytes and scales are exact.  Products: whole numbers below 2^24 are exact; an fp32 result may be off by one step
@@ -291,6 +291,30 @@ def _join_run(cuda, dtype, pdtype, B, T, C, post, norm, gate, p, branch, act="no
 @pytest.mark.parametrize("C", [1, 7, 8, 33, 64, 65, 128, 200, 256, 500, 512, 1000, 1024, 2048, 2050, 4096, 5001, 8192, 16384])
 def test_residual_norm_widths(cuda, dtype, C):
     _join_run(cuda, dtype, dtype, 2, 37, C, "rms", "layer", "channel", 0.1, True)
+
+
+@pytest.mark.parametrize("C", [1031, 1536, 4100, 5001, 8192, 9000])
+def test_residual_norm_wide_rows_with_wider_parameters(cuda, C):
+    """bf16 rows, fp32 parameters, workgroups of the row's size: odd and whole widths on either side of their limits."""
+    _join_run(cuda, torch.bfloat16, torch.float32, 2, 19, C, "layer", "rms", "sample", 0.2, True, act="relu")
+    _join_run(cuda, torch.bfloat16, torch.float32, 1, 5, C, None, "layer", None, 0.0, False, act="relu")
+
+
+def test_residual_norm_beyond_32_bit_offsets(cuda):
+    """4.3e9 elements: the last rows are those of a call of their own (a mask by element index among them)."""
+    C, R = 4104, 1047000
+    assert R * C > 1 << 32
+    x = torch.zeros((R, C), dtype=torch.bfloat16, device=cuda)
+    tail = torch.randn(8, C, device=cuda).bfloat16()
+    x[-8:] = tail
+    w, rng = torch.randn(C, device=cuda).bfloat16(), rng_of(3, 4, cuda)
+    h, y = ffn_ops.residual_norm(x, x, scale=0.5, norm=ffn_ops.Norm("layer", w), dropout=(0.25, rng, 2))
+    keep = torch.from_numpy(fo.drop_scale(0.25, 3, 4, 2, (8, C), start=(R - 8) * C)).to(cuda).float() * 0.5
+    hw, yw = ffn_ops.residual_norm(tail, tail, gate=keep.bfloat16(), norm=ffn_ops.Norm("layer", w))
+    within(h[-8:], d(tail) * (1 + d(keep)), 1.01 * U[torch.bfloat16] * np.abs(d(tail)) * (1 + d(keep)), "h")
+    # 0.5 / 0.75 rounded to bf16 as a gate, h rounded on either side, y rounded on either side: five half steps, one for the statistics
+    assert (y[-8:].float() - yw.float()).norm() <= 6 * U[torch.bfloat16] * yw.float().norm()
+    assert (h[: 8] == 0).all() and (y[: 8] == 0).all()
 
 
 @BOTH
@@ -586,6 +610,40 @@ def test_fp8_partial_gradients_and_refusals(cuda):
                  lambda: ffn_ops.Fp8Weight.from_blocks(w, torch.zeros(1, 1, device=cuda, dtype=torch.int32))):
         with pytest.raises(PillarnetHipError):
             call()
+
+
+def test_fp8_beyond_32_bit_offsets(cuda):
+    """x and out of 4.3e9 elements each: the last rows are those of a call of their own (the same sums, other kernels: whole numbers)."""
+    M, K, N = (1 << 21) + 5, 2056, 24
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device=cuda)
+    x[-300:] = torch.randint(-3, 4, (300, K), device=cuda).bfloat16()
+    w = torch.randint(-3, 4, (N, K), device=cuda).float()
+    y = ffn_ops.fp8_linear(x, ffn_ops.Fp8Weight(w), out_dtype=torch.float32)
+    assert torch.equal(y[-300:], x[-300:].float() @ w.t()) and (y[: 300] == 0).all()
+    q, qt = ffn_ops.fp8_quantize(x, transposed=True)
+    assert torch.equal(qt.values()[:, -300:], x[-300:].float().t())
+    del x, q, qt, y
+    K, N = 128, 2056
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device=cuda)
+    x[-300:] = torch.randint(-3, 4, (300, K), device=cuda).bfloat16()
+    w = torch.randint(-3, 4, (N, K), device=cuda).float()
+    y = ffn_ops.fp8_linear(x, ffn_ops.Fp8Weight(w))
+    assert torch.equal(y[-300:], (x[-300:].float() @ w.t()).bfloat16()) and (y[: 300] == 0).all()
+
+
+def test_second_derivatives_are_refused(cuda):
+    """create_graph gives the first gradient; asking for the gradient of it raises instead of giving zeros."""
+    x = torch.randn(6, 64, device=cuda, requires_grad=True)
+    w = torch.randn(32, 64, device=cuda, requires_grad=True)
+    for call in (lambda: ffn_ops.act_dropout(x, 0.0, act="gelu"), lambda: ffn_ops.residual_norm(x, norm=ffn_ops.Norm("rms")),
+                 lambda: ffn_ops.fp8_linear_train(x, w)):
+        (g,) = torch.autograd.grad(call().square().sum(), x, create_graph=True)
+        (want,) = torch.autograd.grad(call().square().sum(), x)
+        assert torch.equal(g, want)
+        with pytest.raises(RuntimeError):                       # torch finds no way from g to x
+            torch.autograd.grad(g.sum(), x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
 
 
 # ---- together ----------------------------------------------------------------------------------------------------------
