@@ -502,7 +502,8 @@ int pn_dropout_draw(void* state, void* used, pnStream stream);
 /* Residual join with the norms around it:
  *   u = post(branch)   v = dropout(u)   h = round(x + scale * gate * v)   y = act(norm(h))
  * post: none / layer / rms; norm: none / layer / rms / affine (weight and bias only); a NULL weight is 1, a NULL bias 0.
- * gate: NULL or [rows / rows_per_gate, cols] (rows_per_gate == rows: one vector for all rows; 1: a gate for each row).
+ * gate: NULL or [rows / rows_per_gate, cols] (rows_per_gate == rows: one vector for all rows; 1: a gate for each row; otherwise up to
+ * 2^23 gates).
  * branch == NULL: h is x and is not written.  Weights, biases and gate have type param_dtype (fp32 where the rows are fp32). */
 #define PN_NORM_NONE 0
 #define PN_NORM_LAYER 1

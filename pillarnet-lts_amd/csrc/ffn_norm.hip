@@ -494,22 +494,26 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
 
 // out[v][c] = sum over the chunks of vector v: blockIdx.x picks the vector (weight, bias, post weight, post bias, then
 // one gate row each), blockIdx.y its 64 columns; 16 chunk lanes.
+// PARTS: blockIdx.z picks a part of SUM_PART chunks and the sums stay fp32 chunk sums, [part][sums][cols] at out[0]: with a chunk for
+// each of many gates a single pass over them would be a few workgroups' (100000 gates of two rows, 256 columns: 10 ms).
+static constexpr int SUM_PART = 256;
 struct SumArgs {
-  const float* partial;
+  const float *partial, *gate_partial;      // chunk sums; those of the gates' rows
   void* out[NSUM_ALL];
   int cols, sums, chunks, chunks_per_group, out_bf16;
 };
-__global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
+template <bool PARTS> __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
   __shared__ float lds[16][64];
-  const int v = blockIdx.x, s = v < NSUM_ALL - 1 ? v : NSUM_ALL - 1, group = v - s;
-  void* out = a.out[s];
+  const int v = blockIdx.x, s = v < NSUM_ALL - 1 ? v : NSUM_ALL - 1, group = PARTS ? blockIdx.z : v - s;
+  void* out = a.out[PARTS ? 0 : s];
   if (!out) return;                                                        // the same for the whole workgroup
-  const bool per_group = s == NSUM_ALL - 1;
-  const int first = per_group ? group * a.chunks_per_group : 0, count = per_group ? a.chunks_per_group : a.chunks;
+  const bool gate = s == NSUM_ALL - 1;
+  const int first = PARTS ? group * SUM_PART : gate ? group * a.chunks_per_group : 0;
+  const int count = PARTS ? min(SUM_PART, a.chunks - first) : gate ? a.chunks_per_group : a.chunks;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 64 + lane;
   float acc = 0.f;
   if (c < a.cols) {
-    const float* p = a.partial + ((size_t)first * a.sums + s) * a.cols + c;
+    const float* p = (gate ? a.gate_partial : a.partial) + ((size_t)first * a.sums + s) * a.cols + c;
 #pragma unroll 8
     for (int i = w; i < count; i += 16) acc += p[(size_t)i * a.sums * a.cols];
   }
@@ -519,11 +523,13 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t += lds[i][lane];
-    const size_t at = (size_t)group * a.cols + c;
-    if (a.out_bf16) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
+    const size_t at = PARTS ? ((size_t)group * a.sums + s) * a.cols + c : (size_t)group * a.cols + c;
+    if (!PARTS && a.out_bf16) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
     else reinterpret_cast<float*>(out)[at] = t;
   }
 }
+// parts that the chunks are added in before the last sum (0: one pass)
+static long long sum_parts(long long chunks) { return chunks > 4 * SUM_PART ? (chunks + SUM_PART - 1) / SUM_PART : 0; }
 
 static int norm_check(const pnResidualNorm* p) {
   PN_CHECK_ARG(p, "residual_norm: null pointer");
@@ -546,6 +552,7 @@ static int norm_check(const pnResidualNorm* p) {
                "residual_norm: x missing or a row stride below the row length");
   PN_CHECK_ARG(!p->gate || (p->rows_per_gate >= 1 && p->rows % p->rows_per_gate == 0),
                "residual_norm: %lld rows do not divide into gates of %lld rows", (long long)p->rows, (long long)p->rows_per_gate);
+  PN_CHECK_ARG(!p->gate || p->rows_per_gate == 1 || p->rows / p->rows_per_gate <= 1 << 23, "residual_norm: more than 2^23 gates of several rows");
   return PN_OK;
 }
 
@@ -636,7 +643,8 @@ static bool norm_reads_branch(const pnResidualNorm* p) { return p->branch && (p-
 extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
   if (norm_check(p) != PN_OK) return 0;
   const NormChunks c = norm_chunks(p, norm_reads_branch(p));
-  return (size_t)c.groups * c.per_group * c.sums * p->cols * sizeof(float);
+  const long long chunks = c.groups * c.per_group;
+  return (size_t)(chunks + sum_parts(chunks)) * c.sums * p->cols * sizeof(float);
 }
 
 template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH> static int norm_bwd(const NormArgs& a, unsigned grid, hipStream_t s) {
@@ -686,11 +694,10 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
   PN_CHECK_ARG(branch || !dbranch, "residual_norm: the branch's gradient is dx itself");
   PN_CHECK_ARG(!dgate || p->gate, "residual_norm: gradient of a gate that there is not");
   const NormChunks c = norm_chunks(p, branch);
-  PN_CHECK_ARG(c.groups * c.per_group < (1ll << 31), "residual_norm: too many gates");
   hipStream_t s = (hipStream_t)stream;
   const long long chunks = p->rows ? c.groups * c.per_group : 0;
   if (chunks) {
-    if (ws_bytes < (size_t)chunks * c.sums * p->cols * sizeof(float) || !ws) {
+    if (ws_bytes < (size_t)(chunks + sum_parts(chunks)) * c.sums * p->cols * sizeof(float) || !ws) {
       pn_set_error("residual_norm: workspace of %zu bytes is too small", ws_bytes);
       return PN_ENOSPC;
     }
@@ -718,9 +725,20 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
   if (dweight || dbias || dpost_weight || dpost_bias || dgate) {
     const long long vecs = dgate ? NSUM_ALL - 1 + c.groups : (dpost_weight || dpost_bias) ? NSUM_ALL - 1 : NSUM_NORM;
     if (!p->rows) dgate = nullptr;                 // no rows, no gates
-    SumArgs q = {(const float*)ws, {dweight, dbias, dpost_weight, dpost_bias, dgate}, p->cols, c.sums, (int)chunks,
+    SumArgs q = {(const float*)ws, (const float*)ws, {dweight, dbias, dpost_weight, dpost_bias, dgate}, p->cols, c.sums, (int)chunks,
                  chunks ? c.per_group : 0, p->param_dtype == PN_DTYPE_BF16};
-    hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((unsigned)vecs, (p->cols + 63) / 64), dim3(1024), 0, s, q);
+    const unsigned col_groups = (p->cols + 63) / 64;
+    if (const long long parts = sum_parts(chunks)) {
+      SumArgs in_parts = q;
+      float* sums = (float*)ws + (size_t)chunks * c.sums * p->cols;
+      in_parts.out[0] = sums;
+      hipLaunchKernelGGL(residual_norm_sum_kernel<true>, dim3(c.sums < NSUM_ALL ? c.sums : NSUM_ALL - 1, col_groups, (unsigned)parts), dim3(1024), 0,
+                         s, in_parts);
+      PN_CHECK_LAUNCH("residual_norm_sum_kernel");
+      q.partial = sums;
+      q.chunks = (int)parts;
+    }
+    hipLaunchKernelGGL(residual_norm_sum_kernel<false>, dim3((unsigned)vecs, col_groups), dim3(1024), 0, s, q);
     PN_CHECK_LAUNCH("residual_norm_sum_kernel");
   }
   return PN_OK;

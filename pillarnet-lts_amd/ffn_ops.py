@@ -285,7 +285,7 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
     """h = x + scale * gate * dropout(post_norm(branch)), rounded to x's type; y = act(norm(h)).
 
     x, branch: [..., C], one type (C up to 16384).  gate: None, [C] (layer scale), x's shape, or one row for each leading
-    sample -- [B, C] or [B, 1, C] with x [B, ..., C].  post_norm: Norm "layer" / "rms" or None; norm: any Norm or None;
+    sample -- [B, C] or [B, 1, C] with x [B, ..., C], B up to 2^23.  post_norm: Norm "layer" / "rms" or None; norm: any Norm or None;
     dropout: (p, rng, call) as act_dropout or None; act ("none" | "relu") on y.  Differentiable in x, branch, gate and the norms'
     weights and biases.  Returns (h, y) with branch and norm, h without a norm, y without a branch (h is then x itself).
 

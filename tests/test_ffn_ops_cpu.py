@@ -71,7 +71,8 @@ def _join(**kw):
     dict(dtype=2), dict(param_dtype=7), dict(param_dtype=1), dict(cols=0), dict(cols=16385), dict(rows=-1), dict(post_kind=3), dict(norm_kind=4),
     dict(act=2), dict(branch=None, gate=16), dict(branch=None, post_kind=1), dict(branch=None, threshold=5, rng=16),
     dict(branch=None, norm_kind=0), dict(threshold=65537, rng=16), dict(threshold=1), dict(call=65536), dict(x=None),
-    dict(ldx=7), dict(ldb=7), dict(gate=16, rows_per_gate=3), dict(gate=16, rows_per_gate=0)])
+    dict(ldx=7), dict(ldb=7), dict(gate=16, rows_per_gate=3), dict(gate=16, rows_per_gate=0),
+    dict(gate=16, rows_per_gate=2, rows=(1 << 24) + 2)])
 def test_residual_norm_arguments_are_checked_before_the_gpu(bad):
     L = _lib.lib()
     s = _join(**bad)

@@ -341,7 +341,7 @@ def test_residual_norm_with_one_output_used(cuda, dtype, use):
 
 
 @BOTH
-@pytest.mark.parametrize("B,T,C", [(1, 1, 256), (300, 1, 64), (7, 1, 5001), (1, 5000, 40), (64, 3, 520)])
+@pytest.mark.parametrize("B,T,C", [(1, 1, 256), (300, 1, 64), (7, 1, 5001), (1, 5000, 40), (64, 3, 520), (1100, 2, 40)])
 def test_residual_norm_row_counts(cuda, dtype, B, T, C):
     _join_run(cuda, dtype, dtype, B, T, C, "layer", "rms", "sample", 0.5, True)
 
