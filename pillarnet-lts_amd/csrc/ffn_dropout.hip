@@ -38,17 +38,11 @@ __device__ __forceinline__ void load8_view(const T* p, long long ld, long long c
 }
 
 template <typename T, int ACT, bool BWD>
-__global__ __launch_bounds__(256) void act_dropout_kernel(DropArgs a) {
-  const unsigned long long total = (unsigned long long)a.rows * a.cols;
-  const unsigned long long e = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (e >= total) return;
-  const int n = total - e < 8 ? (int)(total - e) : 8;
-  float x[8], g[8], o[8];
-  const T* xp = reinterpret_cast<const T*>(a.x);
-  if (!BWD || ACT != PN_ACT_NONE) load8_view(xp, a.ldx, a.cols, e, n, x);
-  if (BWD) load8_view(reinterpret_cast<const T*>(a.g), a.ldg, a.cols, e, n, g);
+__device__ __forceinline__ void act_dropout_piece(const DropArgs& a, const PhiloxKey& key, unsigned long long e, int n, const float (&x)[8],
+                                                  const float (&g)[8]) {
   Keep8 keep = keep_all();
-  if (a.threshold && !(BWD && ACT == PN_ACT_RELU)) keep = keep8_group(philox_key(a.rng, a.call), e >> 3, a.threshold);
+  if (a.threshold && !(BWD && ACT == PN_ACT_RELU)) keep = keep8_group(key, e >> 3, a.threshold);
+  float o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (!BWD) {
@@ -63,10 +57,37 @@ __global__ __launch_bounds__(256) void act_dropout_kernel(DropArgs a) {
   store8(reinterpret_cast<T*>(a.out) + e, n, o);
 }
 
+// Where a workgroup's pieces are all whole and the rows lie one behind the other, no load stands behind a branch of its own.
+template <typename T, int ACT, bool BWD>
+__global__ __launch_bounds__(256) void act_dropout_kernel(DropArgs a) {
+  const unsigned long long total = (unsigned long long)a.rows * a.cols, block = (unsigned long long)blockIdx.x * 2048, e = block + threadIdx.x * 8;
+  const T *xp = reinterpret_cast<const T*>(a.x), *gp = reinterpret_cast<const T*>(a.g);
+  constexpr bool X = !BWD || ACT != PN_ACT_NONE;
+  PhiloxKey key{};
+  if (a.threshold && !(BWD && ACT == PN_ACT_RELU)) key = philox_key(a.rng, a.call);
+  float x[8], g[8];
+  if (block + 2048 <= total && (!X || a.ldx == a.cols) && (!BWD || a.ldg == a.cols)) {
+    Raw8<T> rx, rg;
+    if (X) rx.load(xp + e);
+    if (BWD) rg.load(gp + e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = X ? rx.get(i) : 0.f;
+      g[i] = BWD ? rg.get(i) : 0.f;
+    }
+    act_dropout_piece<T, ACT, BWD>(a, key, e, 8, x, g);
+    return;
+  }
+  if (e >= total) return;
+  const int n = total - e < 8 ? (int)(total - e) : 8;
+  if (X) load8_view(xp, a.ldx, a.cols, e, n, x);
+  if (BWD) load8_view(gp, a.ldg, a.cols, e, n, g);
+  act_dropout_piece<T, ACT, BWD>(a, key, e, n, x, g);
+}
+
 template <typename T, bool BWD>
 static int launch_act_dropout(const DropArgs& a, int act, hipStream_t s) {
-  const long long groups = (a.rows * a.cols + 7) / 8, blocks = (groups + 255) / 256;
-  const dim3 grid((unsigned)blocks), wg(256);
+  const dim3 grid((unsigned)((a.rows * a.cols + 2047) / 2048)), wg(256);
   switch (act) {
     case PN_ACT_NONE: hipLaunchKernelGGL((act_dropout_kernel<T, PN_ACT_NONE, BWD>), grid, wg, 0, s, a); break;
     case PN_ACT_RELU: hipLaunchKernelGGL((act_dropout_kernel<T, PN_ACT_RELU, BWD>), grid, wg, 0, s, a); break;

@@ -564,7 +564,10 @@ static NormArgs norm_args(const pnResidualNorm* p) {
   return a;
 }
 
-static constexpr int FWD_WAVES = 8192;                  // 32 a CU: what the forward kernel keeps resident
+// Waves of the forward pass: 32 a CU, which then go from row to row with the next row on its way.  Without post norm and dropout rows
+// up to 4096 gain from four times as many (their own turnover overlaps better: 16499 x 2048 bf16 52 -> 47 us, 32768 x 4096 204 -> 199);
+// wider ones and the others lose (4096 x 8192 with both: 68 -> 79 us).
+static constexpr int FWD_WAVES = 8192, FWD_WAVES_PLAIN = 32768;
 
 // Threads per row: the fewest that hold the row at eight elements each (K pieces of eight over 8192 columns, and in the backward
 // pass with a branch over 4096), so that a narrow row does not idle a wave; over 1024 columns the workgroup is as large as its row.
@@ -578,7 +581,7 @@ template <typename T, typename P, int L, int K, int NT> static int norm_fwd(cons
 #define FWD(MODE, L_, K_, NT_)                                                                                                \
   do {                                                                                                                       \
     const int threads = norm_threads(a.p.cols, L_, K_, NT_), slots = L_ ? NT_ / (L_ ? L_ : 1) : 1;                                \
-    const long long need = (a.p.rows + slots - 1) / slots, most = FWD_WAVES / (threads / 64);                            \
+    const long long need = (a.p.rows + slots - 1) / slots, most = (full || NT_ > 512 ? FWD_WAVES : FWD_WAVES_PLAIN) / (threads / 64);                            \
     const dim3 grid((unsigned)(need < most ? need : most)), wg(threads);                                                         \
     if (full) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, true>), grid, wg, 0, s, a);              \
     else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, false>), grid, wg, 0, s, a);                  \
