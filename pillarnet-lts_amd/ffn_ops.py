@@ -76,6 +76,14 @@ def _rows(x):
     return x.contiguous().view(-1, C)
 
 
+def _strided(x):
+    """(x or a copy of it, its row stride) as _rows, without a view where x is contiguous."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
+    x = _rows(x)
+    return x, x.stride(0)
+
+
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -128,10 +136,10 @@ def _check_rng(what, rng, device, call):
 
 def _act_dropout_forward(x, threshold, rng, call, act):
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    v = _rows(x)
-    R, C = v.shape
-    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), R, C, v.stride(0), act, threshold, _ptr(rng), call,
-          y.data_ptr())
+    C = x.shape[-1]
+    v, ld = _strided(x)
+    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), x.numel() // C if C else 0, C, ld, act, threshold, _ptr(rng),
+          call, y.data_ptr())
     return y
 
 
@@ -148,11 +156,11 @@ class _ActDropout(torch.autograd.Function):
         rng, saved = ctx.saved_tensors
         threshold, call, act = ctx.args
         dx = torch.empty_like(g, memory_format=torch.contiguous_format)
-        gv = _rows(g)
-        sv = None if saved is None else _rows(saved)
-        R, C = gv.shape
-        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), R, C, gv.stride(0),
-              0 if sv is None else sv.stride(0), act, threshold, _ptr(rng), call, dx.data_ptr())
+        C = g.shape[-1]
+        gv, ldg = _strided(g)
+        sv, lds = (None, 0) if saved is None else _strided(saved)
+        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), g.numel() // C if C else 0, C, ldg, lds, act,
+              threshold, _ptr(rng), call, dx.data_ptr())
         return dx, None, None, None, None
 
 
@@ -198,14 +206,6 @@ _JoinCfg = namedtuple("_JoinCfg", "post norm post_eps norm_eps scale threshold c
 
 
 _JOIN = struct.Struct("@6i4q3f2I8Q")                     # pnResidualNorm, fields in order
-
-
-def _strided(x):
-    """(x or a copy of it, its row stride) as _rows, without a view where x is contiguous."""
-    if x.is_contiguous():
-        return x, x.shape[-1]
-    x = _rows(x)
-    return x, x.stride(0)
 
 
 def _join_struct(cfg, rows, x, f, gate, pw, pb, w, b, rng):
@@ -455,12 +455,12 @@ def fp8_linear(x, weight, act="none", out_dtype=None):
     _require(not _wants_grad(x), "fp8_linear: forward only (fp8_linear_train has gradients)")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     _require(out_dtype in _DTYPES and act in _lib.PN_ACT, f"fp8_linear: output {out_dtype}, activation {act!r}")
-    v = _rows(x.detach())
-    M = v.shape[0]
+    v, ldx = _strided(x)
+    M = x.numel() // K
     out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
     size = _lib.lib().pn_fp8_linear_workspace_bytes(M, N, K)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _call("pn_fp8_linear", dev, _DTYPES[x.dtype], v.data_ptr(), M, v.stride(0), weight.data.data.data_ptr(), N, K, _ptr(weight.bias),
+    _call("pn_fp8_linear", dev, _DTYPES[x.dtype], v.data_ptr(), M, ldx, weight.data.data.data_ptr(), N, K, _ptr(weight.bias),
           weight.bias_dtype, _lib.PN_ACT[act], _DTYPES[out_dtype], out.data_ptr(), N, _ptr(ws), size)
     return out
 
@@ -470,8 +470,9 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, grads):
         need_x, need_w = grads and x.requires_grad, grads and weight.requires_grad
         L, dev = _lib.lib(), x.device
-        v, wv = _rows(x), _rows(weight)
-        (M, K), N = v.shape, wv.shape[0]
+        (v, ldx), (wv, ldw) = _strided(x), _strided(weight)
+        N, K = weight.shape
+        M = x.numel() // K
         y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
         saved = None
         if M:
@@ -480,8 +481,8 @@ class _Fp8Linear(torch.autograd.Function):
             saved = torch.empty(L.pn_fp8_train_saved_bytes(M, N, K) if need_x or need_w else 1, dtype=torch.uint8, device=dev)
             ws = torch.empty(L.pn_fp8_train_workspace_bytes(M, N, K, 0), dtype=torch.uint8, device=dev)
             b = None if bias is None else bias.contiguous()
-            _call("pn_fp8_train_forward", dev, _DTYPES[x.dtype], v.data_ptr(), M, v.stride(0), _DTYPES[weight.dtype], wv.data_ptr(), N, K,
-                  wv.stride(0), _ptr(b), 0 if b is None else _DTYPES[b.dtype], y.data_ptr(), int(need_w), int(need_x), saved.data_ptr(),
+            _call("pn_fp8_train_forward", dev, _DTYPES[x.dtype], v.data_ptr(), M, ldx, _DTYPES[weight.dtype], wv.data_ptr(), N, K,
+                  ldw, _ptr(b), 0 if b is None else _DTYPES[b.dtype], y.data_ptr(), int(need_w), int(need_x), saved.data_ptr(),
                   ws.data_ptr())
         ctx.save_for_backward(saved)
         ctx.meta = (x.shape, weight.dtype, None if bias is None else bias.dtype)
@@ -492,15 +493,16 @@ class _Fp8Linear(torch.autograd.Function):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         (saved,) = ctx.saved_tensors
         shape, w_dtype, b_dtype = ctx.meta
-        dev, gv = g.device, _rows(g)
-        (M, N), K = gv.shape, shape[-1]
+        dev, (gv, ldg) = g.device, _strided(g)
+        N, K = g.shape[-1], shape[-1]
+        M = g.numel() // N
         dx = torch.empty(shape, dtype=g.dtype, device=dev) if need_x else None
         dw = torch.empty((N, K), dtype=w_dtype, device=dev) if need_w else None
         db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
         if M == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None
         ws = torch.empty(_lib.lib().pn_fp8_train_workspace_bytes(M, N, K, 1), dtype=torch.uint8, device=dev)
-        _call("pn_fp8_train_backward", dev, _DTYPES[g.dtype], gv.data_ptr(), M, gv.stride(0), _DTYPES[w_dtype], N, K, saved.data_ptr(),
+        _call("pn_fp8_train_backward", dev, _DTYPES[g.dtype], gv.data_ptr(), M, ldg, _DTYPES[w_dtype], N, K, saved.data_ptr(),
               _ptr(dx), _ptr(dw), _ptr(db), _DTYPES[b_dtype] if need_b else 0, ws.data_ptr())
         return dx, dw, db, None
 
