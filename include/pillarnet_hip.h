@@ -521,7 +521,7 @@ typedef struct {
  * while serving). */
 int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* y, float* stats, pnStream stream);
 /* gh, gy: gradients of h and y (either may be NULL).  dx [rows, cols]; dbranch [rows, cols], NULL where the branch enters
- * as it is (no gate, post norm, dropout, scale 1: its gradient is dx); the parameters' gradients have type param_dtype and
+ * as it is (no gate, post norm, dropout, scale 1: its gradient is dx; with another scale alone its values are not read); the parameters' gradients have type param_dtype and
  * gate's shape for dgate; any may be NULL.  Deterministic: column sums go through chunk sums in the workspace. */
 size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p);
 int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const float* stats, const void* gh, const void* gy,

@@ -417,6 +417,14 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
       for (int k = 0; k < K; ++k)
         if (live && own.any(k)) own.store(reinterpret_cast<T*>(a.dx) + row * C, k, dh[k]);
     }
+    if (!BRANCH && a.df) {                                // a branch that is only scaled: its values are not needed
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dh[k][i] *= p.scale;
+        if (live && own.any(k)) own.store(reinterpret_cast<T*>(a.df) + row * C, k, dh[k]);
+      }
+    }
     if constexpr (BRANCH) {
       float fh[K][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -641,7 +649,7 @@ static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
   c.sums = branch ? NSUM_ALL : NSUM_NORM;
   return c;
 }
-static bool norm_reads_branch(const pnResidualNorm* p) { return p->branch && (p->gate || p->post_kind != PN_NORM_NONE || p->threshold || p->scale != 1.f); }
+static bool norm_reads_branch(const pnResidualNorm* p) { return p->branch && (p->gate || p->post_kind != PN_NORM_NONE || p->threshold); }
 
 extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
   if (norm_check(p) != PN_OK) return 0;
@@ -694,7 +702,7 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
   PN_CHECK_ARG(p->rows == 0 || stats || (p->norm_kind != PN_NORM_LAYER && p->norm_kind != PN_NORM_RMS && p->post_kind == PN_NORM_NONE),
                "residual_norm: the stored statistics are needed");
   PN_CHECK_ARG(((uintptr_t)stats & 15) == 0, "residual_norm: the statistics must be 16-byte aligned");
-  PN_CHECK_ARG(branch || !dbranch, "residual_norm: the branch's gradient is dx itself");
+  PN_CHECK_ARG(!dbranch || (p->branch && (branch || p->scale != 1.f)), "residual_norm: the branch's gradient is dx itself");
   PN_CHECK_ARG(!dgate || p->gate, "residual_norm: gradient of a gate that there is not");
   const NormChunks c = norm_chunks(p, branch);
   hipStream_t s = (hipStream_t)stream;

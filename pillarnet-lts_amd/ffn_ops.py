@@ -237,7 +237,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, rows, rng, x, f, gate, pw, pb, w, b):
         h, y, stats = _join_forward(cfg, rows, x, f, gate, pw, pb, w, b, rng, True)
-        reads_f = f is not None and (gate is not None or cfg.post or cfg.threshold or cfg.scale != 1.0)
+        reads_f = f is not None and (gate is not None or cfg.post or cfg.threshold)
         ctx.cfg, ctx.rows, ctx.has_branch, ctx.reads_f = cfg, rows, f is not None, reads_f
         # the norm's backward reads the rows it normalised; x itself is needed only where it is those rows
         ctx.save_for_backward(rng, h if f is not None else x, f if reads_f else None, gate, pw, pb, w, b, stats)
@@ -257,11 +257,12 @@ class _ResidualNorm(torch.autograd.Function):
         need_x, need_f, *need = ctx.needs_input_grad[3:]
         gh = None if gh is None else gh.contiguous()
         gy = None if gy is None else gy.contiguous()
-        if gy is None and has_branch and not reads_f:
+        shared = has_branch and not reads_f and cfg.scale == 1.0          # the branch's gradient is dx itself
+        if gy is None and shared:
             return None, None, None, gh if need_x else None, gh if need_f else None, None, None, None, None, None
         contiguous = torch.contiguous_format
-        dx = torch.empty_like(h, memory_format=contiguous) if need_x or (need_f and not reads_f) else None
-        df = torch.empty_like(h, memory_format=contiguous) if need_f and reads_f else None
+        dx = torch.empty_like(h, memory_format=contiguous) if need_x or (need_f and shared) else None
+        df = torch.empty_like(h, memory_format=contiguous) if need_f and not shared else None
         sums = [torch.empty_like(t, memory_format=contiguous) if n and t is not None else None for t, n in zip((gate, pw, pb, w, b), need)]
         if rows == 0:
             for t in sums:
@@ -276,7 +277,7 @@ class _ResidualNorm(torch.autograd.Function):
             _call("pn_residual_norm_backward", h.device, s, h.data_ptr(), stats.data_ptr(), None if gh is None else gh.data_ptr(),
                   None if gy is None else gy.data_ptr(), None if dx is None else dx.data_ptr(), None if df is None else df.data_ptr(),
                   dw, db, dpw, dpb, dgate, ws.data_ptr(), size)
-        if has_branch and not reads_f:
+        if shared:
             df = dx if need_f else None
         return (None, None, None, dx if need_x else None, df, *sums)
 

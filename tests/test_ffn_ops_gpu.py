@@ -338,6 +338,7 @@ def test_residual_norm_without_a_branch(cuda, dtype, norm, B, T):
 def test_residual_norm_with_one_output_used(cuda, dtype, use):
     _join_run(cuda, dtype, dtype, 2, 19, 96, "rms", "layer", "sample", 0.2, True, use=use)
     _join_run(cuda, dtype, dtype, 2, 19, 96, None, "layer", None, 0.0, True, scale=1.0, use=use)     # the branch's gradient is dx
+    _join_run(cuda, dtype, dtype, 2, 19, 100, None, "rms", None, 0.0, True, scale=0.3, use=use)      # ... or a multiple of it
 
 
 @BOTH
