@@ -5,6 +5,10 @@
 // does not reach the output or the gradient.  p is the 16-bit threshold's: T / 65536, and the scale uses that T.
 // Backward of ReLU + dropout reads y instead of x: y > 0 exactly where the element was kept and positive (scaling up never
 // underflows), which frees x and needs no generator.
+//
+// Bound by memory.  A thread takes eight elements, what one run of the generator decides and 16 bytes of bf16: 65536 x 2048 bf16
+// with ReLU, p = 0.1: forward 85 us (6.3 TB/s), backward 142 us (5.7 TB/s).  In fp32 with GELU (6271 x 1023: 13 and 17 us, 4 and
+// 4.5 TB/s) the generator's 40 integer multiplies and the fitted tail are about half the cycles.
 #include "ffn_common.h"
 
 struct DropArgs {

@@ -5,6 +5,13 @@
 //
 // Statistics are two-pass (mean, then the mean of squared distances) in fp32 over the registers.  The norm reads h as it is
 // stored, so the backward pass, which reads the stored h again, differentiates exactly what was computed.
+//
+// Bound by memory, with the next row on its way while one is worked on: 32768 x 4096 bf16, layer scale and LayerNorm, 199 us
+// (5.4 TB/s); 65536 x 256 fp32, LayerNorm, 42 us (6.4 TB/s).  With both norms, gate and dropout (16 x 1031 x 2048 bf16: forward
+// 58 us, 4.6 TB/s; backward 92 us, 4.4 TB/s, and 6.6 for the column sums) the generator and two sums across each row leave too
+// few waves to hide all of it.  Slower than that: rows whose length is no multiple of eight, with dropout (every piece draws two
+// groups: 8192 x 4100 bf16 forward 130 us against 58 at 4096), and training over 8192 columns, where registers spill
+// (2048 x 16384 bf16, both norms: backward 0.8 ms).
 #include "ffn_common.h"
 
 struct NormArgs {

@@ -2,7 +2,13 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes a whole block of 128 in one instruction, with the two scales as byte operands:
 // the blocks' scales cost no vector instruction and the partial sums stay in fp32 accumulators.  The order of k inside a
-// block does not matter as long as both operands agree, so a lane simply holds 32 consecutive bytes of its row.
+// block does not matter as long as both operands agree, so a lane simply holds 32 bytes of its row as they lie in the operand's tile.
+//
+// The instruction rounds the products of eight neighbouring k to 16 bits below the largest of them before it adds (measured with
+// single pairs of products: 1.4e-5 relative at worst).  That is far below a bf16 result's own rounding and far above an fp32
+// result's: for fp32 outputs (WIDE) the same bytes are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16.
+// Measured: 8192^3 398 - 436 us into bf16 (2.5 - 2.8 PFLOP/s), 865 - 944 into fp32 (1.2 - 1.3 PFLOP/s, the bf16 instruction's
+// own bound with the widening beside it); 16384 x 4096 x 8192 with bias and GELU 470 us; one row of 8192 x 8192 15 us (4.4 TB/s).
 #include "ffn_common.h"
 #include <type_traits>
 

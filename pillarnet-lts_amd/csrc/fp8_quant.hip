@@ -8,6 +8,9 @@
 // One 128 x 128 tile per workgroup, read once; from its registers come the bytes along the rows (blocks 1 x 128), along the
 // columns (the transposed operand of a weight gradient, blocks 128 x 1), both with one scale for the whole tile
 // (BLOCK: weights), and the tile's column sums (bias gradients).
+//
+// Bound by memory: 8200 x 4096 bf16 into both operands 32 us (4.2 TB/s), 16384 x 4096 along the rows alone 31 - 50 us (4 - 6.5
+// TB/s).  Small matrices are bound by a tile's way through LDS (512 x 3136 fp32, both operands: 100 tiles, 15 us).
 #include "ffn_common.h"
 
 struct QuantArgs {

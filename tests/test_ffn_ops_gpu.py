@@ -43,6 +43,14 @@ def rng_of(seed, offset, cuda):
     return torch.tensor([seed, offset], dtype=torch.int64, device=cuda)
 
 
+@pytest.fixture
+def large(cuda):
+    """cuda, for tests whose tensors should not count in the peaks that later tests look at."""
+    yield cuda
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+
+
 # ---- activation + dropout ----------------------------------------------------------------------------------------------
 @BOTH
 @pytest.mark.parametrize("act", ["none", "relu", "gelu"])
@@ -132,7 +140,7 @@ def test_dropout_state_moves_on_and_replays(cuda):
         assert torch.equal(out, want), i
 
 
-def test_act_dropout_beyond_32_bit_offsets(cuda):
+def test_act_dropout_beyond_32_bit_offsets(large, cuda):
     """4.3e9 elements: the last groups have element indices past 2^32."""
     cols, rows = 1 << 20, 4099
     x = torch.ones((rows, cols), dtype=torch.bfloat16, device=cuda)
@@ -300,7 +308,7 @@ def test_residual_norm_wide_rows_with_wider_parameters(cuda, C):
     _join_run(cuda, torch.bfloat16, torch.float32, 1, 5, C, None, "layer", None, 0.0, False, act="relu")
 
 
-def test_residual_norm_beyond_32_bit_offsets(cuda):
+def test_residual_norm_beyond_32_bit_offsets(large, cuda):
     """4.3e9 elements: the last rows are those of a call of their own (a mask by element index among them)."""
     C, R = 4104, 1047000
     assert R * C > 1 << 32
@@ -613,7 +621,7 @@ def test_fp8_partial_gradients_and_refusals(cuda):
             call()
 
 
-def test_fp8_beyond_32_bit_offsets(cuda):
+def test_fp8_beyond_32_bit_offsets(large, cuda):
     """x and out of 4.3e9 elements each: the last rows are those of a call of their own (the same sums, other kernels: whole numbers)."""
     M, K, N = (1 << 21) + 5, 2056, 24
     x = torch.zeros((M, K), dtype=torch.bfloat16, device=cuda)
@@ -621,9 +629,13 @@ def test_fp8_beyond_32_bit_offsets(cuda):
     w = torch.randint(-3, 4, (N, K), device=cuda).float()
     y = ffn_ops.fp8_linear(x, ffn_ops.Fp8Weight(w), out_dtype=torch.float32)
     assert torch.equal(y[-300:], x[-300:].float() @ w.t()) and (y[: 300] == 0).all()
-    q, qt = ffn_ops.fp8_quantize(x, transposed=True)
-    assert torch.equal(qt.values()[:, -300:], x[-300:].float().t())
-    del x, q, qt, y
+    q, s = ffn_ops.fp8_quantize(x, rows=False, transposed=True)[1]._parts()
+    B = q.shape[1]                                                           # (the last three blocks of the transpose, by hand)
+    vals = q[:, -3:].permute(0, 4, 1, 3, 2, 5).reshape(-1, 3 * 128)[:K].view(torch.float8_e4m3fn).float()
+    scale = torch.stack([s[b // 4, :, b % 4] for b in range(B - 3, B)], 1).int() << 23
+    got = (vals * scale.view(torch.float32).repeat_interleave(128, 1))[:, : M - (B - 3) * 128]
+    assert torch.equal(got[:, -200:], x[-200:].float().t())
+    del x, q, s, y
     K, N = 128, 2056
     x = torch.zeros((M, K), dtype=torch.bfloat16, device=cuda)
     x[-300:] = torch.randint(-3, 4, (300, K), device=cuda).bfloat16()
