@@ -145,10 +145,9 @@ SIGNATURES = {
     "pn_act_dropout_backward": (c_int, [c_int, c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong, c_int,
                                         c_uint32, c_void_p, c_uint32, c_void_p, c_void_p]),
     "pn_dropout_draw": (c_int, [c_void_p, c_void_p, c_void_p]),
-    # const pnResidualNorm* as an address: byref(pnResidualNorm(...)) or the packed bytes of one, a tenth of the host time
-    "pn_residual_norm_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "pn_residual_norm_workspace_bytes": (c_size_t, [c_void_p]),
-    "pn_residual_norm_backward": (c_int, [c_void_p] * 13 + [c_size_t, c_void_p]),
+    "pn_residual_norm_forward": (c_int, [POINTER(pnResidualNorm), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pn_residual_norm_workspace_bytes": (c_size_t, [POINTER(pnResidualNorm)]),
+    "pn_residual_norm_backward": (c_int, [POINTER(pnResidualNorm)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
     "pn_fp8_operand_bytes": (c_size_t, [c_longlong, c_longlong]),
     "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "pn_fp8_gemm": (c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong,
@@ -183,6 +182,28 @@ def lib():
             fn.argtypes = args
         _lib = h
     return _lib
+
+
+_autograd = None
+
+
+def autograd():
+    """The extension with the autograd nodes of ffn_ops (csrc/ffn_autograd.cpp); raises if it has not been built."""
+    global _autograd
+    if _autograd is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_ffn_autograd.so")
+        if not os.path.exists(path):
+            raise PillarnetHipError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+        import importlib.util
+        import torch  # noqa: F401  (its libraries first)
+        lib()
+        ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)      # the extension's pn_* entries are this library's
+        spec = importlib.util.spec_from_file_location("_ffn_autograd", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_error_class(PillarnetHipError)
+        _autograd = mod
+    return _autograd
 
 
 def check(rc, what):

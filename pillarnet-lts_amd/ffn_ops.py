@@ -9,11 +9,9 @@ with Dropout of roi_head_template.py:23-39, the mixers of mlp_layers.py:24-117) 
 All take fp32 or bf16 tensors on the GPU, run on the current stream of the tensors' device, allocate through torch's
 caching allocator only and wait for nothing, so they can be captured into a HIP graph.  A graph that holds a backward pass
 is captured while no eager autograd graph over the same leaves is alive (torch's own rule for captured backward passes)."""
-import struct
 from collections import namedtuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import PillarnetHipError
@@ -58,6 +56,17 @@ def _call(name, device, *args):
         _lib.check(rc, name)
 
 
+_EXT = None
+
+
+def _nodes():
+    """The autograd nodes (csrc/ffn_autograd.cpp)."""
+    global _EXT
+    if _EXT is None:
+        _EXT = _lib.autograd()
+    return _EXT
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -92,16 +101,6 @@ def _wants_grad(*tensors):
     return False
 
 
-def _backward(fn):
-    """A backward pass that is not itself differentiable: the guard against a second derivative is only put up where one could
-    be asked for (create_graph), as it costs as much host time as a launch."""
-    guarded = once_differentiable(fn)
-
-    def backward(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
-    return staticmethod(backward)
-
-
 # ---- activation + dropout ----------------------------------------------------------------------------------------------
 def dropout_threshold(p):
     """The 16-bit threshold of a drop probability: p is taken to the nearest 1 / 65536, at least one step for p > 0 and
@@ -134,36 +133,6 @@ def _check_rng(what, rng, device, call):
     _require(0 <= call < 65536, f"{what}: call {call} (0 to 65535)")
 
 
-def _act_dropout_forward(x, threshold, rng, call, act):
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    C = x.shape[-1]
-    v, ld = _strided(x)
-    _call("pn_act_dropout_forward", x.device, _DTYPES[x.dtype], v.data_ptr(), x.numel() // C if C else 0, C, ld, act, threshold, _ptr(rng),
-          call, y.data_ptr())
-    return y
-
-
-class _ActDropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, threshold, rng, call, act):
-        y = _act_dropout_forward(x, threshold, rng, call, act)
-        ctx.save_for_backward(rng, x if act == _lib.PN_ACT["gelu"] else y if act == _lib.PN_ACT["relu"] else None)
-        ctx.args = (threshold, call, act)
-        return y
-
-    @_backward
-    def backward(ctx, g):
-        rng, saved = ctx.saved_tensors
-        threshold, call, act = ctx.args
-        dx = torch.empty_like(g, memory_format=torch.contiguous_format)
-        C = g.shape[-1]
-        gv, ldg = _strided(g)
-        sv, lds = (None, 0) if saved is None else _strided(saved)
-        _call("pn_act_dropout_backward", g.device, _DTYPES[g.dtype], gv.data_ptr(), _ptr(sv), g.numel() // C if C else 0, C, ldg, lds, act,
-              threshold, _ptr(rng), call, dx.data_ptr())
-        return dx, None, None, None, None
-
-
 def act_dropout(x, p, rng=None, call=0, act="none"):
     """dropout(act(x), p) with act "none" | "relu" | "gelu" (erf form), differentiable in x.
 
@@ -180,9 +149,7 @@ def act_dropout(x, p, rng=None, call=0, act="none"):
         if act == "none":
             return x
         rng, call = None, 0
-    if _wants_grad(x):
-        return _ActDropout.apply(x, threshold, rng, call, _lib.PN_ACT[act])
-    return _act_dropout_forward(x.detach(), threshold, rng, call, _lib.PN_ACT[act])
+    return _nodes().act_dropout(x, threshold, rng, call, _lib.PN_ACT[act])
 
 
 # ---- residual join and norms -------------------------------------------------------------------------------------------
@@ -200,86 +167,6 @@ class Norm(namedtuple("Norm", "kind weight bias eps")):
         _require(kind is not None and len(module.normalized_shape) == 1, f"Norm.of: {module}")
         eps = module.eps if module.eps is not None else torch.finfo(torch.float32).eps
         return cls(kind, module.weight, getattr(module, "bias", None), eps)
-
-
-_JoinCfg = namedtuple("_JoinCfg", "post norm post_eps norm_eps scale threshold call act rows_per_gate")
-
-
-_JOIN = struct.Struct("@6i4q3f2I8Q")                     # pnResidualNorm, fields in order
-
-
-def _join_struct(cfg, rows, x, f, gate, pw, pb, w, b, rng):
-    """(packed struct, tensors that must outlive the launch)."""
-    x, ldx = _strided(x)
-    f, ldf = (None, 0) if f is None else _strided(f)
-    param = gate if gate is not None else pw if pw is not None else pb if pb is not None else w if w is not None else b
-    s = _JOIN.pack(
-        _DTYPES[x.dtype], _lib.PN_DTYPE_F32 if param is None else _DTYPES[param.dtype], cfg.post, cfg.norm, cfg.act, x.shape[-1],
-        rows, cfg.rows_per_gate, ldx, ldf, cfg.scale, cfg.post_eps, cfg.norm_eps, cfg.threshold, cfg.call,
-        0 if rng is None else rng.data_ptr(), x.data_ptr(), 0 if f is None else f.data_ptr(), 0 if gate is None else gate.data_ptr(),
-        0 if pw is None else pw.data_ptr(), 0 if pb is None else pb.data_ptr(), 0 if w is None else w.data_ptr(),
-        0 if b is None else b.data_ptr())
-    return s, (x, f)
-
-
-def _join_forward(cfg, rows, x, f, gate, pw, pb, w, b, rng, want_stats):
-    s, keep = _join_struct(cfg, rows, x, f, gate, pw, pb, w, b, rng)
-    h = torch.empty_like(x, memory_format=torch.contiguous_format) if f is not None else None
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if cfg.norm else None
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    if rows:                            # (an empty tensor has no address to tell the branch by)
-        _call("pn_residual_norm_forward", x.device, s, None if h is None else h.data_ptr(), None if y is None else y.data_ptr(),
-              None if stats is None else stats.data_ptr())
-    return h, y, stats
-
-
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, cfg, rows, rng, x, f, gate, pw, pb, w, b):
-        h, y, stats = _join_forward(cfg, rows, x, f, gate, pw, pb, w, b, rng, True)
-        reads_f = f is not None and (gate is not None or cfg.post or cfg.threshold)
-        ctx.cfg, ctx.rows, ctx.has_branch, ctx.reads_f = cfg, rows, f is not None, reads_f
-        # the norm's backward reads the rows it normalised; x itself is needed only where it is those rows
-        ctx.save_for_backward(rng, h if f is not None else x, f if reads_f else None, gate, pw, pb, w, b, stats)
-        ctx.set_materialize_grads(False)
-        return (h, y) if f is not None and cfg.norm else h if f is not None else y
-
-    @_backward
-    def backward(ctx, *grads):
-        cfg, rows, has_branch, reads_f = ctx.cfg, ctx.rows, ctx.has_branch, ctx.reads_f
-        rng, h, f, gate, pw, pb, w, b, stats = ctx.saved_tensors
-        if has_branch:
-            gh, gy = grads if cfg.norm else (grads[0], None)
-        else:
-            gh, gy = None, grads[0]
-        if gh is None and gy is None:
-            return (None,) * 10
-        need_x, need_f, *need = ctx.needs_input_grad[3:]
-        gh = None if gh is None else gh.contiguous()
-        gy = None if gy is None else gy.contiguous()
-        shared = has_branch and not reads_f and cfg.scale == 1.0          # the branch's gradient is dx itself
-        if gy is None and shared:
-            return None, None, None, gh if need_x else None, gh if need_f else None, None, None, None, None, None
-        contiguous = torch.contiguous_format
-        dx = torch.empty_like(h, memory_format=contiguous) if need_x or (need_f and shared) else None
-        df = torch.empty_like(h, memory_format=contiguous) if need_f and not shared else None
-        sums = [torch.empty_like(t, memory_format=contiguous) if n and t is not None else None for t, n in zip((gate, pw, pb, w, b), need)]
-        if rows == 0:
-            for t in sums:
-                if t is not None:
-                    t.zero_()
-        else:
-            # without reads_f the struct still needs a branch pointer to say that h is a stored tensor: h stands in, unread
-            s, keep = _join_struct(cfg, rows, h, (f if reads_f else h) if has_branch else None, gate, pw, pb, w, b, rng)
-            size = _lib.lib().pn_residual_norm_workspace_bytes(s)
-            ws = torch.empty(size, dtype=torch.uint8, device=h.device)
-            dgate, dpw, dpb, dw, db = [None if t is None else t.data_ptr() for t in sums]
-            _call("pn_residual_norm_backward", h.device, s, h.data_ptr(), stats.data_ptr(), None if gh is None else gh.data_ptr(),
-                  None if gy is None else gy.data_ptr(), None if dx is None else dx.data_ptr(), None if df is None else df.data_ptr(),
-                  dw, db, dpw, dpb, dgate, ws.data_ptr(), size)
-        if shared:
-            df = dx if need_f else None
-        return (None, None, None, dx if need_x else None, df, *sums)
 
 
 def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=None, dropout=None, act="none"):
@@ -336,13 +223,11 @@ def residual_norm(x, branch=None, gate=None, scale=1.0, post_norm=None, norm=Non
             gate, pw, pb, w, b = [None if q is None else (q if same else q.float()).contiguous() for q in (gate, pw, pb, w, b)]
             break
         first = first if t is None else t.dtype
-    cfg = _JoinCfg(_lib.PN_NORM[post_norm.kind] if post_norm is not None else 0, _lib.PN_NORM[norm.kind] if norm is not None else 0,
-                   post_norm.eps if post_norm is not None else 0.0, norm.eps if norm is not None else 0.0, float(scale), threshold, call,
-                   _lib.PN_ACT[act], rows_per_gate)
-    if _wants_grad(x, branch, gate, pw, pb, w, b):
-        return _ResidualNorm.apply(cfg, R, rng, x, branch, gate, pw, pb, w, b)
-    h, y, _ = _join_forward(cfg, R, x, branch, gate, pw, pb, w, b, rng, False)
-    return (h, y) if h is not None and y is not None else h if y is None else y
+    out = _nodes().residual_norm(
+        x, branch, gate, pw, pb, w, b, rng, _lib.PN_NORM[post_norm.kind] if post_norm is not None else 0,
+        _lib.PN_NORM[norm.kind] if norm is not None else 0, post_norm.eps if post_norm is not None else 0.0,
+        norm.eps if norm is not None else 0.0, scale, threshold, call, _lib.PN_ACT[act], R, rows_per_gate)
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 # ---- products in fp8 ---------------------------------------------------------------------------------------------------
@@ -466,48 +351,6 @@ def fp8_linear(x, weight, act="none", out_dtype=None):
     return out
 
 
-class _Fp8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, grads):
-        need_x, need_w = grads and x.requires_grad, grads and weight.requires_grad
-        L, dev = _lib.lib(), x.device
-        (v, ldx), (wv, ldw) = _strided(x), _strided(weight)
-        N, K = weight.shape
-        M = x.numel() // K
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-        saved = None
-        if M:
-            # the transposed operands that the backward pass reads: a byte an element; x and the weight are not kept
-            # (one byte stands in where neither gradient is wanted)
-            saved = torch.empty(L.pn_fp8_train_saved_bytes(M, N, K) if need_x or need_w else 1, dtype=torch.uint8, device=dev)
-            ws = torch.empty(L.pn_fp8_train_workspace_bytes(M, N, K, 0), dtype=torch.uint8, device=dev)
-            b = None if bias is None else bias.contiguous()
-            _call("pn_fp8_train_forward", dev, _DTYPES[x.dtype], v.data_ptr(), M, ldx, _DTYPES[weight.dtype], wv.data_ptr(), N, K,
-                  ldw, _ptr(b), 0 if b is None else _DTYPES[b.dtype], y.data_ptr(), int(need_w), int(need_x), saved.data_ptr(),
-                  ws.data_ptr())
-        ctx.save_for_backward(saved)
-        ctx.meta = (x.shape, weight.dtype, None if bias is None else bias.dtype)
-        return y
-
-    @_backward
-    def backward(ctx, g):
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        (saved,) = ctx.saved_tensors
-        shape, w_dtype, b_dtype = ctx.meta
-        dev, (gv, ldg) = g.device, _strided(g)
-        N, K = g.shape[-1], shape[-1]
-        M = g.numel() // N
-        dx = torch.empty(shape, dtype=g.dtype, device=dev) if need_x else None
-        dw = torch.empty((N, K), dtype=w_dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
-        if M == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None
-        ws = torch.empty(_lib.lib().pn_fp8_train_workspace_bytes(M, N, K, 1), dtype=torch.uint8, device=dev)
-        _call("pn_fp8_train_backward", dev, _DTYPES[g.dtype], gv.data_ptr(), M, ldg, _DTYPES[w_dtype], N, K, saved.data_ptr(),
-              _ptr(dx), _ptr(dw), _ptr(db), _DTYPES[b_dtype] if need_b else 0, ws.data_ptr())
-        return dx, dw, db, None
-
-
 def fp8_linear_train(x, weight, bias=None):
     """x @ weight.T + bias for x [..., K], weight [N, K] (fp32 or bf16 master weight), with every product in fp8:
       y = Q(x) Qw(weight)^T + bias,  dx = Q(g) Qw(weight),  dweight = Q(g^T) Q(x^T)^T,  dbias = column sums of g (fp32 sums of g
@@ -518,4 +361,4 @@ def fp8_linear_train(x, weight, bias=None):
              f"fp8_linear_train: x {tuple(x.shape)} for a weight {tuple(weight.shape)}")
     _require(bias is None or bias.shape == (weight.shape[0],), f"fp8_linear_train: the bias has shape [{weight.shape[0]}]")
     _require(max(x.numel() // x.shape[-1], *weight.shape) <= 1 << 22, "fp8_linear_train: more than 2^22 rows or features")
-    return _Fp8Linear.apply(x, weight, bias, torch.is_grad_enabled())
+    return _nodes().fp8_linear_train(x, weight, bias)

@@ -141,8 +141,6 @@ def test_dropout_and_fp8_arguments_are_checked_before_the_gpu():
 
 def test_struct_layout_matches_header():
     assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers
-    values = [3, 1, 2, 1, 0, 64, 10, 5, 64, 64, 0.5, 1e-5, 1e-6, 77, 9, *range(1 << 33, (1 << 33) + 8)]
-    assert ffn_ops._JOIN.pack(*values) == bytes(_lib.pnResidualNorm(*values))           # what ffn_ops hands over
 
 
 def test_a_head_without_a_fused_path_says_so():
