@@ -9,9 +9,9 @@
 // Bound by memory, with the next row on its way while one is worked on: 32768 x 4096 bf16, layer scale and LayerNorm, 199 us
 // (5.4 TB/s); 65536 x 256 fp32, LayerNorm, 42 us (6.4 TB/s).  With both norms, gate and dropout (16 x 1031 x 2048 bf16: forward
 // 58 us, 4.6 TB/s; backward 92 us, 4.4 TB/s, and 6.6 for the column sums) the generator and two sums across each row leave too
-// few waves to hide all of it.  Slower than that: rows whose length is no multiple of eight, with dropout (every piece draws two
-// groups: 8192 x 4100 bf16 forward 130 us against 58 at 4096), and training over 8192 columns, where registers spill
-// (2048 x 16384 bf16, both norms: backward 0.8 ms).
+// few waves to hide all of it.  Slower than that: rows whose length is no multiple of eight (16 x 1031 x 2047: 77 and 135 us), rows
+// a little over a power of two (4096 x 4200 bf16, both norms: forward 61 us, 2.3 TB/s: one workgroup of twelve waves on a CU, nine of
+// them with columns), and training over 8192 columns, where registers spill (2048 x 16384 bf16, both norms: backward 0.8 ms).
 #include "ffn_common.h"
 
 struct NormArgs {
@@ -585,23 +585,33 @@ static NormArgs norm_args(const pnResidualNorm* p) {
 static constexpr int FWD_WAVES = 8192, FWD_WAVES_PLAIN = 32768;
 
 // Threads per row: the fewest that hold the row at eight elements each (K pieces of eight over 8192 columns, and in the backward
-// pass with a branch over 4096), so that a narrow row does not idle a wave; over 1024 columns the workgroup is as large as its row.
+// pass with a branch over 4096), so that a narrow row does not idle a wave; over 1024 columns the workgroup is as large as its row,
+// in whole waves (granule 64) or in a wave for each SIMD (256).  Where registers leave room for 8 or 16 waves a CU, odd numbers of
+// them leave SIMDs idle: backward with a branch 16496 x 2104 bf16 184 us against 229, 8192 x 3000 104 against 153; forward with post
+// norm or dropout over 2048 columns 59 against 70 (8192 x 3000), below it whole waves are as good or better (16496 x 1304: 51 against
+// 56).  Without them whole waves win up to 2560 columns forward (16496 x 2104: 59 against 68; 4096 x 7000: 57 against 47) and at all
+// widths backward.
 #define NORM_BY_COLS(C, WIDE, GO)                                                \
   (C) <= 64 ? GO(8, 1, 256) : (C) <= 128 ? GO(16, 1, 256) : (C) <= 256 ? GO(32, 1, 256) : (C) <= 512 ? GO(64, 1, 256) \
   : (C) <= 1024 ? GO(128, 1, 256) : (C) <= 4096 ? GO(0, 1, 512) : (C) <= 8192 ? WIDE : GO(0, 2, 1024)
-static int norm_threads(int C, int L, int K, int NT) { return L ? NT : ((C + 8 * K - 1) / (8 * K) + 63) / 64 * 64; }
+static int norm_threads(int C, int L, int K, int NT, int granule) {
+  return L ? NT : ((C + 8 * K - 1) / (8 * K) + granule - 1) / granule * granule;
+}
+static int fwd_granule(int C, bool full) { return C <= (full ? 2048 : 2560) ? 64 : 256; }
+static int bwd_granule(bool branch) { return branch ? 256 : 64; }
 
 template <typename T, typename P, int L, int K, int NT> static int norm_fwd(const NormArgs& a, hipStream_t s) {
   const bool full = a.p.post_kind != PN_NORM_NONE || a.p.threshold;
+  const int granule = fwd_granule(a.p.cols, full);
 #define FWD(MODE, L_, K_, NT_)                                                                                                \
   do {                                                                                                                       \
-    const int threads = norm_threads(a.p.cols, L_, K_, NT_), slots = L_ ? NT_ / (L_ ? L_ : 1) : 1;                                \
+    const int threads = norm_threads(a.p.cols, L_, K_, NT_, granule), slots = L_ ? NT_ / (L_ ? L_ : 1) : 1;                                \
     const long long need = (a.p.rows + slots - 1) / slots, most = (full || NT_ > 512 ? FWD_WAVES : FWD_WAVES_PLAIN) / (threads / 64);                            \
     const dim3 grid((unsigned)(need < most ? need : most)), wg(threads);                                                         \
     if (full) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, true>), grid, wg, 0, s, a);              \
     else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, P, L_, K_, NT_, MODE, false>), grid, wg, 0, s, a);                  \
   } while (0)
-  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT)) * K * 8) FWD(EXACT, L, K, NT);
+  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT, granule)) * K * 8) FWD(EXACT, L, K, NT);
   else if (a.p.cols >= 8) FWD(RAGGED, L, K, NT);
   else FWD(TINY, 8, 1, 256);
 #undef FWD
@@ -641,7 +651,7 @@ static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
   if (c.groups < 1) c.groups = 1;
   c.group_rows = c.groups > 1 ? p->rows_per_gate : p->rows;
 #define SLOTS_OF(L, K, NT) (L ? NT / (L ? L : 1) : 1)
-#define WAVES_OF(L, K, NT) (norm_threads(p->cols, L, K, NT) / 64)
+#define WAVES_OF(L, K, NT) (norm_threads(p->cols, L, K, NT, bwd_granule(branch)) / 64)
   const int slots = NORM_BY_COLS(p->cols, 1, SLOTS_OF), waves = NORM_BY_COLS(p->cols, (branch ? WAVES_OF(0, 2, 512) : WAVES_OF(0, 1, 1024)), WAVES_OF);
 #undef SLOTS_OF
 #undef WAVES_OF
@@ -666,7 +676,7 @@ extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
 }
 
 template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH> static int norm_bwd(const NormArgs& a, unsigned grid, hipStream_t s) {
-  const int threads = norm_threads(a.p.cols, L, K, NT);
+  const int threads = norm_threads(a.p.cols, L, K, NT, bwd_granule(BRANCH));
   size_t lds = 0;
   if (bwd_parks(L, K, NT, BRANCH)) {
     lds = (size_t)4 * K * 8 * sizeof(P) * threads;
@@ -684,7 +694,7 @@ template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH> s
   return PN_OK;
 }
 template <typename T, typename P, int L, int K, int NT, bool BRANCH> static int norm_bwd_by_mode(const NormArgs& a, unsigned grid, hipStream_t s) {
-  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT)) * K * 8) return norm_bwd<T, P, L, K, NT, EXACT, BRANCH>(a, grid, s);
+  if (a.p.cols == (L ? L : norm_threads(a.p.cols, L, K, NT, bwd_granule(BRANCH))) * K * 8) return norm_bwd<T, P, L, K, NT, EXACT, BRANCH>(a, grid, s);
   return a.p.cols >= 8 ? norm_bwd<T, P, L, K, NT, RAGGED, BRANCH>(a, grid, s) : norm_bwd<T, P, 8, 1, 256, TINY, BRANCH>(a, grid, s);
 }
 template <typename T, typename P, bool BRANCH> static int norm_bwd_by_cols(const NormArgs& a, unsigned grid, hipStream_t s) {
