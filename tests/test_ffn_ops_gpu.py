@@ -697,3 +697,45 @@ def test_feed_forward_block_captured_and_on_another_stream(cuda):
         for k, (a, b) in enumerate(zip(out, want[i])):
             assert torch.equal(a, b), (i, k)
         (x0 @ P["w1"].t()).relu().sum().item()                                   # eager work between replays
+
+
+def test_operators_under_torchs_other_modes(cuda):
+    """inference mode, activation checkpointing (the second forward pass draws the same masks) and saved tensors kept on the host give
+    the bits of the plain pass."""
+    from torch.utils.checkpoint import checkpoint
+    gen = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen).to(cuda).requires_grad_()
+    x, w1, b1, w2, nw, gate, rng = r(40, 72), r(136, 72), r(136), r(72, 136), r(72), r(72), rng_of(8, 1, cuda)
+    leaves, g = [x, w1, b1, w2, nw, gate], torch.randn(40, 72, generator=gen).to(cuda)
+
+    def block(x):
+        a = ffn_ops.act_dropout(ffn_ops.fp8_linear_train(x, w1, b1), 0.3, rng, 0, "gelu")
+        return ffn_ops.residual_norm(x, ffn_ops.fp8_linear_train(a, w2), gate=gate, norm=ffn_ops.Norm("rms", nw), dropout=(0.3, rng, 1))[1]
+
+    y = block(x)
+    want = torch.autograd.grad(y, leaves, g)
+    with torch.inference_mode():
+        assert torch.equal(block(x.detach()), y)
+    z = checkpoint(block, x, use_reentrant=False)
+    assert torch.equal(z, y)
+    for a, b in zip(torch.autograd.grad(z, leaves, g), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.save_on_cpu():
+        z = block(x)
+    for a, b in zip(torch.autograd.grad(z, leaves, g), want):
+        assert torch.equal(a, b)
+    y = block(x)
+    with torch.no_grad():
+        nw.mul_(2)                                                 # a parameter that the backward pass reads
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaves, g)
+
+
+def test_an_entrys_refusal_is_the_frameworks_error(cuda):
+    B = (1 << 23) + 1
+    x = torch.zeros(B, 2, 1, device=cuda)
+    with pytest.raises(PillarnetHipError, match="gates of several rows"):
+        ffn_ops.residual_norm(x, x, gate=torch.zeros(B, 1, device=cuda))
+    x.requires_grad_()
+    with pytest.raises(PillarnetHipError, match="gates of several rows"):
+        ffn_ops.residual_norm(x, x, gate=torch.zeros(B, 1, device=cuda))
