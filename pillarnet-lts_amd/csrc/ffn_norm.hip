@@ -642,7 +642,7 @@ extern "C" int pn_residual_norm_forward(const pnResidualNorm* p, void* h, void* 
 }
 
 // Chunks of the backward pass: about BWD_WAVES waves in all (8 a CU: what the kernel with a branch keeps resident; a workgroup a CU at the least), whole passes
-// over the row slots, none across two gates.
+// over the row slots, none across two gates.  Half as many again leave a part-filled round: 8192 x 4096 bf16 with a branch 95 -> 118 us.
 static constexpr int BWD_WAVES = 2048;
 struct NormChunks { long long groups, group_rows; int per_group, rows, sums; };
 static NormChunks norm_chunks(const pnResidualNorm* p, bool branch) {
