@@ -297,6 +297,11 @@ def fp8_matmul(x, w, bias=None, act="none", out_dtype=torch.bfloat16):
     return out
 
 
+def _scale_bytes(exponents):
+    """Exponents of any integer type -> scale bytes e + 127; clamped before the sum, which a narrow type cannot hold."""
+    return (exponents.long().clamp(-126, 127) + 127).to(torch.uint8)
+
+
 class Fp8Weight:
     """A layer's weight [N, K] laid out once for fp8_linear: e4m3 bytes, one scale for each 128 x 128 tile."""
 
@@ -324,7 +329,7 @@ class Fp8Weight:
         q, s = data._parts()
         pad = torch.nn.functional.pad(values.view(torch.uint8), (0, kb * 128 - K, 0, q.shape[0] * 16 - N))
         q.copy_(pad.view(q.shape[0], 16, kb, 4, 2, 16).permute(0, 2, 4, 3, 1, 5))
-        e = torch.nn.functional.pad((exponents + 127).clamp(1, 254).to(torch.uint8), (0, s.shape[0] * 4 - kb))
+        e = torch.nn.functional.pad(_scale_bytes(exponents), (0, s.shape[0] * 4 - kb))
         s.copy_(e.repeat_interleave(128, 0)[:N].view(N, -1, 4).permute(1, 0, 2))
         self._set(data, bias)
         return self

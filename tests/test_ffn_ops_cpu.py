@@ -60,6 +60,14 @@ def test_host_tensors_are_refused():
         ffn_ops.Norm("group", w, w)
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_scale_bytes_of_any_integer_type_clamp_to_the_nearer_end(dtype):
+    lim = torch.iinfo(dtype)
+    e = sorted({lim.min, lim.max, 0, 1, 5, 126, 127, *((-127, -126, -125, -1) if lim.min < 0 else (128, 200))})
+    got = ffn_ops._scale_bytes(torch.tensor([e], dtype=dtype))
+    assert got.dtype == torch.uint8 and got[0].tolist() == [max(-126, min(127, v)) + 127 for v in e]
+
+
 def _join(**kw):
     d = dict(dtype=0, param_dtype=0, post_kind=0, norm_kind=1, act=0, cols=8, rows=4, rows_per_gate=4, ldx=8, ldb=8, scale=1.0,
              post_eps=1e-5, norm_eps=1e-5, threshold=0, call=0, x=16, branch=16)

@@ -549,6 +549,16 @@ def test_fp8_weight_from_blocks_and_infinities(cuda):
     assert (z == 0).all()
 
 
+@pytest.mark.parametrize("etype", [torch.int8, torch.uint8, torch.int16, torch.int64])
+def test_fp8_weight_exponents_of_any_integer_type(cuda, etype):
+    """exponents in a narrow type stand for what they say, and those past -126 .. 127 for the nearer end."""
+    v = torch.ones(3, 200, device=cuda).to(torch.float8_e4m3fn)
+    for a, b in ((5, 3), (torch.iinfo(etype).max, 0), (max(torch.iinfo(etype).min, -200), 1)):
+        e = torch.tensor([[a, b]], dtype=etype, device=cuda)
+        got = ffn_ops.Fp8Weight.from_blocks(v, e).data.bytes_and_exponents()[1]
+        assert got.tolist() == [[max(-126, min(127, a)), b]] * 3
+
+
 @pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16], ids=["w32", "w16"])
 @BOTH
 @pytest.mark.parametrize("M,K,N,bias", [(1, 8, 8, True), (5, 130, 260, False), (130, 257, 96, True), (512, 640, 256, True), (700, 129, 515, False)])
