@@ -81,6 +81,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// The nodes have no forward-mode derivative; a bare kernel would drop an input's tangent without a word.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) throw Failed(std::string(what) + ": no forward-mode derivative");
+}
+
 // ---- residual join and norms ----
 struct Join {
   Tensor x, f, gate, pw, pb, w, b, rng;
@@ -190,6 +196,7 @@ std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& f, const Maybe& 
   j.s.norm_eps = (float)norm_eps;
   j.s.threshold = threshold;
   j.s.call = call;
+  no_tangents("residual_norm", {&j.x, &j.f, &j.gate, &j.pw, &j.pb, &j.w, &j.b});
   if (wants_grad({&j.x, &j.f, &j.gate, &j.pw, &j.pb, &j.w, &j.b})) return ResidualNorm::apply(x, f, gate, pw, pb, w, b, &j);
   const Joined o = join_forward(j, false);
   if (!o.h.defined()) return {o.y};
@@ -241,6 +248,7 @@ struct ActDropout : torch::autograd::Function<ActDropout> {
 
 Tensor act_dropout(const Tensor& x, unsigned threshold, const Maybe& rng, unsigned call, int act) {
   const Drop d = {or_none(rng), threshold, call, act};
+  no_tangents("act_dropout", {&x});
   return wants_grad({&x}) ? ActDropout::apply(x, &d) : drop_forward(x, d);
 }
 
@@ -295,6 +303,8 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
 };
 
 Tensor fp8_linear_train(const Tensor& x, const Tensor& weight, const Maybe& bias) {
+  const Tensor b = or_none(bias);
+  no_tangents("fp8_linear_train", {&x, &weight, &b});
   return Fp8Linear::apply(x, weight, bias, (bool)at::GradMode::is_enabled());
 }
 

@@ -8,10 +8,12 @@ with Dropout of roi_head_template.py:23-39, the mixers of mlp_layers.py:24-117) 
 
 All take fp32 or bf16 tensors on the GPU, run on the current stream of the tensors' device, allocate through torch's
 caching allocator only and wait for nothing, so they can be captured into a HIP graph.  A graph that holds a backward pass
-is captured while no eager autograd graph over the same leaves is alive (torch's own rule for captured backward passes)."""
+is captured while no eager autograd graph over the same leaves is alive (torch's own rule for captured backward passes).
+Derivatives are reverse-mode and of first order: tensors with a forward-mode tangent are refused."""
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import PillarnetHipError
@@ -99,6 +101,12 @@ def _wants_grad(*tensors):
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _no_tangent(what, x):
+    """Where a kernel is called outside of the autograd nodes: a tangent would be dropped without a word."""
+    if forward_ad._current_level >= 0:
+        _require(forward_ad.unpack_dual(x).tangent is None, f"{what}: no forward-mode derivative")
 
 
 # ---- activation + dropout ----------------------------------------------------------------------------------------------
@@ -344,6 +352,7 @@ def fp8_linear(x, weight, act="none", out_dtype=None):
     _require(x.dim() >= 1 and x.shape[-1] == K, f"fp8_linear: rows of {tuple(x.shape)} for a weight of {K}")
     _require(dev == weight.data.data.device, f"fp8_linear: x on {dev}, the weight on {weight.data.data.device}")
     _require(not _wants_grad(x), "fp8_linear: forward only (fp8_linear_train has gradients)")
+    _no_tangent("fp8_linear", x)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     _require(out_dtype in _DTYPES and act in _lib.PN_ACT, f"fp8_linear: output {out_dtype}, activation {act!r}")
     v, ldx = _strided(x)

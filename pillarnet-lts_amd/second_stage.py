@@ -641,7 +641,7 @@ class RoIHeadTemplate(nn.Module):
         grads = torch.is_grad_enabled() and (x.requires_grad or m.weight.requires_grad or (m.bias is not None and m.bias.requires_grad))
         if self.fp8 and not grads:
             plan = FP8_PLANS.get(m, lambda m: ffn_ops.Fp8Weight(m.weight.flatten(1), m.bias))
-            return ffn_ops.fp8_linear(x.detach(), plan, act)
+            return ffn_ops.fp8_linear(x, plan, act)
         y = ffn_ops.fp8_linear_train(x, w, m.bias) if self.fp8 else Fn.linear(x, w, m.bias)
         return y if act == "none" else ffn_ops.act_dropout(y, 0.0, act=act)
 

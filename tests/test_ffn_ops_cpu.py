@@ -68,6 +68,25 @@ def test_scale_bytes_of_any_integer_type_clamp_to_the_nearer_end(dtype):
     assert got.dtype == torch.uint8 and got[0].tolist() == [max(-126, min(127, v)) + 127 for v in e]
 
 
+def test_forward_mode_tangents_are_refused():
+    """neither the nodes nor a kernel called beside them drop a tangent in silence (empty tensors launch nothing)."""
+    fw, n = torch.autograd.forward_ad, _lib.autograd()
+    e, w = torch.zeros(0, 8), torch.zeros(8)
+    join = lambda x, f=None, gate=None, w=None: n.residual_norm(x, f, gate, None, None, w, None, None, 0, 1, 0.0, 1e-5, 1.0, 0, 0, 0, 0, 1)
+    with fw.dual_level():
+        d, dw = fw.make_dual(e, torch.ones(0, 8)), fw.make_dual(w, torch.ones(8))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: n.act_dropout(d, 0, None, 0, 2), lambda: join(d), lambda: join(e, d), lambda: join(e, e, dw),
+                             lambda: join(e, w=dw), lambda: n.fp8_linear_train(d, torch.zeros(4, 8), None),
+                             lambda: n.fp8_linear_train(e, torch.zeros(8, 8), dw), lambda: ffn_ops._no_tangent("fp8_linear", d)):
+                    with pytest.raises(PillarnetHipError, match="no forward-mode derivative"):
+                        call()
+                assert n.act_dropout(e, 0, None, 0, 2).shape == join(e)[0].shape == (0, 8)      # others go on as ever
+                ffn_ops._no_tangent("fp8_linear", e)
+    ffn_ops._no_tangent("fp8_linear", d)
+
+
 def _join(**kw):
     d = dict(dtype=0, param_dtype=0, post_kind=0, norm_kind=1, act=0, cols=8, rows=4, rows_per_gate=4, ldx=8, ldb=8, scale=1.0,
              post_eps=1e-5, norm_eps=1e-5, threshold=0, call=0, x=16, branch=16)

@@ -669,6 +669,24 @@ def test_second_derivatives_are_refused(cuda):
             g.sum().backward()
 
 
+def test_forward_mode_tangents_are_refused(cuda):
+    from pillarnet_lts_amd import second_stage
+    fw = torch.autograd.forward_ad
+    x, w = torch.randn(6, 64, device=cuda), torch.randn(32, 64, device=cuda)
+    plan = ffn_ops.Fp8Weight(w)
+    head = second_stage.RoIHeadTemplate(1, {}).to(cuda)
+    head.fp8 = True
+    fc = torch.nn.Linear(64, 32).to(cuda).requires_grad_(False)
+    with fw.dual_level():
+        t = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ffn_ops.act_dropout(t, 0.0, act="gelu"), lambda: ffn_ops.residual_norm(t, norm=ffn_ops.Norm("rms")),
+                     lambda: ffn_ops.residual_norm(x, t), lambda: ffn_ops.fp8_linear_train(t, w), lambda: ffn_ops.fp8_linear(t, plan),
+                     lambda: head.fused_linear(fc, t)):
+            with pytest.raises(PillarnetHipError, match="no forward-mode derivative"):
+                call()
+        assert head.fused_linear(fc, x).shape == (6, 32)
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------
 def test_feed_forward_block_captured_and_on_another_stream(cuda):
     """one block as the heads use it -- norm, fp8 product, activation + dropout, fp8 product, residual join -- forward and backward,
