@@ -508,39 +508,43 @@ __global__ __launch_bounds__(NT) void residual_norm_bwd_kernel(NormArgs a) {
 }
 
 // out[v][c] = sum over the chunks of vector v: blockIdx.x picks the vector (weight, bias, post weight, post bias, then
-// one gate row each), blockIdx.y its 64 columns; 16 chunk lanes.
+// one gate row each), blockIdx.y its 64 columns; 16 chunk lanes.  A launch holds less than 2^32 threads along x, 2^22 workgroups of this
+// kernel: past SUM_GRID vectors a workgroup goes on to another.
 // PARTS: blockIdx.z picks a part of SUM_PART chunks and the sums stay fp32 chunk sums, [part][sums][cols] at out[0]: with a chunk for
 // each of many gates a single pass over them would be a few workgroups' (100000 gates of two rows, 256 columns: 10 ms).
-static constexpr int SUM_PART = 256;
+static constexpr int SUM_PART = 256, SUM_GRID = 1 << 21;
 struct SumArgs {
   const float *partial, *gate_partial;      // chunk sums; those of the gates' rows
   void* out[NSUM_ALL];
-  int cols, sums, chunks, chunks_per_group, out_bf16;
+  int cols, sums, chunks, chunks_per_group, out_bf16, vecs;
 };
 template <bool PARTS> __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(SumArgs a) {
   __shared__ float lds[16][64];
-  const int v = blockIdx.x, s = v < NSUM_ALL - 1 ? v : NSUM_ALL - 1, group = PARTS ? blockIdx.z : v - s;
-  void* out = a.out[PARTS ? 0 : s];
-  if (!out) return;                                                        // the same for the whole workgroup
-  const bool gate = s == NSUM_ALL - 1;
-  const int first = PARTS ? group * SUM_PART : gate ? group * a.chunks_per_group : 0;
-  const int count = PARTS ? min(SUM_PART, a.chunks - first) : gate ? a.chunks_per_group : a.chunks;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 64 + lane;
-  float acc = 0.f;
-  if (c < a.cols) {
-    const float* p = (gate ? a.gate_partial : a.partial) + ((size_t)first * a.sums + s) * a.cols + c;
+  for (int v = blockIdx.x; v < a.vecs; v += gridDim.x) {
+    const int s = v < NSUM_ALL - 1 ? v : NSUM_ALL - 1, group = PARTS ? blockIdx.z : v - s;
+    void* out = a.out[PARTS ? 0 : s];
+    if (!out) continue;                                                    // the same for the whole workgroup
+    const bool gate = s == NSUM_ALL - 1;
+    const int first = PARTS ? group * SUM_PART : gate ? group * a.chunks_per_group : 0;
+    const int count = PARTS ? min(SUM_PART, a.chunks - first) : gate ? a.chunks_per_group : a.chunks;
+    float acc = 0.f;
+    if (c < a.cols) {
+      const float* p = (gate ? a.gate_partial : a.partial) + ((size_t)first * a.sums + s) * a.cols + c;
 #pragma unroll 8
-    for (int i = w; i < count; i += 16) acc += p[(size_t)i * a.sums * a.cols];
-  }
-  lds[w][lane] = acc;
-  __syncthreads();
-  if (w == 0 && c < a.cols) {
-    float t = 0.f;
+      for (int i = w; i < count; i += 16) acc += p[(size_t)i * a.sums * a.cols];
+    }
+    lds[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && c < a.cols) {
+      float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += lds[i][lane];
-    const size_t at = PARTS ? ((size_t)group * a.sums + s) * a.cols + c : (size_t)group * a.cols + c;
-    if (!PARTS && a.out_bf16) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
-    else reinterpret_cast<float*>(out)[at] = t;
+      for (int i = 0; i < 16; ++i) t += lds[i][lane];
+      const size_t at = PARTS ? ((size_t)group * a.sums + s) * a.cols + c : (size_t)group * a.cols + c;
+      if (!PARTS && a.out_bf16) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
+      else reinterpret_cast<float*>(out)[at] = t;
+    }
+    __syncthreads();                                                       // read before the next vector's sums overwrite them
   }
 }
 // parts that the chunks are added in before the last sum (0: one pass)
@@ -677,6 +681,7 @@ extern "C" size_t pn_residual_norm_workspace_bytes(const pnResidualNorm* p) {
 
 template <typename T, typename P, int L, int K, int NT, int MODE, bool BRANCH> static int norm_bwd(const NormArgs& a, unsigned grid, hipStream_t s) {
   const int threads = norm_threads(a.p.cols, L, K, NT, bwd_granule(BRANCH));
+  PN_CHECK_ARG((unsigned long long)grid * threads < 1ull << 32, "residual_norm: %u chunks of %d threads are more than one launch takes", grid, threads);
   size_t lds = 0;
   if (bwd_parks(L, K, NT, BRANCH)) {
     lds = (size_t)4 * K * 8 * sizeof(P) * threads;
@@ -754,19 +759,19 @@ extern "C" int pn_residual_norm_backward(const pnResidualNorm* p, const void* h,
     const long long vecs = dgate ? NSUM_ALL - 1 + c.groups : (dpost_weight || dpost_bias) ? NSUM_ALL - 1 : NSUM_NORM;
     if (!p->rows) dgate = nullptr;                 // no rows, no gates
     SumArgs q = {(const float*)ws, (const float*)ws, {dweight, dbias, dpost_weight, dpost_bias, dgate}, p->cols, c.sums, (int)chunks,
-                 chunks ? c.per_group : 0, p->param_dtype == PN_DTYPE_BF16};
+                 chunks ? c.per_group : 0, p->param_dtype == PN_DTYPE_BF16, (int)vecs};
     const unsigned col_groups = (p->cols + 63) / 64;
     if (const long long parts = sum_parts(chunks)) {
       SumArgs in_parts = q;
       float* sums = (float*)ws + (size_t)chunks * c.sums * p->cols;
       in_parts.out[0] = sums;
-      hipLaunchKernelGGL(residual_norm_sum_kernel<true>, dim3(c.sums < NSUM_ALL ? c.sums : NSUM_ALL - 1, col_groups, (unsigned)parts), dim3(1024), 0,
-                         s, in_parts);
+      in_parts.vecs = c.sums < NSUM_ALL ? c.sums : NSUM_ALL - 1;
+      hipLaunchKernelGGL(residual_norm_sum_kernel<true>, dim3(in_parts.vecs, col_groups, (unsigned)parts), dim3(1024), 0, s, in_parts);
       PN_CHECK_LAUNCH("residual_norm_sum_kernel");
       q.partial = sums;
       q.chunks = (int)parts;
     }
-    hipLaunchKernelGGL(residual_norm_sum_kernel<false>, dim3((unsigned)vecs, col_groups), dim3(1024), 0, s, q);
+    hipLaunchKernelGGL(residual_norm_sum_kernel<false>, dim3((unsigned)(vecs < SUM_GRID ? vecs : SUM_GRID), col_groups), dim3(1024), 0, s, q);
     PN_CHECK_LAUNCH("residual_norm_sum_kernel");
   }
   return PN_OK;

@@ -419,6 +419,25 @@ def test_residual_norm_repeats_its_bits(cuda):
             assert torch.equal(a, b)
 
 
+def test_residual_norm_most_gates_of_several_rows(large, cuda):
+    """2^23 gates of two rows: more vectors of column sums than one launch has workgroups of 1024 threads.  Whole numbers: exact."""
+    B = 1 << 23
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    whole = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=gen, device=cuda).float()
+    x, f, gate, gh = whole(-3, 4, B, 2, 1), whole(-3, 4, B, 2, 1), whole(-2, 3, B, 1), whole(-3, 4, B, 2, 1)
+    gy, w = torch.zeros(B, 2, 1, device=cuda), whole(2, 3, 1)
+    gy[::1 << 10] = 1.0                                                # 2^14 rows of 2^24: their sum with |h| <= 9 stays below 2^24
+    leaves = [t.requires_grad_() for t in (x, f, gate, w)]
+    h, y = ffn_ops.residual_norm(x, f, gate=gate, norm=ffn_ops.Norm("affine", w))
+    dx, df, dg, dw = torch.autograd.grad((h, y), leaves, (gh, gy))
+    g = gate.detach()[:, None]
+    want = x + g * f
+    assert torch.equal(h, want) and torch.equal(y, 2 * want)
+    dh = gh + 2 * gy
+    assert torch.equal(dx, dh) and torch.equal(df, g * dh) and torch.equal(dg, (dh * f).sum(1))
+    assert dw.item() == (gy * want).double().sum().item()
+
+
 def test_residual_norm_refusals(cuda):
     x = torch.zeros(4, 6, 8, device=cuda)
     w, N = torch.zeros(8, device=cuda), ffn_ops.Norm
