@@ -490,7 +490,7 @@ int pn_points_to_voxel(const float* points, long long n, int feats, const float*
  * is keyed by rng = {seed, offset} (two uint64 in device memory, read when the kernel runs), `call` (< 65536: the dropout's
  * number within a pass) and the element's index row * cols + col, so no mask is stored and strides do not matter.
  * Backward: dx = keep ? g * scale * act'(x) : 0 with the same rng contents; `saved` is x for PN_ACT_GELU, y for PN_ACT_RELU,
- * NULL for PN_ACT_NONE.  Dropped elements are exactly zero, whatever x or g hold there. */
+ * NULL for PN_ACT_NONE.  Dropped elements are exactly zero, whatever x or g hold there.  Up to 2^35 - 2048 elements. */
 int pn_act_dropout_forward(int dtype, const void* x, long long rows, long long cols, long long ldx, int act,
                            unsigned threshold, const void* rng, unsigned call, void* y, pnStream stream);
 int pn_act_dropout_backward(int dtype, const void* g, const void* saved, long long rows, long long cols, long long ldg,

@@ -107,7 +107,8 @@ static int act_dropout(bool bwd, int dtype, DropArgs a, int act, void* stream) {
   PN_CHECK_ARG(a.threshold <= 65536u && a.call < 65536u, "act_dropout: threshold %u (0..65536), call %u (0..65535)", a.threshold, a.call);
   PN_CHECK_ARG(a.rows >= 0 && a.cols >= 0, "act_dropout: negative size");
   if (a.rows == 0 || a.cols == 0) return PN_OK;
-  PN_CHECK_ARG(a.rows <= (1ll << 41) / a.cols, "act_dropout: %lld x %lld elements are more than one launch takes", a.rows, a.cols);
+  // (workgroups of 256 threads and 2048 elements; a launch holds less than 2^32 threads)
+  PN_CHECK_ARG(a.rows <= ((1ll << 35) - 2048) / a.cols, "act_dropout: %lld x %lld elements are more than one launch takes", a.rows, a.cols);
   PN_CHECK_ARG(a.out && (a.x || (bwd && act == PN_ACT_NONE)) && (a.g || !bwd), "act_dropout: null pointer");
   PN_CHECK_ARG(a.rng || !a.threshold, "act_dropout: dropping needs the generator's state");
   PN_CHECK_ARG((!a.x || a.ldx >= a.cols || a.rows == 1) && (!a.g || a.ldg >= a.cols || a.rows == 1), "act_dropout: row stride below the row length");

@@ -146,7 +146,8 @@ def act_dropout(x, p, rng=None, call=0, act="none"):
 
     rng: int64 [2] (seed, offset) on x's device, what `DropoutState.draw()` returns; it is read when the kernels run, the
     backward pass included, so its contents stay until then.  call (< 65536) tells the dropouts of one pass apart.  p = 0
-    needs no rng, p = 1 gives zeros.  The mask depends on (seed, offset, call, element index) only, not on strides."""
+    needs no rng, p = 1 gives zeros.  The mask depends on (seed, offset, call, element index) only, not on strides.
+    Up to 2^35 - 2048 elements."""
     _check("act_dropout", x)
     _require(act in _lib.PN_ACT, f"act_dropout: activation {act!r}")
     _require(x.dim() >= 1, "act_dropout: a tensor of at least one dimension")

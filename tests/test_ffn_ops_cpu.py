@@ -166,6 +166,15 @@ def test_dropout_and_fp8_arguments_are_checked_before_the_gpu():
     assert L.pn_fp8_train_saved_bytes(0, 8, 8) == 0 and L.pn_fp8_train_workspace_bytes(4, 8, 8, 1) >= 4 * 8
 
 
+def test_more_elements_than_a_launch_takes_are_refused():
+    """a launch holds less than 2^32 threads along a dimension: 256 a workgroup here, for 2048 elements."""
+    L = _lib.lib()
+    for rows, cols in (((1 << 35) - 2047, 1), (1, (1 << 35) - 2047), (1 << 20, 1 << 15), (1 << 24, 1 << 17)):
+        for rc in (L.pn_act_dropout_forward(1, 16, rows, cols, cols, 0, 5, 16, 0, 16, None),
+                   L.pn_act_dropout_backward(1, 16, None, rows, cols, cols, cols, 0, 5, 16, 0, 16, None)):
+            assert rc == -1 and b"more than one launch takes" in L.pn_last_error()
+
+
 def test_struct_layout_matches_header():
     assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers
 
