@@ -539,7 +539,7 @@ int pn_residual_norm_backward(const pnResidualNorm* p, const void* h, const floa
  *   scales  behind them, words [ceil(blocks / 4)][rows]: byte b % 4 of word (b / 4, row) = e + 127 of block b of the row.
  * pn_fp8_quantize writes q, the operand of x, and / or qt, that of its transpose.  block_rows 1: blocks of 1 x 128 along either
  * operand's contraction (activations, gradients); 128: one scale for each 128 x 128 tile, the same in both (weights).
- * colsum: NULL or [ceil(rows / 128)][cols] fp32, column sums of x over each 128 rows. */
+ * colsum: NULL or [ceil(rows / 128)][cols] fp32, column sums of x over each 128 rows.  Fewer than 2^24 tiles of 128 x 128. */
 size_t pn_fp8_operand_bytes(long long rows, long long cols);
 int pn_fp8_quantize(int dtype, const void* x, long long rows, int cols, long long ldx, int block_rows, void* q, void* qt,
                     float* colsum, pnStream stream);

@@ -156,11 +156,14 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
 }
 
 int fp8_quantize_launch(const Fp8QuantJob& j, hipStream_t s) {
+  // (a launch holds less than 2^32 threads; many rows of few columns get there within the card's memory)
+  const long long tiles = (j.rows + 127) / 128 * ((j.cols + 127ll) / 128);
+  PN_CHECK_ARG(tiles < 1ll << 24, "fp8 quantiser: %lld x %d elements are more than one launch takes", j.rows, j.cols);
   const Fp8Operand q = fp8_operand(j.q, j.rows, j.cols), qt = fp8_operand(j.qt, j.cols, j.rows);
   const int col_blocks = (j.cols + 127) / 128;
   QuantArgs a = {j.x, j.rows, j.rows == 1 ? 0 : j.ldx, j.cols, col_blocks, (unsigned char*)q.q, (unsigned char*)q.scale,
                  (unsigned char*)qt.q, (unsigned char*)qt.scale, j.colsum};
-  const dim3 grid((unsigned)((j.rows + 127) / 128 * col_blocks)), wg(256);
+  const dim3 grid((unsigned)tiles), wg(256);
   if (j.dtype == PN_DTYPE_F32) {
     if (j.block_rows == 1) hipLaunchKernelGGL((fp8_quantize_kernel<float, false>), grid, wg, 0, s, a);
     else hipLaunchKernelGGL((fp8_quantize_kernel<float, true>), grid, wg, 0, s, a);
@@ -178,8 +181,7 @@ extern "C" int pn_fp8_quantize(int dtype, const void* x, long long rows, int col
                                float* colsum, void* stream) {
   PN_CHECK_ARG(dtype == PN_DTYPE_F32 || dtype == PN_DTYPE_BF16, "pn_fp8_quantize: element type %d (fp32 or bf16)", dtype);
   PN_CHECK_ARG(block_rows == 1 || block_rows == 128, "pn_fp8_quantize: blocks of %d rows (1 or 128)", block_rows);
-  PN_CHECK_ARG(rows >= 0 && cols >= 1 && (rows + 127) / 128 < (1ll << 31) / ((cols + 127) / 128), "pn_fp8_quantize: %lld x %d elements",
-               rows, cols);
+  PN_CHECK_ARG(rows >= 0 && cols >= 1 && rows < (1ll << 40) / cols, "pn_fp8_quantize: %lld x %d elements", rows, cols);
   if (rows == 0) return PN_OK;
   PN_CHECK_ARG(x && (rows == 1 || ldx >= cols), "pn_fp8_quantize: x missing or its row stride below the row length");
   PN_CHECK_ARG(q || qt || colsum, "pn_fp8_quantize: output missing");

@@ -173,6 +173,9 @@ def test_more_elements_than_a_launch_takes_are_refused():
         for rc in (L.pn_act_dropout_forward(1, 16, rows, cols, cols, 0, 5, 16, 0, 16, None),
                    L.pn_act_dropout_backward(1, 16, None, rows, cols, cols, cols, 0, 5, 16, 0, 16, None)):
             assert rc == -1 and b"more than one launch takes" in L.pn_last_error()
+    for rows, cols in (((1 << 31) - 127, 1), (1 << 27, 2048), (128, (1 << 31) - 127)):        # 2^24 tiles of 128 x 128
+        assert L.pn_fp8_quantize(1, 16, rows, cols, cols, 1, None, 256, None, None) == -1
+        assert b"more than one launch takes" in L.pn_last_error()
 
 
 def test_struct_layout_matches_header():
