@@ -130,7 +130,7 @@ FP8_PLANS = dense_hip.PlanCache(lambda m: (dense_hip.params_version(m), tuple(p.
 class FoldedMLP:
     """Eval-mode stack of (Conv1d(k=1) | Linear) + BatchNorm1d + ReLU [+ Dropout] ... as plain fp32
     `relu(x @ W' + b')` launches with the norm folded into W', b'; `fp8`: the products in e4m3 with block scales
-    (ffn_ops.fp8_linear), fp32 in between."""
+    (ffn_ops.fp8_linear; fp8_linear_train on the same weights for rows that want a gradient), fp32 in between."""
 
     def __init__(self, layers, fp8=False):
         self.fp8 = fp8
@@ -151,7 +151,7 @@ class FoldedMLP:
             if j < len(mods) and isinstance(mods[j], nn.ReLU):
                 relu, j = True, j + 1
             if fp8:
-                self.steps.append((ffn_ops.Fp8Weight(w.float(), b.float()), None, relu))
+                self.steps.append((ffn_ops.Fp8Weight(w.float(), b.float()), (w.float(), b.float()), relu))
             else:
                 self.steps.append((w.t().float().contiguous(), b.float().contiguous(), relu))
             i = j
@@ -159,7 +159,10 @@ class FoldedMLP:
     def __call__(self, x):
         for wt, b, relu in self.steps:
             if self.fp8:
-                x = ffn_ops.fp8_linear(x, wt, "relu" if relu else "none")
+                if torch.is_grad_enabled() and x.requires_grad:
+                    x = ffn_ops.act_dropout(ffn_ops.fp8_linear_train(x, *b), 0.0, act="relu" if relu else "none")
+                else:
+                    x = ffn_ops.fp8_linear(x, wt, "relu" if relu else "none")
                 continue
             x = torch.addmm(b, x, wt)
             if relu:

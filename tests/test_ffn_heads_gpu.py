@@ -132,6 +132,35 @@ def test_ffn_head_dropout_and_fp8_layers(cuda):
         assert not torch.equal(old, head.fused_linear(fc1, x))
 
 
+def test_fp8_evaluation_with_gradients_enabled(cuda):
+    """a folded stack in fp8 gives its rows' gradient, dx = Q(g) Qw(W), and evaluating a head outside of no_grad works as it does
+    without fp8."""
+    torch.manual_seed(4)
+    fc = torch.nn.Linear(96, 40).to(cuda)
+    mlp = second_stage.FoldedMLP([fc, torch.nn.ReLU()], fp8=True)
+    x, g = torch.randn(70, 96, device=cuda, requires_grad=True), torch.randn(70, 40, device=cuda)
+    y = mlp(x)
+    dx, = torch.autograd.grad(y, x, g)
+    rounded = lambda t, b: ffn_ops.fp8_quantize(t, b)[0].values().double()
+    w = rounded(fc.weight, 128)
+    # fp32 sums of 96 and 40 products and a bias: K + 2 roundings of 2^-24 of the sum of magnitudes at most
+    xq, gq = rounded(x, 1), rounded(g * (y > 0), 1)
+    assert ((y - (xq @ w.t() + fc.bias).relu()).abs() <= 200 * 2.0 ** -24 * (xq.abs() @ w.t().abs() + fc.bias.abs())).all()
+    assert ((dx - gq @ w).abs() <= 100 * 2.0 ** -24 * (gq.abs() @ w.abs())).all()
+    assert not mlp(x.detach()).requires_grad
+    head, batch, _ = _mix_head(cuda, fp8=True)
+    head.eval()
+    feats = batch["roi_features"].clone().requires_grad_()
+    out = head(dict(batch, roi_features=feats), training=False)["batch_cls_preds"]
+    with torch.no_grad():
+        want = head(dict(batch), training=False)["batch_cls_preds"]
+    # sums in another order; an input that then falls on the other side of an e4m3 border moves one of some hundred summands of a
+    # row by 2^-3 of itself: 1e-2 of the norm has room for many of those
+    assert (out - want).norm() <= 1e-2 * want.norm()
+    grads = torch.autograd.grad(out.sum(), [feats, *head.mlp_mixer.parameters()])
+    assert all(torch.isfinite(q).all() for q in grads) and grads[0].abs().sum() > 0
+
+
 def test_heads_refuse_host_tensors_when_fused():
     from pillarnet_lts_amd._lib import PillarnetHipError
     head = second_stage.RoIFFNHead(model_cfg=ConfigDict(CFG), feedforward_channels=48, content_dim=32, fused_ops=True)
