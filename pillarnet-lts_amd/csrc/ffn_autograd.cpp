@@ -5,6 +5,7 @@
 #include <cstring>
 #include <string>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
@@ -17,7 +18,9 @@ typedef std::optional<Tensor> Maybe;
 
 namespace {
 
+PyObject* error_class = nullptr;                           // PillarnetHipError
 struct Failed : std::runtime_error { using std::runtime_error::runtime_error; };
+void set_python_error(const Failed& e) { PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what()); }
 void check(int rc, const char* entry) {
   if (rc != PN_OK) throw Failed(std::string(entry) + " failed (rc=" + std::to_string(rc) + "): " + pn_last_error());
 }
@@ -60,6 +63,20 @@ struct Rows {
     }
   }
 };
+
+// A node's backward runs on the engine's thread, behind torch's own binding, which knows no Failed: the exception that carries a
+// Python error from there to the caller takes its place.
+template <typename F> variable_list on_engine_thread(const F& f) {
+  try {
+    return f();
+  } catch (const Failed& e) {
+    pybind11::gil_scoped_acquire gil;
+    set_python_error(e);
+    python_error carried;
+    carried.persist();
+    throw carried;
+  }
+}
 
 // A gradient that cannot be differentiated again says so, as torch's once_differentiable does.
 variable_list only_once(const variable_list& grads, variable_list out) {
@@ -139,6 +156,9 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     return {o.h, o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     Join j;
     memcpy(&j.s, ctx->saved_data["s"].toStringRef().data(), sizeof(j.s));
@@ -231,6 +251,9 @@ struct ActDropout : torch::autograd::Function<ActDropout> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const int64_t args = ctx->saved_data["args"].toInt(), cols = grads[0].size(-1);
     const Tensor& g = grads[0];
@@ -279,6 +302,9 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const Tensor &g = grads[0], saved = ctx->get_saved_variables()[0];
     const int64_t N = g.size(-1), K = ctx->saved_data["k"].toInt(), M = g.numel() / N, bt = ctx->saved_data["b"].toInt();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bt >= 0 && ctx->needs_input_grad(2);
@@ -310,15 +336,13 @@ Tensor fp8_linear_train(const Tensor& x, const Tensor& weight, const Maybe& bias
 
 }  // namespace
 
-static PyObject* error_class = nullptr;                    // PillarnetHipError
-
 PYBIND11_MODULE(_ffn_autograd, m) {
   m.def("set_error_class", [](const pybind11::object& c) { error_class = c.inc_ref().ptr(); });
   pybind11::register_local_exception_translator([](std::exception_ptr p) {
     try {
       if (p) std::rethrow_exception(p);
     } catch (const Failed& e) {
-      PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
+      set_python_error(e);
     }
   });
   m.def("act_dropout", &act_dropout);

@@ -786,3 +786,21 @@ def test_an_entrys_refusal_is_the_frameworks_error(cuda):
     x.requires_grad_()
     with pytest.raises(PillarnetHipError, match="gates of several rows"):
         ffn_ops.residual_norm(x, x, gate=torch.zeros(B, 1, device=cuda))
+
+
+def test_a_refusal_in_a_backward_pass_is_the_frameworks_error(cuda):
+    """an entry that refuses its arguments on the engine's thread; the hooks hand the nodes saved tensors that the host's checks refuse."""
+    x, w, rng = torch.randn(6, 64, device=cuda, requires_grad=True), torch.randn(32, 64, device=cuda), rng_of(1, 2, cuda)
+    off = lambda t, step: torch.empty(t.numel() + step, dtype=t.dtype, device=cuda)[step:].view(t.shape)
+    cases = [(lambda: ffn_ops.residual_norm(x, norm=ffn_ops.Norm("rms")), lambda t: off(t, 1) if t.shape == (6, 4) else t, "16-byte aligned"),
+             (lambda: ffn_ops.act_dropout(x, 0.5, rng), lambda t: t[:0].clone() if t.dtype == torch.int64 else t, "generator's state"),
+             (lambda: ffn_ops.fp8_linear_train(x, w), lambda t: off(t, 1), "256-byte alignment")]
+    for call, unpack, says in cases:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y, z = call(), call()
+        with pytest.raises(PillarnetHipError, match=says):
+            y.sum().backward()
+        with pytest.raises(PillarnetHipError, match=says):
+            torch.autograd.grad(z.sum(), x)
+    assert torch.isfinite(torch.autograd.grad(ffn_ops.fp8_linear_train(x, w).sum(), x)[0]).all()
+
