@@ -552,6 +552,16 @@ int pn_fp8_gemm(const void* x, long long m, const void* w, int n, int k, const v
 size_t pn_fp8_linear_workspace_bytes(long long m, int n, int k);
 int pn_fp8_linear(int dtype, const void* x, long long m, long long ldx, const void* w, int n, int k, const void* bias, int bias_dtype,
                   int act, int out_dtype, void* out, long long ldo, void* workspace, size_t workspace_bytes, pnStream stream);
+/* Which kernel a product of these sizes takes on the current device; launches nothing.  laid_out: pn_fp8_gemm (and the training step's
+ * products), otherwise pn_fp8_linear.  The rows behind the last whole tiles may take another, in bits 4 and up (0: they do not).
+ * DIRECT_n: 16 x n outputs a workgroup, its waves share the contraction (pn_fp8_linear lays x out on the way); TILE_n: n x n outputs;
+ * PAIR: 256 x 256 (fp32 outputs 128 x 256) in two groups of waves. */
+#define PN_FP8_DIRECT_32 1
+#define PN_FP8_DIRECT_64 2
+#define PN_FP8_TILE_64 3
+#define PN_FP8_TILE_128 4
+#define PN_FP8_PAIR 5
+int pn_fp8_kernels(long long m, int n, int k, int out_dtype, int laid_out);
 /* Training, y [m, n] = x w^T + bias with x [m, k] and the weight [n, k] as they are; all sizes 1 .. 2^22:
  *   forward   y (x's type, dense); keeps the transposed operands of x (save_x) and of the weight (save_w) in `saved`
  *             (pn_fp8_train_saved_bytes, for the backward pass); workspace: pn_fp8_train_workspace_bytes(.., 0).

@@ -16,6 +16,7 @@ PN_DTYPE_F32, PN_DTYPE_BF16 = 0, 1
 PN_ACT = {"none": 0, "relu": 1, "gelu": 2}
 PN_NORM = {"none": 0, "layer": 1, "rms": 2, "affine": 3}
 PN_NORM_MAX_COLS = 16384
+PN_FP8_DIRECT_32, PN_FP8_DIRECT_64, PN_FP8_TILE_64, PN_FP8_TILE_128, PN_FP8_PAIR = 1, 2, 3, 4, 5
 
 
 class PillarnetHipError(RuntimeError):
@@ -152,6 +153,7 @@ SIGNATURES = {
     "pn_fp8_quantize": (c_int, [c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "pn_fp8_gemm": (c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong,
                             c_void_p]),
+    "pn_fp8_kernels": (c_int, [c_longlong, c_int, c_int, c_int, c_int]),
     "pn_fp8_linear_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
     "pn_fp8_linear": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
                               c_void_p, c_longlong, c_void_p, c_size_t, c_void_p]),

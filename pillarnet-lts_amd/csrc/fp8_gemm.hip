@@ -808,38 +808,52 @@ static float fp8_cost(const Fp8Cost& c, long long m, int n, int kblocks, int cus
 // work is spread over more CUs by 16 rows x 32 or 64 columns, the blocks dealt to a workgroup's waves (512 x 3136 x 256: 6 us
 // against 11).
 static bool fp8_spread(long long m, int n, int k) { return k >= 1024 && (m + 15) / 16 * ((n + 63) / 64) <= 256; }
-template <typename T> static int fp8_direct_by_size(const Fp8DirectArgs& d, hipStream_t s) {
-  return (d.g.M + 15) / 16 * ((d.g.N + 31) / 32) <= 256 ? fp8_direct<T, 2, 8, 2>(d, s) : fp8_direct<T, 4, 8, 2>(d, s);
+static int fp8_direct_kind(long long m, int n) { return (m + 15) / 16 * ((n + 31) / 32) <= 256 ? PN_FP8_DIRECT_32 : PN_FP8_DIRECT_64; }
+template <typename T> static int fp8_direct_by_kind(int kind, const Fp8DirectArgs& d, hipStream_t s) {
+  return kind == PN_FP8_DIRECT_32 ? fp8_direct<T, 2, 8, 2>(d, s) : fp8_direct<T, 4, 8, 2>(d, s);
 }
 
-template <bool WIDE> static int fp8_small(const Fp8GemmArgs& a, int cus, hipStream_t s) {
-  if (fp8_spread(a.M, a.N, a.kblocks * 128)) return fp8_direct_by_size<Fp8Laid>(Fp8DirectArgs{a, nullptr, 0, a.kblocks * 128}, s);
-  if (fp8_cost(FP8_64[WIDE], a.M, a.N, a.kblocks, cus) <= fp8_cost(FP8_128[WIDE], a.M, a.N, a.kblocks, cus))
-    return fp8_tile<64, 64, 2, 2, 2, WIDE>(a, s);
-  return fp8_tile<128, 128, 2, 2, 2, WIDE>(a, s);
+// The kernel of a product's first `rows` rows, and that of the rows behind them (0: there are none)
+struct Fp8Plan { int kind, rest; long long rows; };
+static int fp8_small_kind(long long m, int n, int kb, int cus, bool wide) {
+  if (fp8_spread(m, n, kb * 128)) return fp8_direct_kind(m, n);
+  return fp8_cost(FP8_64[wide], m, n, kb, cus) <= fp8_cost(FP8_128[wide], m, n, kb, cus) ? PN_FP8_TILE_64 : PN_FP8_TILE_128;
 }
-
-template <bool WIDE> static int fp8_gemm_by_size(Fp8GemmArgs a, hipStream_t s) {
-  const int cus = fp8_cus(), kb = a.kblocks, bm = FP8_PAIR[WIDE].bm;
-  auto small = [&](long long m) {
-    const float c64 = fp8_cost(FP8_64[WIDE], m, a.N, kb, cus), c128 = fp8_cost(FP8_128[WIDE], m, a.N, kb, cus);
+static Fp8Plan fp8_plan(long long m, int n, int kb, bool wide) {
+  const int cus = fp8_cus(), bm = FP8_PAIR[wide].bm;
+  auto small = [&](long long rows) {
+    const float c64 = fp8_cost(FP8_64[wide], rows, n, kb, cus), c128 = fp8_cost(FP8_128[wide], rows, n, kb, cus);
     return c64 < c128 ? c64 : c128;
   };
-  const float by_small = small(a.M), by_pair = fp8_cost(FP8_PAIR[WIDE], a.M, a.N, kb, cus);
+  const float by_small = small(m), by_pair = fp8_cost(FP8_PAIR[wide], m, n, kb, cus);
   // Rows that fill whole tiles of the pair kernel, and the few behind them in a launch of their own: 8200 x 2048 x 4096 takes
   // 94 us as three rounds of 256 x 256, 90 us in 128 x 128, 72 us as two rounds and 8 for a strip of 8 rows
-  const long long whole = a.M / bm * bm;
-  const float by_split = whole && whole < a.M ? fp8_cost(FP8_PAIR[WIDE], whole, a.N, kb, cus) + small(a.M - whole) : 1e30f;
-  if (by_small <= by_pair && by_small <= by_split) return fp8_small<WIDE>(a, cus, s);
-  if (by_pair <= by_split) return fp8_pair<WIDE>(a, s);
+  const long long whole = m / bm * bm;
+  const float by_split = whole && whole < m ? fp8_cost(FP8_PAIR[wide], whole, n, kb, cus) + small(m - whole) : 1e30f;
+  if (by_small <= by_pair && by_small <= by_split) return Fp8Plan{fp8_small_kind(m, n, kb, cus, wide), 0, m};
+  if (by_pair <= by_split) return Fp8Plan{PN_FP8_PAIR, 0, m};
+  return Fp8Plan{PN_FP8_PAIR, fp8_small_kind(m - whole, n, kb, cus, wide), whole};
+}
+
+template <bool WIDE> static int fp8_gemm_by_kind(int kind, const Fp8GemmArgs& a, hipStream_t s) {
+  switch (kind) {
+    case PN_FP8_TILE_64: return fp8_tile<64, 64, 2, 2, 2, WIDE>(a, s);
+    case PN_FP8_TILE_128: return fp8_tile<128, 128, 2, 2, 2, WIDE>(a, s);
+    case PN_FP8_PAIR: return fp8_pair<WIDE>(a, s);
+    default: return fp8_direct_by_kind<Fp8Laid>(kind, Fp8DirectArgs{a, nullptr, 0, a.kblocks * 128}, s);
+  }
+}
+template <bool WIDE> static int fp8_gemm_by_size(Fp8GemmArgs a, hipStream_t s) {
+  const Fp8Plan plan = fp8_plan(a.M, a.N, a.kblocks, WIDE);
   Fp8GemmArgs t = a;
-  a.M = whole;
-  t.M -= whole;
-  t.x += (size_t)(whole / 16) * kb * 2048;
-  t.xs += whole;
-  t.out = (char*)t.out + whole * t.ldo * (WIDE ? 4 : 2);
-  const int rc = fp8_pair<WIDE>(a, s);
-  return rc != PN_OK ? rc : fp8_small<WIDE>(t, cus, s);
+  a.M = plan.rows;
+  const int rc = fp8_gemm_by_kind<WIDE>(plan.kind, a, s);
+  if (rc != PN_OK || !plan.rest) return rc;
+  t.M -= plan.rows;
+  t.x += (size_t)(plan.rows / 16) * a.kblocks * 2048;
+  t.xs += plan.rows;
+  t.out = (char*)t.out + plan.rows * t.ldo * (WIDE ? 4 : 2);
+  return fp8_gemm_by_kind<WIDE>(plan.rest, t, s);
 }
 
 int fp8_gemm_launch(const Fp8Gemm& g, hipStream_t s) {
@@ -875,6 +889,14 @@ extern "C" int pn_fp8_gemm(const void* x, long long m, const void* w, int n, int
 // With half as many, 16 x 32: 500 x 3136 x 256 7.7 us against 9.0, 1000 x 3136 x 256 13.5 against 9.2.
 static bool fp8_is_direct(long long m, int n, int k) { return k >= 128 && (m + 15) / 16 * ((n + 63) / 64) <= 256; }
 
+extern "C" int pn_fp8_kernels(long long m, int n, int k, int out_dtype, int laid_out) {
+  PN_CHECK_ARG(m >= 1 && n >= 1 && k >= 1 && (out_dtype == PN_DTYPE_F32 || out_dtype == PN_DTYPE_BF16), "pn_fp8_kernels: %lld x %d x %d, type %d", m, n, k,
+               out_dtype);
+  if (!laid_out && fp8_is_direct(m, n, k)) return fp8_direct_kind(m, n);
+  const Fp8Plan plan = fp8_plan(m, n, (k + 127) / 128, out_dtype == PN_DTYPE_F32);
+  return plan.kind | plan.rest << 4;
+}
+
 extern "C" size_t pn_fp8_linear_workspace_bytes(long long m, int n, int k) {
   return m < 1 || n < 1 || k < 1 || fp8_is_direct(m, n, k) ? 0 : fp8_bytes(m, k);
 }
@@ -889,7 +911,8 @@ extern "C" int pn_fp8_linear(int dtype, const void* x, long long m, long long ld
   if (fp8_is_direct(m, n, k)) {
     Fp8DirectArgs d = {{nullptr, (const unsigned char*)w, nullptr, fp8_operand(w, n, k).scale, m, m, n, (k + 127) / 128, (k + 511) / 512, 0, 0,
                         bias, bias_dtype, act, out_dtype, out, ldo}, x, m == 1 ? 0 : ldx, k};
-    return dtype == PN_DTYPE_F32 ? fp8_direct_by_size<float>(d, s) : fp8_direct_by_size<__bf16>(d, s);
+    const int kind = fp8_direct_kind(m, n);
+    return dtype == PN_DTYPE_F32 ? fp8_direct_by_kind<float>(kind, d, s) : fp8_direct_by_kind<__bf16>(kind, d, s);
   }
   if (ws_bytes < fp8_bytes(m, k) || !ws) {
     pn_set_error("pn_fp8_linear: workspace of %zu bytes is too small", ws_bytes);

@@ -178,6 +178,23 @@ def test_more_elements_than_a_launch_takes_are_refused():
         assert b"more than one launch takes" in L.pn_last_error()
 
 
+def test_product_cases_take_every_kernel():
+    """the sizes that products are tested at on the GPU reach every kernel, also after the rules by size have moved."""
+    import fp8_product_cases as pc
+    L = _lib.lib()
+    for (m, k, n), out, laid, kind, rest in pc.CASES:
+        got = L.pn_fp8_kernels(m, n, k, out, laid)
+        assert (got & 15, got >> 4) == (kind, rest), ((m, k, n), out, laid, got)
+    for (m, k, n), dtype, kinds in pc.TRAIN:
+        assert tuple(L.pn_fp8_kernels(*q, 1) for q in pc.products(m, k, n, dtype)) == kinds
+    taken = {(out, laid or kind not in (pc.D32, pc.D64), kind) for _, out, laid, kind, _ in pc.CASES}
+    assert taken >= {(o, True, kind) for o in (pc.F32, pc.BF16) for kind in (pc.D32, pc.D64, pc.T64, pc.T128, pc.PAIR)}
+    assert taken >= {(o, False, kind) for o in (pc.F32, pc.BF16) for kind in (pc.D32, pc.D64)}
+    assert {(out, rest) for _, out, _, _, rest in pc.CASES} >= {(o, r) for o in (pc.F32, pc.BF16) for r in (pc.D32, pc.D64, pc.T64)}
+    for bad in ((0, 1, 1, 0), (1, 0, 1, 0), (1, 1, 0, 0), (1, 1, 1, 7)):
+        assert L.pn_fp8_kernels(*bad, 1) == -1
+
+
 def test_struct_layout_matches_header():
     assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers
 

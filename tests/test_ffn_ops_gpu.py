@@ -18,8 +18,9 @@ import numpy as np
 import pytest
 import torch
 
+import fp8_product_cases as pc
 from oracle import ffn_oracle as fo
-from pillarnet_lts_amd import ffn_ops
+from pillarnet_lts_amd import _lib, ffn_ops
 from pillarnet_lts_amd._lib import PillarnetHipError
 
 pytestmark = pytest.mark.gpu
@@ -602,6 +603,65 @@ def test_fp8_linear_train(cuda, dtype, wdtype, M, K, N, bias):
     if bias:
         want = d(g).sum(0)
         within(db[0], want, U32 * np.abs(want) + (M + 8) * U32 * np.abs(d(g)).sum(0), "db")
+
+
+def _whole(gen, R, C, step, cuda):
+    """[R, C] of whole numbers up to 8 times a power of two for each row and, by 2^(+-block % 3), each block of 128 columns: e4m3 holds
+    them exactly, and products of two such operands with opposite steps are whole numbers times their rows' powers."""
+    v = torch.randint(-8, 9, (R, C), generator=gen, device=cuda).float()
+    return v * torch.exp2(step * (torch.arange(C, device=cuda) // 128 % 3).float())
+
+
+@pytest.mark.parametrize("case", pc.CASES, ids=lambda c: "x".join(map(str, c[0])) + ("-fp32" if c[1] == pc.F32 else "-bf16") + ("-laid" if c[2] else ""))
+def test_fp8_products_of_every_kernel_are_exact(large, cuda, case):
+    """Whole numbers: partial sums stay below 5129 * 64 * 2^3 * 2^2 < 2^24 steps of the smallest power, so fp32 results are exact in any
+    order of the sums, and bf16 ones are rounded once (all products of an instruction lie within its 16 bits)."""
+    (M, K, N), out, laid, kind, rest = case
+    got = _lib.lib().pn_fp8_kernels(M, N, K, out, laid)
+    assert (got & 15, got >> 4) == (kind, rest)
+    dtype = torch.float32 if out == pc.F32 else torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(M + N)
+    x = _whole(gen, M, K, 1, cuda) * torch.exp2(torch.randint(-2, 3, (M, 1), generator=gen, device=cuda).float())
+    w = _whole(gen, N, K, -1, cuda) * torch.exp2((torch.arange(N, device=cuda) // 128 % 2).float())[:, None]
+    b = torch.randint(-4, 5, (N,), generator=gen, device=cuda).float()
+    want = x.double() @ w.double().t() + b.double()
+    x = x.to(dtype)
+    if laid:
+        y = ffn_ops.fp8_matmul(ffn_ops.fp8_quantize(x)[0], ffn_ops.fp8_quantize(w, 128)[0], b, out_dtype=dtype)
+    else:
+        y = ffn_ops.fp8_linear(x, ffn_ops.Fp8Weight(w, b))
+    assert y.dtype == dtype and torch.equal(y, want.to(torch.float32).to(dtype))
+    plan = ffn_ops.Fp8Weight(w)                                                  # the public entry, ReLU in the epilogue, no bias
+    assert torch.equal(ffn_ops.fp8_linear(x, plan, "relu"), (want - b.double()).relu().to(torch.float32).to(dtype))
+
+
+@pytest.mark.parametrize("case", pc.TRAIN, ids=lambda c: "x".join(map(str, c[0])) + ("-fp32" if c[1] == pc.F32 else "-bf16"))
+def test_fp8_training_products_of_every_kernel_are_exact(large, cuda, case):
+    (M, K, N), out, kinds = case
+    assert tuple(_lib.lib().pn_fp8_kernels(*q, 1) for q in pc.products(M, K, N, out)) == kinds
+    dtype = torch.float32 if out == pc.F32 else torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    whole = lambda *s: torch.randint(-8, 9, s, generator=gen, device=cuda).float()
+    x, w, g = whole(M, K).to(dtype).requires_grad_(), whole(N, K).requires_grad_(), whole(M, N).to(dtype)
+    b = whole(N).requires_grad_()
+    y = ffn_ops.fp8_linear_train(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    X, W, G = (t.detach().double() for t in (x, w, g))
+    assert torch.equal(y, (X @ W.t() + b.double()).float().to(dtype))           # sums below 6314 * 64 < 2^19
+    assert torch.equal(dx, (G @ W).float().to(dtype))
+    assert torch.equal(dw, (G.t() @ X).float()) and torch.equal(db, G.sum(0).float())
+
+
+def test_fp8_matmul_refusals(cuda):
+    x, w = (ffn_ops.fp8_quantize(torch.randn(*s, device=cuda))[0] for s in ((6, 64), (32, 64)))
+    assert ffn_ops.fp8_matmul(x, w).shape == (6, 32)
+    assert ffn_ops.fp8_matmul(ffn_ops.fp8_quantize(torch.zeros(0, 64, device=cuda))[0], w).shape == (0, 32)
+    b = torch.zeros(32, device=cuda)
+    for call in (lambda: ffn_ops.fp8_matmul(torch.zeros(6, 64, device=cuda), w), lambda: ffn_ops.fp8_matmul(x, ffn_ops.fp8_quantize(torch.zeros(32, 65, device=cuda))[0]),
+                 lambda: ffn_ops.fp8_matmul(x, w, b[:5]), lambda: ffn_ops.fp8_matmul(x, w, b.cpu()), lambda: ffn_ops.fp8_matmul(x, w, act="silu"),
+                 lambda: ffn_ops.fp8_matmul(x, w, out_dtype=torch.float16)):
+        with pytest.raises(PillarnetHipError):
+            call()
 
 
 def test_fp8_linear_train_gradient_against_differences(cuda):
