@@ -302,6 +302,14 @@ def test_residual_norm_widths(cuda, dtype, C):
     _join_run(cuda, dtype, dtype, 2, 37, C, "rms", "layer", "channel", 0.1, True)
 
 
+@BOTH
+@pytest.mark.parametrize("C", [7, 64, 120, 250, 512, 1001, 1024, 2048, 2104, 3000, 4096, 4200, 8192, 9000, 16384])
+def test_residual_norm_widths_without_post_norm_and_dropout(cuda, dtype, C):
+    """the kernels for a gate alone, and for no branch."""
+    _join_run(cuda, dtype, dtype, 2, 23, C, None, "rms", "channel", 0.0, True)
+    _join_run(cuda, dtype, dtype, 1, 29, C, None, "layer", None, 0.0, False, act="relu")
+
+
 @pytest.mark.parametrize("C", [1031, 1536, 4100, 5001, 8192, 9000])
 def test_residual_norm_wide_rows_with_wider_parameters(cuda, C):
     """bf16 rows, fp32 parameters, workgroups of the row's size: odd and whole widths on either side of their limits."""
