@@ -122,9 +122,23 @@ def roi_grid_pool_torch(rois, feature_map, grid, cell_size, x_min, y_min):
     return out.view(B, R, grid * grid, C), pts
 
 
-# weights laid out for fp8 products (PLANS holds the same modules' fp32 plans), anew where a weight was written in place or its
-# storage replaced
-FP8_PLANS = dense_hip.PlanCache(lambda m: (dense_hip.params_version(m), tuple(p.data_ptr() for p in m.parameters())))
+class Fp8Plans(dense_hip.PlanCache):
+    """Weights laid out for fp8 products (PLANS holds the same modules' fp32 plans), anew where a parameter or buffer was written in
+    place or its storage replaced.  An entry keeps the storages that it was made of: while it lives, no other tensor has their
+    addresses."""
+
+    @staticmethod
+    def _tensors(m):
+        return [*m.parameters(), *m.buffers()]
+
+    def __init__(self):
+        super().__init__(lambda m: (dense_hip.params_version(m), tuple(t.data_ptr() for t in self._tensors(m))))
+
+    def get(self, module, builder):
+        return super().get(module, lambda m: (builder(m), [t.detach() for t in self._tensors(m)]))[0]
+
+
+FP8_PLANS = Fp8Plans()
 
 
 class FoldedMLP:

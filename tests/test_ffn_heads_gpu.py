@@ -161,6 +161,25 @@ def test_fp8_evaluation_with_gradients_enabled(cuda):
     assert all(torch.isfinite(q).all() for q in grads) and grads[0].abs().sum() > 0
 
 
+def test_fp8_plans_follow_replaced_storages(cuda):
+    """a weight that moves into a storage at the address that its old one gave back is laid out anew; so is one behind a replaced
+    running mean."""
+    head = second_stage.RoIHeadTemplate(1, {}).to(cuda).eval()
+    head.fp8 = True
+    fc, x = torch.nn.Linear(512, 512, bias=False).to(cuda), torch.ones(4, 512, device=cuda)
+    with torch.no_grad():
+        for k in range(4):
+            fc.weight.data = torch.zeros(1, device=cuda)
+            fc.weight.data = torch.full((512, 512), 2.0 ** k, device=cuda)
+            assert (head.fused_linear(fc, x) == 512 * 2.0 ** k).all(), k
+        head, batch, _ = _mix_head(cuda, fp8=True)
+        head.eval()
+        bn = head.shared_fc_layer[1]
+        old = head(dict(batch), training=False)["batch_cls_preds"]
+        bn.running_mean = bn.running_mean + 0.5
+        assert not torch.equal(old, head(dict(batch), training=False)["batch_cls_preds"])
+
+
 def test_heads_refuse_host_tensors_when_fused():
     from pillarnet_lts_amd._lib import PillarnetHipError
     head = second_stage.RoIFFNHead(model_cfg=ConfigDict(CFG), feedforward_channels=48, content_dim=32, fused_ops=True)

@@ -199,6 +199,25 @@ def test_struct_layout_matches_header():
     assert ctypes.sizeof(_lib.pnResidualNorm) == 6 * 4 + 4 * 8 + 5 * 4 + 4 + 8 * 8      # 4 bytes of padding before the pointers
 
 
+def test_fp8_plans_follow_replaced_storages():
+    """a plan is made anew when a parameter or a buffer gets another storage, also one that a freed storage's address went to."""
+    from pillarnet_lts_amd import second_stage
+    m = torch.nn.Sequential(torch.nn.Linear(512, 512), torch.nn.BatchNorm1d(512))
+    plan = lambda: second_stage.FP8_PLANS.get(m, lambda m: object())
+    a = plan()
+    assert plan() is a
+    m[1].running_mean = torch.ones(512)
+    b = plan()
+    assert b is not a and plan() is b
+    for _ in range(8):
+        before = plan()
+        m[0].weight.data = torch.zeros(1)
+        m[0].weight.data = torch.ones(512, 512)         # where the allocator finds a megabyte: the place just freed, as a rule
+        assert plan() is not before
+    m[1].running_var.add_(1)
+    assert plan() is not before
+
+
 def test_a_head_without_a_fused_path_says_so():
     from pillarnet_lts_amd import legacy
     head = legacy.RoIHead(16, dict(SHARED_FC=[8], CLS_FC=[8], REG_FC=[8], DP_RATIO=0.0))
