@@ -1091,9 +1091,9 @@ class PillarRCNN(BaseDetector):
 
     def to_inference(self, dtype=torch.bfloat16, device="cuda", dense_backend="hip", roi_fp8=False):
         """roi_fp8: the RoI head's layers as products in fp8 with block scales (RoIHeadTemplate.use_fused)."""
+        if roi_fp8:                # (refuses a head without the path before anything is converted)
+            self.roi_head.use_fused(fp8=True, dropout_seed=self.roi_head.dropout_seed)
         self.single_det.to_inference(dtype, device, dense_backend)
-        if roi_fp8:
-            self.roi_head.use_fused(fp8=True)
         self.eval().to(device)
         for m in list(self.second_stage) + [self.point_head, self.roi_head]:
             if m is not None:

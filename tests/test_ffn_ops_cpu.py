@@ -225,3 +225,14 @@ def test_a_head_without_a_fused_path_says_so():
         with pytest.raises(PillarnetHipError, match="RoIHead has no fused path"):
             head.use_fused(**kw)
     assert head.use_fused(False) is head and not head.fused_ops
+
+
+def test_to_inference_refuses_a_head_without_fp8_before_it_converts():
+    from types import SimpleNamespace
+    from pillarnet_lts_amd import legacy, second_stage
+    converted = []
+    stage = SimpleNamespace(to_inference=lambda *a: converted.append(a))
+    head = legacy.RoIHead(16, dict(SHARED_FC=[8], CLS_FC=[8], REG_FC=[8], DP_RATIO=0.0))
+    with pytest.raises(PillarnetHipError, match="no fused path"):
+        second_stage.PillarRCNN.to_inference(SimpleNamespace(single_det=stage, roi_head=head), roi_fp8=True)
+    assert not converted
