@@ -130,6 +130,7 @@ class DropoutState:
         _require(self.state.device.type == "cuda", "DropoutState: the state must live on the GPU (no CPU fallback)")
 
     def draw(self):
+        _require(torch._C._current_graph_task_id() == -1, "DropoutState: no draw inside a backward pass (draw outside of what is checkpointed)")
         used = torch.empty_like(self.state)
         _call("pn_dropout_draw", self.state.device, self.state.data_ptr(), used.data_ptr())
         return used

@@ -635,7 +635,7 @@ class RoIHeadTemplate(nn.Module):
         counter-based generator of their own instead of torch's: other masks, the same distribution).  fp8 (implies fused_ops):
         its Linear / 1x1 layers too, as products in e4m3 with block scales, forward and backward.  dropout_seed: the
         generator's seed (default torch.initial_seed(); data-parallel ranks add their rank); its offset starts at 0 and is no part
-        of the state dict, so a resumed run takes another seed."""
+        of the state dict, so a resumed run takes another seed.  A head that drops is not checkpointed as a whole (DropoutState)."""
         if (fused_ops or fp8) and not self.HAS_FUSED:
             raise _lib.PillarnetHipError(f"{type(self).__name__} has no fused path")
         self.fused_ops, self.fp8, self.dropout_seed, self._dropout_state = bool(fused_ops or fp8), bool(fp8), dropout_seed, None

@@ -872,3 +872,17 @@ def test_a_refusal_in_a_backward_pass_is_the_frameworks_error(cuda):
             torch.autograd.grad(z.sum(), x)
     assert torch.isfinite(torch.autograd.grad(ffn_ops.fp8_linear_train(x, w).sum(), x)[0]).all()
 
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_draw_inside_a_recomputed_pass_is_refused(cuda, reentrant):
+    """it would drop other elements than the pass whose gradient is asked for; drawn outside, checkpointing gives the plain gradient."""
+    from torch.utils.checkpoint import checkpoint
+    st, x = ffn_ops.DropoutState(3, cuda), torch.randn(8, 64, device=cuda, requires_grad=True)
+    y = checkpoint(lambda x: ffn_ops.act_dropout(x, 0.5, st.draw(), act="gelu").square(), x, use_reentrant=reentrant)
+    with pytest.raises(PillarnetHipError, match="inside a backward pass"):
+        y.sum().backward()
+    rng = st.draw()
+    block = lambda x: ffn_ops.act_dropout(x, 0.5, rng, act="gelu").square()
+    x.grad = None
+    checkpoint(block, x, use_reentrant=reentrant).sum().backward()
+    assert torch.equal(x.grad, torch.autograd.grad(block(x).sum(), x)[0])
