@@ -8,7 +8,8 @@
 //
 // Bound by memory.  A thread takes eight elements, what one run of the generator decides and 16 bytes of bf16: 65536 x 2048 bf16
 // with ReLU, p = 0.1: forward 85 us (6.3 TB/s), backward 142 us (5.7 TB/s).  In fp32 with GELU (6271 x 1023: 13 and 17 us, 4 and
-// 4.5 TB/s) the generator's 40 integer multiplies and the fitted tail are about half the cycles.
+// 4.5 TB/s) the generator's 40 integer multiplies and the fitted tail are about half the cycles.  Strided rows take a 64-bit division a
+// piece, and in fp32 16 - 24 bytes of scratch a lane (load8_view's elements).
 #include "ffn_common.h"
 
 struct DropArgs {

@@ -8,10 +8,21 @@
 //
 // Bound by memory, with the next row on its way while one is worked on: 32768 x 4096 bf16, layer scale and LayerNorm, 199 us
 // (5.4 TB/s); 65536 x 256 fp32, LayerNorm, 42 us (6.4 TB/s).  With both norms, gate and dropout (16 x 1031 x 2048 bf16: forward
-// 58 us, 4.6 TB/s; backward 92 us, 4.4 TB/s, and 6.6 for the column sums) the generator and two sums across each row leave too
-// few waves to hide all of it.  Slower than that: rows whose length is no multiple of eight (16 x 1031 x 2047: 77 and 135 us), rows
-// a little over a power of two (4096 x 4200 bf16, both norms: forward 61 us, 2.3 TB/s: one workgroup of twelve waves on a CU, nine of
-// them with columns), and training over 8192 columns, where registers spill (2048 x 16384 bf16, both norms: backward 0.8 ms).
+// 57 us, 4.8 TB/s; backward 91 us, 4.4 TB/s, and 7 for the column sums) the generator and two sums across each row leave too
+// few waves to hide all of it.  Slower than that: rows whose length is no multiple of eight (16 x 1031 x 2047: 78 and 124 us), and rows
+// a little over a power of two (4096 x 4200 bf16, both norms: forward 65 us, 2.1 TB/s: one workgroup of twelve waves on a CU, nine of
+// them with columns).
+//
+// Small launches (512 x 49 x 64 fp32, LayerNorm: 9 us forward and 10 backward for 26 MB each, 3 TB/s) are one pass of 784 workgroups: the
+// launch, one trip to memory there and one back, and nothing to hide them behind.
+//
+// Where registers do not suffice (bytes of scratch a lane as the compiler reports them):
+//   backward with a branch, 4097 - 8192 columns: 32 - 36 for bf16 rows with fp32 parameters, 100 - 116 for fp32 rows, none for bf16 with
+//     bf16 parameters (4096 x 8192, both norms: 131, 244 and 115 us; the rows are 403 MB in bf16);
+//   forward over 8192 columns, where 1024 threads have 128 registers for 16 columns each: 172 - 324 with post norm or dropout (2048 x
+//     16384, both norms: bf16 131 us, fp32 257), up to 100 without (LayerNorm: 59 and 153);
+//   backward over 8192 columns: 780 - 1108 with a branch that is read (bf16 761 us, fp32 1166: 0.5 - 0.7 TB/s), 276 - 408 otherwise (164, 302).
+// The backward kernel that reads the branch keeps five column sums whatever is asked for: with dropout or a gate alone it is hardly faster.
 #include "ffn_common.h"
 
 struct NormArgs {
@@ -267,7 +278,8 @@ __global__ __launch_bounds__(NT) void residual_norm_fwd_kernel(NormArgs a) {
 // order: no atomics, the same bits on every run.
 //
 // Rows over 4096 wide with a branch, 16 columns a thread (at eight, 1024 threads leave 128 registers each: the sums alone are 40,
-// and spilled ones wait for the next row's loads): the parameters wait in LDS, and no row is fetched ahead.
+// and spilled ones wait for the next row's loads): the parameters wait in LDS, and no row is fetched ahead.  Up to 8192 columns that
+// leaves little or no scratch; past them 1024 threads have 128 registers again.
 static constexpr __host__ __device__ bool bwd_parks(int L, int K, int NT, bool branch) { return branch && L == 0 && K == 2 && NT == 512; }
 static constexpr int NSUM_NORM = 2, NSUM_ALL = 5;      // weight, bias | post weight, post bias, gate
 

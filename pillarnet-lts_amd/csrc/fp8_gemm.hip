@@ -7,8 +7,9 @@
 // The instruction rounds the products of eight neighbouring k to 16 bits below the largest of them before it adds (measured with
 // single pairs of products: 1.4e-5 relative at worst).  That is far below a bf16 result's own rounding and far above an fp32
 // result's: for fp32 outputs (WIDE) the same bytes are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16.
-// Measured: 8192^3 398 - 436 us into bf16 (2.5 - 2.8 PFLOP/s), 865 - 944 into fp32 (1.2 - 1.3 PFLOP/s, the bf16 instruction's
-// own bound with the widening beside it); 16384 x 4096 x 8192 with bias and GELU 470 us; one row of 8192 x 8192 15 us (4.4 TB/s).
+// Measured (from card to card): 8192^3 386 - 436 us into bf16 (2.5 - 2.8 PFLOP/s), 836 - 944 into fp32 (1.2 - 1.3 PFLOP/s, the bf16
+// instruction's own bound with the widening beside it); 16384 x 4096 x 8192 with bias and GELU 455 - 470 us; one row of 8192 x 8192 15 us
+// (4.4 TB/s).
 #include "ffn_common.h"
 #include <type_traits>
 
@@ -501,7 +502,8 @@ __global__ __launch_bounds__(512) void fp8_pair_kernel(Fp8GemmArgs a) {
 
 // Few rows (one row at the least): a workgroup owns 16 rows and FN * 16 columns, its waves deal the blocks of 128 among
 // themselves and add up through LDS at the end.  The rows of x come as they are and are laid out on the way, a block at a time,
-// through 2 KB of LDS of the wave's own: one launch, and no bytes of x in memory.  What bounds it is the weights' read.
+// through 2 KB of LDS of the wave's own: one launch, and no bytes of x in memory.  What bounds it is the weights' read.  (fp32 rows into
+// fp32 results with 64 columns take all 256 registers and 12 bytes of scratch a lane.)
 struct Fp8DirectArgs {
   Fp8GemmArgs g;
   const void* x;             // [M][ldx] fp32 or bf16
