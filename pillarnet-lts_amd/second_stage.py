@@ -9,6 +9,8 @@ head stay torch ops.  Training: ProposalTargetLayer (HIP rotated 3-D IoU, the re
 RoI class / box losses, the PointHead's grid-point targets (`pn_points_in_boxes_2d`) and focal loss, and
 `combine_loss`; the pooled features are differentiable through a torch expression of the same bilinear
 weights (`roi_grid_pool` itself is forward-only)."""
+import weakref
+
 import numpy as np
 import torch
 import torch.nn as nn
@@ -125,7 +127,7 @@ def roi_grid_pool_torch(rois, feature_map, grid, cell_size, x_min, y_min):
 class Fp8Plans(dense_hip.PlanCache):
     """Weights laid out for fp8 products (PLANS holds the same modules' fp32 plans), anew where a parameter or buffer was written in
     place or its storage replaced.  An entry keeps the storages that it was made of: while it lives, no other tensor has their
-    addresses."""
+    addresses.  It goes with its module."""
 
     @staticmethod
     def _tensors(m):
@@ -135,6 +137,9 @@ class Fp8Plans(dense_hip.PlanCache):
         super().__init__(lambda m: (dense_hip.params_version(m), tuple(t.data_ptr() for t in self._tensors(m))))
 
     def get(self, module, builder):
+        key = id(module)
+        if key not in self._d:
+            weakref.finalize(module, lambda: self._d.pop(key, None)).atexit = False
         return super().get(module, lambda m: (builder(m), [t.detach() for t in self._tensors(m)]))[0]
 
 

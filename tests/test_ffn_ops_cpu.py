@@ -218,6 +218,21 @@ def test_fp8_plans_follow_replaced_storages():
     assert plan() is not before
 
 
+def test_fp8_plans_go_with_their_modules():
+    import gc
+    import weakref
+    from pillarnet_lts_amd import second_stage
+    m = torch.nn.Linear(8, 8)
+    for k in range(3):
+        m.weight.data = torch.full((8, 8), float(k))
+        second_stage.FP8_PLANS.get(m, lambda m: object())
+    key, gone = id(m), weakref.ref(m)
+    assert key in second_stage.FP8_PLANS._d
+    del m
+    gc.collect()
+    assert gone() is None and key not in second_stage.FP8_PLANS._d
+
+
 def test_a_head_without_a_fused_path_says_so():
     from pillarnet_lts_amd import legacy
     head = legacy.RoIHead(16, dict(SHARED_FC=[8], CLS_FC=[8], REG_FC=[8], DP_RATIO=0.0))
