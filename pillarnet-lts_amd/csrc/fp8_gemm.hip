@@ -6,7 +6,8 @@
 //
 // The instruction rounds the products of eight neighbouring k to 16 bits below the largest of them before it adds (measured with
 // single pairs of products: 1.4e-5 relative at worst).  That is far below a bf16 result's own rounding and far above an fp32
-// result's: for fp32 outputs (WIDE) the same bytes are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16.
+// result's: for fp32 outputs (WIDE) the same bytes are widened to bf16 and multiplied by v_mfma_f32_16x16x32_bf16.  That is exact down
+// to bf16's smallest step, 2^-133: in blocks of an exponent below -124 (no element over 1.1e-35) a value may be off by half of that.
 // Measured (from card to card): 8192^3 386 - 436 us into bf16 (2.5 - 2.8 PFLOP/s), 836 - 944 into fp32 (1.2 - 1.3 PFLOP/s, the bf16
 // instruction's own bound with the widening beside it); 16384 x 4096 x 8192 with bias and GELU 455 - 470 us; one row of 8192 x 8192 15 us
 // (4.4 TB/s).
@@ -36,7 +37,7 @@ __device__ __forceinline__ fp8_f32x4 mfma_fp8(i32x8 a, i32x8 b, fp8_f32x4 c, uin
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }
 
-// eight bytes widened to bf16 and multiplied by their block's scale, both exact
+// eight bytes widened to bf16 and multiplied by their block's scale, both exact down to 2^-133
 __device__ __forceinline__ fp8_bf16x8 widen8(int lo, int hi, float scale) {
   const fp8_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
   const fp8_bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);

@@ -660,6 +660,25 @@ def test_fp8_training_products_of_every_kernel_are_exact(large, cuda, case):
     assert torch.equal(dw, (G.t() @ X).float()) and torch.equal(db, G.sum(0).float())
 
 
+@pytest.mark.parametrize("M,K,N", [(8, 384, 64), (300, 90, 300), (2104, 1160, 69), (2312, 1160, 2312)])
+@pytest.mark.parametrize("k", [100, 124, 126, 130, 135])
+def test_fp8_products_of_tiny_rows(cuda, M, K, N, k):
+    """rows down to fp32's smallest normal numbers, on every kind of kernel: a bf16 result is what it is at any scale, an fp32 result is off by
+    half of bf16's smallest step, 2^-134, for each value of x beyond its sums' rounding."""
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    x, w = _whole(gen, M, K, 0, cuda), _whole(gen, N, K, 0, cuda)
+    x[:, ::5] *= 2.0 ** -9
+    x[:, ::7] *= 56
+    x = (x.double() * 2.0 ** -k).float()
+    xq, W = ffn_ops.fp8_quantize(x)[0].values().double(), w.double()
+    want, mags = xq @ W.t(), xq.abs() @ W.abs().t()
+    plan = ffn_ops.Fp8Weight(w)
+    y = ffn_ops.fp8_linear(x, plan)
+    assert ((y.double() - want).abs() <= 2 * K * U32 * mags + 2.0 ** -134 * W.abs().sum(1) + 2.0 ** -149).all()
+    y = ffn_ops.fp8_linear(x, plan, out_dtype=torch.bfloat16)
+    assert ((y.double() - want).abs() <= (2 * K * U32 + 7 * 2.0 ** -16) * mags + U[torch.bfloat16] * want.abs() + 2.0 ** -134).all()
+
+
 def test_fp8_matmul_refusals(cuda):
     x, w = (ffn_ops.fp8_quantize(torch.randn(*s, device=cuda))[0] for s in ((6, 64), (32, 64)))
     assert ffn_ops.fp8_matmul(x, w).shape == (6, 32)
